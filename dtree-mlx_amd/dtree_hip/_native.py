@@ -30,6 +30,9 @@ W_TILED = 1
 W_TILED_F16 = 3  # tiled fp16 weights + one fp16 activation plane
 W_Q4G64 = 2
 
+T_F32 = 0  # element types of row buffers
+T_BF16 = 1
+
 
 class DtreeError(RuntimeError):
     pass
@@ -110,6 +113,28 @@ class GdnArgs(C.Structure):
     ]
 
 
+class KvQ8(C.Structure):
+    _fields_ = [
+        ("k_pages", C.c_void_p), ("v_pages", C.c_void_p), ("k_scales", C.c_void_p), ("v_scales", C.c_void_p),
+        ("num_pages", C.c_int32), ("num_kv_heads", C.c_int32), ("head_dim", C.c_int32), ("num_seqs", C.c_int32),
+        ("page_tables", C.c_void_p), ("ld_page_table", C.c_int32),
+        ("max_past_length", C.c_int32), ("max_rows", C.c_int32), ("total_rows", C.c_int32),
+        ("past_lengths", C.c_void_p), ("row_counts", C.c_void_p), ("row_starts", C.c_void_p),
+    ]
+
+
+class AttnQ8Args(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("q_type", C.c_int32), ("ld_q", C.c_int32), ("q_stride", C.c_int32),
+        ("q_norm", C.c_void_p), ("eps", C.c_float),
+        ("rope_cos", C.c_void_p), ("rope_sin", C.c_void_p), ("rope_dims", C.c_int32),
+        ("ancestors", C.c_void_p), ("sink", C.c_int32), ("window", C.c_int32),
+        ("out", C.c_void_p), ("out_lo", C.c_void_p), ("ld_out", C.c_int32), ("out_layout", C.c_int32),
+        ("num_heads", C.c_int32), ("scale", C.c_float), ("gated", C.c_int32), ("rows_padded", C.c_int32),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
 _vp, _i32, _f32, _sz = C.c_void_p, C.c_int32, C.c_float, C.c_size_t
 
 # name -> (restype, argtypes)
@@ -167,6 +192,14 @@ SIGNATURES = {
     "dtree_gdn_layer_gated_norm": (C.c_int, [C.POINTER(GdnArgs), _vp]),
     "dtree_gdn_layer_commit": (C.c_int, [C.POINTER(GdnArgs), _vp]),
     "dtree_gdn_layer_chain": (C.c_int, [C.POINTER(GdnArgs), C.c_int32, _vp]),
+    "dtree_kv_q8_bytes": (_sz, []),
+    "dtree_attn_q8_args_bytes": (_sz, []),
+    "dtree_kv_q8_append": (C.c_int, [C.POINTER(KvQ8), _vp, _vp, _i32, _i32, _i32, _vp, _f32, _vp, _vp, _i32, _vp]),
+    "dtree_kv_q8_read": (C.c_int, [C.POINTER(KvQ8), _vp, _vp, _i32, _i32, _i32, _vp]),
+    "dtree_kv_q8_compact": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _vp, _i32, _vp, _i32, _vp,
+                                      _vp]),
+    "dtree_attention_q8_workspace_bytes": (_sz, [C.POINTER(KvQ8), C.POINTER(AttnQ8Args)]),
+    "dtree_attention_q8": (C.c_int, [C.POINTER(KvQ8), C.POINTER(AttnQ8Args), _vp]),
     "dtree_graph_begin": (C.c_int, [_vp]),
     "dtree_graph_end": (C.c_int, [_vp, C.POINTER(C.c_void_p)]),
     "dtree_graph_launch": (C.c_int, [_vp, _vp]),
@@ -193,7 +226,8 @@ def lib() -> C.CDLL:
     if h.dtree_abi_version() != ABI_VERSION:
         raise DtreeError("libdtree_hip.so ABI version mismatch; rebuild it")
     for fn, struct in (("dtree_step_desc_bytes", StepDesc), ("dtree_gemm_args_bytes", GemmArgs),
-                       ("dtree_attn_args_bytes", AttnArgs), ("dtree_gdn_args_bytes", GdnArgs)):
+                       ("dtree_attn_args_bytes", AttnArgs), ("dtree_gdn_args_bytes", GdnArgs),
+                       ("dtree_kv_q8_bytes", KvQ8), ("dtree_attn_q8_args_bytes", AttnQ8Args)):
         if getattr(h, fn)() != C.sizeof(struct):
             raise DtreeError(f"{struct.__name__} layout mismatch between Python and the library")
     _LIB = h

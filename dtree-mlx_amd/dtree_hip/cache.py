@@ -19,6 +19,7 @@ import functools
 
 import torch
 
+from . import _native as N
 from ._native import PAGE
 
 
@@ -146,6 +147,151 @@ class PagedKVCache:
         for pages, rows, which in ((self.k_pages[layer], keys, "k"), (self.v_pages[layer], values, "v")):
             off = _block_index(self.head_dim, which).to(dev)[slot].view(T, 1, self.head_dim)
             pages[page, head, off] = rows
+
+    def reset(self, offset: int = 0) -> None:
+        self.offset = offset
+
+
+# ---- 8-bit cache -------------------------------------------------------------------
+@functools.lru_cache(maxsize=None)
+def _block_index_q8(head_dim: int, which: str) -> torch.Tensor:
+    """[PAGE, head_dim] int64: byte offset of (slot, dim) inside a (page, kv head)
+    block of the 8-bit cache (q8_k_off / q8_v_off in csrc/kv_q8.h)."""
+    slot = torch.arange(PAGE).view(PAGE, 1)
+    d = torch.arange(head_dim).view(1, head_dim)
+    block = ((slot >> 5) * (head_dim >> 5) + (d >> 5)) * 64
+    if which == "k":
+        return ((block + ((d >> 4) & 1) * 32 + (slot & 31)) << 4) + (d & 15)
+    return ((block + ((slot >> 2) & 1) * 32 + (d & 31)) << 4) + (((slot >> 3) & 3) << 2) + (slot & 3)
+
+
+def quantise_q8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Rows [..., head_dim] as (int8, fp32 scale): scale = fp32(max |x| / 127),
+    the integer nearest to x / scale, ties to even (dtree_kv_q8_append's rule,
+    in 64 bits); a row that is not finite has scale NaN and zeros."""
+    x = x.double()
+    amax = x.abs().amax(-1)
+    fine = torch.isfinite(x).all(-1)
+    scale = torch.where(fine, amax / 127, torch.nan).float()
+    inv = torch.where(scale > 0, 1.0 / scale.double(), 0.0)
+    q = torch.where(fine[..., None], x, 0.0) * inv[..., None]
+    return torch.round(q).clamp_(-127, 127).to(torch.int8), scale
+
+
+class PagedKVCacheQ8:
+    """Paged KV cache in 8 bits: head_dim integers and one fp32 scale per
+    (position, kv head) row (DtreeKvQ8), for ``num_seqs`` sequences of up to
+    ``capacity`` positions each, which share the page pool.
+
+    k_pages, v_pages   [layers, n_pages, kv_heads, PAGE * head_dim] int8
+    k_scales, v_scales [layers, n_pages, kv_heads, PAGE] fp32
+    page_table         [num_seqs, pages] int32; -1 marks a page given away
+
+    ``offset`` is the committed length of a single sequence, as PagedKVCache's.
+    """
+
+    def __init__(self, layers: int, kv_heads: int, head_dim: int, capacity: int, num_seqs: int = 1, device="cuda",
+                 page_order: torch.Tensor | None = None):
+        if head_dim not in (64, 128, 256):
+            raise ValueError("head_dim must be 64, 128 or 256")
+        if capacity < 1 or num_seqs < 1:
+            raise ValueError("capacity and num_seqs must be positive")
+        self.layers, self.kv_heads, self.head_dim, self.num_seqs = layers, kv_heads, head_dim, num_seqs
+        pages = (capacity + PAGE - 1) // PAGE
+        self.capacity = pages * PAGE
+        self.n_pages = pages * num_seqs
+        dev = torch.device(device)
+        self.k_pages = torch.zeros(layers, self.n_pages, kv_heads, PAGE * head_dim, dtype=torch.int8, device=dev)
+        self.v_pages = torch.zeros_like(self.k_pages)
+        self.k_scales = torch.zeros(layers, self.n_pages, kv_heads, PAGE, dtype=torch.float32, device=dev)
+        self.v_scales = torch.zeros_like(self.k_scales)
+        if page_order is None:
+            page_order = torch.arange(self.n_pages, dtype=torch.int32)
+        if sorted(page_order.reshape(-1).tolist()) != list(range(self.n_pages)):
+            raise ValueError("page_order must be a permutation of the pages")
+        self.page_table = page_order.reshape(num_seqs, pages).to(device=dev, dtype=torch.int32).contiguous()
+        self.offset = 0
+
+    @property
+    def layer_stride(self) -> int:
+        return self.n_pages * self.kv_heads * PAGE * self.head_dim
+
+    def record(self, layer: int, past_lengths, row_counts, max_past_length: int, max_rows: int, total_rows: int,
+               row_starts=None) -> N.KvQ8:
+        """The layer and a batch's rows as the kernels take them. past_lengths,
+        row_counts and row_starts are device int32 arrays: tensors, which the record
+        keeps alive with the cache, or addresses."""
+        if not 0 <= layer < self.layers:
+            raise IndexError(layer)
+
+        def ptr(t):
+            if isinstance(t, torch.Tensor):
+                if t.dtype != torch.int32 or not t.is_contiguous() or t.device != self.k_pages.device:
+                    raise ValueError("past_lengths, row_counts and row_starts are contiguous int32 device tensors")
+                if t.numel() < self.num_seqs:
+                    raise ValueError("past_lengths, row_counts and row_starts have one entry per sequence")
+                return t.data_ptr()
+            return t
+
+        r = N.KvQ8()
+        rows = layer * self.n_pages * self.kv_heads * PAGE
+        r.k_pages = self.k_pages.data_ptr() + rows * self.head_dim
+        r.v_pages = self.v_pages.data_ptr() + rows * self.head_dim
+        r.k_scales = self.k_scales.data_ptr() + 4 * rows; r.v_scales = self.v_scales.data_ptr() + 4 * rows
+        r.num_pages = self.n_pages; r.num_kv_heads = self.kv_heads; r.head_dim = self.head_dim
+        r.num_seqs = self.num_seqs
+        r.page_tables = self.page_table.data_ptr(); r.ld_page_table = self.page_table.shape[1]
+        r.max_past_length = max_past_length; r.max_rows = max_rows; r.total_rows = total_rows
+        r.past_lengths = ptr(past_lengths); r.row_counts = ptr(row_counts); r.row_starts = ptr(row_starts)
+        r.keep = (self, past_lengths, row_counts, row_starts, self.page_table)
+        return r
+
+    def __len__(self) -> int:
+        return self.layers
+
+    def __getitem__(self, i: int) -> LayerCacheView:
+        if not 0 <= i < self.layers:
+            raise IndexError(i)
+        return LayerCacheView(self, i)
+
+    def __iter__(self):
+        return (LayerCacheView(self, i) for i in range(self.layers))
+
+    # ---- logical views (tests, checkers, cache import) -------------------
+    def _logical(self, pages: torch.Tensor, scales: torch.Tensor, T: int, seq: int, which: str) -> torch.Tensor:
+        n = (T + PAGE - 1) // PAGE
+        table = self.page_table[seq, :n].long()
+        idx = _block_index_q8(self.head_dim, which).to(pages.device).reshape(-1)
+        rows = pages[table][:, :, idx].view(n, self.kv_heads, PAGE, self.head_dim).float()
+        rows = rows * scales[table].unsqueeze(-1)
+        return rows.permute(0, 2, 1, 3).reshape(n * PAGE, self.kv_heads, self.head_dim)[:T]
+
+    def logical_keys(self, layer: int, length: int | None = None, seq: int = 0) -> torch.Tensor:
+        """[T, kv_heads, head_dim] fp32, logical order: the values the rows stand for."""
+        T = self.offset if length is None else length
+        return self._logical(self.k_pages[layer], self.k_scales[layer], T, seq, "k")
+
+    def logical_values(self, layer: int, length: int | None = None, seq: int = 0) -> torch.Tensor:
+        T = self.offset if length is None else length
+        return self._logical(self.v_pages[layer], self.v_scales[layer], T, seq, "v")
+
+    def write_logical(self, layer: int, keys: torch.Tensor, values: torch.Tensor, start: int = 0,
+                      seq: int = 0) -> None:
+        """Quantise [T, kv_heads, head_dim] rows into positions start..start+T-1."""
+        T = keys.shape[0]
+        if start + T > self.capacity:
+            raise ValueError("cache capacity exceeded")
+        dev = self.k_pages.device
+        pos = torch.arange(start, start + T, device=dev)
+        page = self.page_table[seq].long()[pos // PAGE]
+        slot = pos % PAGE
+        head = torch.arange(self.kv_heads, device=dev)
+        for pages, scales, rows, which in ((self.k_pages[layer], self.k_scales[layer], keys, "k"),
+                                           (self.v_pages[layer], self.v_scales[layer], values, "v")):
+            q, scale = quantise_q8(rows.to(dev))
+            off = _block_index_q8(self.head_dim, which).to(dev)[slot].view(T, 1, self.head_dim)
+            pages[page.view(T, 1, 1), head.view(1, -1, 1), off] = q
+            scales[page.view(T, 1), head.view(1, -1), slot.view(T, 1)] = scale
 
     def reset(self, offset: int = 0) -> None:
         self.offset = offset

@@ -568,6 +568,116 @@ int dtree_gdn_layers_commit(const DtreeGdnArgs* args, int32_t num_layers, hipStr
  * launches. */
 int dtree_gdn_layer_chain(const DtreeGdnArgs* args, int32_t num_tokens, hipStream_t stream);
 
+/*
+ * 8-bit paged KV cache of a batch of sequences: what make_cache
+ * (adapters.py:478-484) holds in bf16 for one sequence, in half the bytes and
+ * for several. A cached row (one position of one kv head, K or V) is head_dim
+ * integers q in [-127, 127] and one fp32 scale = fp32(max |x| / 127), q the
+ * integer nearest to x / scale (ties to even); it stands for q * scale. A row
+ * with an infinity or a NaN has scale NaN. K and V pages are
+ * [page][kv_head][DTREE_PAGE * head_dim] int8 blocks, the scales
+ * [page][kv_head][DTREE_PAGE] fp32. Element (slot s, dim d) of a block is
+ *   K: ((((s/32)*(head_dim/32) + d/32)*64 + ((d/16)%2)*32 + s%32) * 16) + d%16
+ *   V: ((((s/32)*(head_dim/32) + d/32)*64 + ((s/4)%2)*32 + d%32) * 16)
+ *        + ((s/8)%4)*4 + s%4
+ * (16 bytes of a lane's two 32x32x16 MFMA operands, a wavefront's load one
+ * contiguous kilobyte).
+ *
+ * The batch: sequence s has past_lengths[s] cached positions before its
+ * row_counts[s] new rows, which are rows row_starts[s] + r of the row buffers
+ * (row_starts NULL: s * max_rows + r) and positions past_lengths[s] + r.
+ * page_tables[s * ld_page_table + i] is the physical page of its positions
+ * 64 i .. 64 i + 63. The three arrays and the tables are device memory, so one
+ * captured graph serves every step; the host gives their bounds. The kernels
+ * keep to them whatever the device arrays hold: a sequence with a negative
+ * start or a past length outside [0, max_past_length] has no rows, rows end at
+ * max_rows, at total_rows and at the page table's last position, and a page
+ * outside [0, num_pages) is absent (nothing is written to it, its keys are
+ * masked, it reads as zeros), so pages that a window has passed can be given
+ * away (-1). Sequences may share pages
+ * that no call writes. Rows of the buffers that belong to no sequence are
+ * neither read nor written.
+ */
+#define DTREE_T_F32 0   /* element types of row buffers */
+#define DTREE_T_BF16 1
+typedef struct DtreeKvQ8 {
+  int8_t* k_pages; int8_t* v_pages;   /* 16-byte aligned */
+  float* k_scales; float* v_scales;   /* 16-byte aligned */
+  int32_t num_pages, num_kv_heads, head_dim;  /* head_dim 64, 128 or 256 */
+  int32_t num_seqs;
+  const int32_t* page_tables; int32_t ld_page_table;  /* pages of at least max_past_length positions */
+  int32_t max_past_length, max_rows, total_rows;
+  const int32_t* past_lengths; const int32_t* row_counts; const int32_t* row_starts;
+} DtreeKvQ8;
+
+/*
+ * New rows into the cache (the cache append of qwen3_tree.py:146 behind the
+ * k_norm and RoPE of :57-62): k and v point to kv head 0 of row 0, rows ld_k /
+ * ld_v elements apart, heads head_dim; `type` DTREE_T_F32 or DTREE_T_BF16, rows
+ * 16-byte aligned. K rows get the RMSNorm (k_norm bf16 [head_dim], NULL none)
+ * and the rotation of dims (i, i + rope_dims / 2) by row r's rope_cos / rope_sin
+ * [total_rows][rope_dims / 2] (rope_dims a multiple of 32, 0 none), all in 64
+ * bits up to the quantisation. No two sequences of a batch may write one page.
+ */
+int dtree_kv_q8_append(const DtreeKvQ8* kv, const void* k, const void* v, int32_t type, int32_t ld_k, int32_t ld_v,
+                       const uint16_t* k_norm, float eps, const float* rope_cos, const float* rope_sin,
+                       int32_t rope_dims, hipStream_t stream);
+/* Cached positions past_lengths[s] + r, r < row_counts[s], as rows of `type` (q *
+ * scale, rounded once): the inverse of dtree_kv_q8_append's writes. k or v may be
+ * NULL. */
+int dtree_kv_q8_read(const DtreeKvQ8* kv, void* k, void* v, int32_t type, int32_t ld_k, int32_t ld_v,
+                     hipStream_t stream);
+/* dtree_compact for the 8-bit cache of one sequence: `layers` layers whose page
+ * pools ([num_pages][num_kv_heads][...]) follow each other; page_table has
+ * `table_pages` entries. */
+int dtree_kv_q8_compact(const DtreeStepDesc* desc, int8_t* k_pages, int8_t* v_pages, float* k_scales, float* v_scales,
+                        int32_t layers, int32_t num_pages, int32_t num_kv_heads, int32_t head_dim,
+                        const int32_t* page_table, int32_t table_pages, const uint16_t* hidden_in,
+                        int32_t hidden_width, uint16_t* hidden_out, hipStream_t stream);
+
+/*
+ * Attention of a batch's new rows over its 8-bit cache, which holds their own
+ * keys and values already (dtree_kv_q8_append): grouped heads, softmax(scale * q
+ * k^T) v over the visible keys. Position p of a sequence sees key j iff j <= p
+ * and, with window > 0, j < sink or p - j < window. Single tokens, chunks and
+ * prompts (qwen3_tree.py:54-76, adapters.py:494-533), in one batch where they
+ * come together. With `ancestors` ([total_rows][DTREE_MASK_WORDS], as in
+ * DtreeStepDesc) new row r sees the cached prefix and new key j of its sequence
+ * iff bit j is set (a draft tree; max_rows <= DTREE_MAX_NODES, window 0).
+ * A row that sees no key gives zeros.
+ *
+ * q points to head 0 of row 0, rows ld_q and heads q_stride elements apart,
+ * q_norm and RoPE as for dtree_kv_q8_append's K. gated: elements head_dim ..
+ * 2 head_dim - 1 of a head gate its output by sigmoid (qwen35_tree.py:503-540).
+ * out: column h * head_dim + d of row r, layouts as for dtree_tree_attention.
+ * rows_padded > 0 (one sequence, row_starts NULL): rows row_counts[0] ..
+ * rows_padded - 1 of out become zero.
+ *
+ * The products run on fp16 MFMA: q and the softmax weights are rounded to fp16
+ * (11 bits, with exponents moved so that they keep them), the cached integers
+ * are exact in it; sums and statistics are fp32. Value scales below 2^-80 count
+ * as 2^-80.
+ * workspace: dtree_attention_q8_workspace_bytes (16-byte aligned, any contents)
+ * holds partial results of key ranges; calls that share one must not overlap.
+ * With less room, or none, fewer ranges are used.
+ */
+typedef struct DtreeAttnQ8Args {
+  const void* q; int32_t q_type, ld_q, q_stride;   /* rows and heads 16-byte aligned */
+  const uint16_t* q_norm; float eps;
+  const float* rope_cos; const float* rope_sin; int32_t rope_dims;
+  const uint32_t* ancestors;
+  int32_t sink, window;
+  uint16_t* out; uint16_t* out_lo; int32_t ld_out, out_layout;
+  int32_t num_heads; float scale;
+  int32_t gated, rows_padded;
+  void* workspace; size_t workspace_bytes;
+} DtreeAttnQ8Args;
+
+size_t dtree_kv_q8_bytes(void);         /* sizeof, for bindings */
+size_t dtree_attn_q8_args_bytes(void);
+size_t dtree_attention_q8_workspace_bytes(const DtreeKvQ8* kv, const DtreeAttnQ8Args* args);
+int dtree_attention_q8(const DtreeKvQ8* kv, const DtreeAttnQ8Args* args, hipStream_t stream);
+
 /* Convert a row-major [n][k] bf16 matrix to DTREE_W_TILED (n % 32 == 0,
  * k % 64 == 0; src and dst must not overlap). */
 int dtree_tile_weight(const uint16_t* src, uint16_t* dst, int32_t n, int32_t k, hipStream_t stream);
