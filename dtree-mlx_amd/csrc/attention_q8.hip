@@ -103,62 +103,58 @@ __device__ __forceinline__ void q8_load16(const AttnQ8Params& p, size_t at, floa
   }
 }
 
-// A lane's half (32-dim blocks J, dims 32 J + 16 h ..) of its pair's query:
-// q_norm, RoPE, the softmax scale in log2 units; 0 where the pair is none.
-// Returns the largest finite magnitude.
+// 16 norm weights / 16 table entries, at any address of their type.
+__device__ __forceinline__ void q8_weights16(const uint16_t* w, float (&x)[16]) {
+  u32x4_t v[2];
+  __builtin_memcpy(v, w, sizeof(v));
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const uint32_t b = v[i >> 3][(i >> 1) & 3];
+    x[i] = __uint_as_float((i & 1) ? (b & 0xffff0000u) : (b << 16));
+  }
+}
+__device__ __forceinline__ void q8_table16(const float* t, float (&x)[16]) { __builtin_memcpy(x, t, sizeof(x)); }
+
+// Chunk c (dims 16 c ..) of a row's query head: q_norm, RoPE, the softmax scale
+// in log2 units; the row's D / 16 chunks are neighbouring lanes. Every load comes
+// before the first use (the rotation's other chunk is loaded rather than
+// exchanged).
 template <int D>
-__device__ __forceinline__ float q8_query(const AttnQ8Params& p, bool live, size_t row, int head, int h,
-                                          float (&x)[D / 32][16]) {
-  constexpr int NB = D / 32;
-  float amax = 0.f;
-  if (!live) {
-#pragma unroll
-    for (int J = 0; J < NB; ++J)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) x[J][i] = 0.f;
-  }
+__device__ __forceinline__ void q8_query16(const AttnQ8Params& p, size_t row, int head, int c, float (&x)[16]) {
   const size_t base = row * p.a.ld_q + (size_t)head * p.a.q_stride;
-  float ss = 0.f;
-  if (live) {
-#pragma unroll
-    for (int J = 0; J < NB; ++J) {
-      q8_load16(p, base + 32 * J + 16 * h, x[J]);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) ss = fmaf(x[J][i], x[J][i], ss);
-    }
+  const int half = p.a.rope_dims / 2, hc = half / 16;  // the rotation's halves, hc chunks each
+  const bool turns = c < 2 * hc, low = c < hc, norm = p.a.q_norm != nullptr;
+  const int co = low ? c + hc : c - hc;
+  float o[16], w[16], wo[16], cs[16], sn[16];
+  q8_load16(p, base + 16 * c, x);
+  if (norm) q8_weights16(p.a.q_norm + 16 * c, w);
+  if (turns) {
+    q8_load16(p, base + 16 * co, o);
+    if (norm) q8_weights16(p.a.q_norm + 16 * co, wo);
+    const size_t at = row * half + 16 * (low ? c : co);
+    q8_table16(p.a.rope_cos + at, cs);
+    q8_table16(p.a.rope_sin + at, sn);
   }
-  ss += __shfl_xor(ss, 32);
-  if (!live) return 0.f;
-  const float rs = p.a.q_norm ? rsqrtf(ss * (1.0f / D) + p.a.eps) : 1.f;
-  const int half = p.a.rope_dims / 2, hc = half / 16;
+  float rs = 1.f;
+  if (norm) {
+    float ss = 0.f;
 #pragma unroll
-  for (int J = 0; J < NB; ++J) {
-    const int c = 2 * J + h;  // the 16-dim chunk
-    if (p.a.q_norm) {
+    for (int i = 0; i < 16; ++i) ss = fmaf(x[i], x[i], ss);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) x[J][i] *= rs * bf2f(p.a.q_norm[16 * c + i]);
-    }
-    if (c < 2 * hc) {  // the rotation's other half, loaded once more
-      const bool low = c < hc;
-      const int co = low ? c + hc : c - hc;
-      float o[16];
-      q8_load16(p, base + 16 * co, o);
-      const size_t at = row * half + 16 * (low ? c : co);
+    for (int k = 1; k < D / 16; k <<= 1) ss += __shfl_xor(ss, k);
+    rs = rsqrtf(ss * (1.0f / D) + p.a.eps);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        if (p.a.q_norm) o[i] *= rs * bf2f(p.a.q_norm[16 * co + i]);
-        const float cs = p.a.rope_cos[at + i], sn = p.a.rope_sin[at + i];
-        x[J][i] = low ? x[J][i] * cs - o[i] * sn : o[i] * sn + x[J][i] * cs;
-      }
-    }
+    for (int i = 0; i < 16; ++i) x[i] *= rs * w[i];
+  }
+  if (turns) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      x[J][i] *= p.scale_log2;
-      const float m = fabsf(x[J][i]);
-      amax = m < INFINITY ? fmaxf(amax, m) : amax;
+      const float y = norm ? o[i] * (rs * wo[i]) : o[i];
+      x[i] = low ? x[i] * cs[i] - y * sn[i] : y * sn[i] + x[i] * cs[i];
     }
   }
-  return amax;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) x[i] *= p.scale_log2;
 }
 
 // 2^e that takes amax into [2^13, 2^14), and its inverse.
@@ -169,14 +165,54 @@ __device__ __forceinline__ void q8_exponent(float amax, float& f, float& inv) {
   inv = __uint_as_float((uint32_t)(254 - ef) << 23);
 }
 
-template <int D>
-__device__ __forceinline__ void q8_pack(const float (&x)[D / 32][16], float f, u32x4_t (&q)[D / 16]) {
+// The queries of up to PAIRS pairs from pair0 on, in fp16 at qs[pair][D + 8]
+// (zeros past `pairs`), moved by one power of two for the workgroup; returns its
+// inverse. WAVES waves; the barriers wait for LDS alone.
+template <int D, int PAIRS, int WAVES>
+__device__ __forceinline__ float q8_queries(const AttnQ8Params& p, const Q8Seq& q, int g, int pair0, int pairs,
+                                            uint16_t* qs, float* wmax) {
+  constexpr int TPR = D / 16, NT = 64 * WAVES, NR = (PAIRS * TPR + NT - 1) / NT;
+  const int tid = threadIdx.x;
+  float x[NR][16], amax = 0.f;
 #pragma unroll
-  for (int J = 0; J < D / 32; ++J)
+  for (int k = 0; k < NR; ++k) {
+    const int u = tid + NT * k, m = pair0 + u / TPR;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < 16; ++i) x[k][i] = 0.f;
+    if (m < pairs && u < PAIRS * TPR) {
+      q8_query16<D>(p, (size_t)q.start + m / p.G, g * p.G + m % p.G, u % TPR, x[k]);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) q[2 * J + i][j] = pack_h2(x[J][8 * i + 2 * j] * f, x[J][8 * i + 2 * j + 1] * f);
+      for (int i = 0; i < 16; ++i) {
+        const float v = fabsf(x[k][i]);
+        amax = v < INFINITY ? fmaxf(amax, v) : amax;  // (what is not finite stays in its row)
+      }
+    }
+  }
+  amax = fmaxf(amax, dpp<0xB1>(amax));
+  amax = fmaxf(amax, dpp<0x4E>(amax));
+  amax = fmaxf(amax, dpp<0x141>(amax));
+  amax = fmaxf(amax, dpp<0x140>(amax));
+  amax = fmaxf(amax, swz_xor16(amax));
+  amax = fmaxf(amax, __shfl_xor(amax, 32));
+  if ((tid & 63) == 0) wmax[tid >> 6] = amax;
+  lds_barrier();
+#pragma unroll
+  for (int k = 0; k < WAVES; ++k) amax = fmaxf(amax, wmax[k]);
+  float f, inv;
+  q8_exponent(amax, f, inv);
+#pragma unroll
+  for (int k = 0; k < NR; ++k) {
+    const int u = tid + NT * k;
+    if (u < PAIRS * TPR) {
+      u32x4_t* o = reinterpret_cast<u32x4_t*>(qs + (u / TPR) * (D + 8) + 16 * (u % TPR));
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        o[j] = u32x4_t{pack_h2(x[k][8 * j] * f, x[k][8 * j + 1] * f), pack_h2(x[k][8 * j + 2] * f, x[k][8 * j + 3] * f),
+                       pack_h2(x[k][8 * j + 4] * f, x[k][8 * j + 5] * f), pack_h2(x[k][8 * j + 6] * f, x[k][8 * j + 7] * f)};
+    }
+  }
+  lds_barrier();
+  return inv;
 }
 
 // (ks, log2 vs, 1 / vs) of a key. A NaN reaches a row that sees the key through
@@ -193,27 +229,28 @@ struct Q8Mask {
   int pos;             // position; -1: the lane has no pair
   int sink, window;    // window 0: all
   bool tree;
-  int past, rows;                  // draft tree: the prefix, the sequence's rows
-  uint32_t a0, a1, a2, a3;         // and the lane's ancestor words (not an array: registers)
+  int past, rows;      // draft tree: the prefix, the sequence's rows,
+  const uint32_t* anc;  // and the pair's ancestor words in LDS
   __device__ __forceinline__ bool sees(int key) const {
     if (tree) {
-      const int n = key - past, i = n >> 5;
-      const uint32_t w = (i == 0 ? a0 : 0u) | (i == 1 ? a1 : 0u) | (i == 2 ? a2 : 0u) | (i == 3 ? a3 : 0u);
-      return pos >= 0 && (n < 0 || (n < rows && ((w >> (n & 31)) & 1u)));
+      const int n = key - past;
+      return pos >= 0 && (n < 0 || (n < rows && ((anc[(n >> 5) & 3] >> (n & 31)) & 1u)));
     }
     return key <= pos && (window == 0 || key < sink || pos - key < window);
   }
 };
-__device__ __forceinline__ Q8Mask q8_mask(const AttnQ8Params& p, const Q8Seq& q, bool live, int r) {
-  Q8Mask k{live ? q.past + r : -1, p.a.sink, p.a.window, p.a.ancestors != nullptr, q.past, q.n, 0, 0, 0, 0};
-  if (k.tree && live) {
-    const uint32_t* w = p.a.ancestors + ((size_t)q.start + r) * DTREE_MASK_WORDS;
-    k.a0 = w[0];
-    k.a1 = w[1];
-    k.a2 = w[2];
-    k.a3 = w[3];
+__device__ __forceinline__ Q8Mask q8_mask(const AttnQ8Params& p, const Q8Seq& q, bool live, int r, const uint32_t* anc) {
+  return Q8Mask{live ? q.past + r : -1, p.a.sink, p.a.window, p.a.ancestors != nullptr, q.past, q.n, anc};
+}
+// The ancestor words of pairs pair0 .. pair0 + n - 1 to LDS (a barrier follows).
+__device__ __forceinline__ void q8_ancestors(const AttnQ8Params& p, const Q8Seq& q, int pair0, int n, int pairs,
+                                             uint32_t (*anc)[DTREE_MASK_WORDS]) {
+  if (!p.a.ancestors) return;
+  for (int u = threadIdx.x; u < n * DTREE_MASK_WORDS; u += blockDim.x) {
+    const int m = pair0 + u / DTREE_MASK_WORDS, w = u % DTREE_MASK_WORDS;
+    anc[u / DTREE_MASK_WORDS][w] =
+        m < pairs ? p.a.ancestors[((size_t)q.start + m / p.G) * DTREE_MASK_WORDS + w] : 0u;
   }
-  return k;
 }
 
 // One 32-key block: the logits' statistics and weights of a lane's 16 keys
@@ -304,19 +341,38 @@ __device__ __forceinline__ void q8_emit(const AttnQ8Params& p, bool split, int p
   q8_store(p, row, head, d, y);
 }
 
-// A workgroup: one KV head's 32 pairs of a sequence (all it has) over one key
-// range, its pages dealt to the four waves in turn. A wave loads its keys
-// straight into registers, the next ones during the current ones (a page at a
-// time, half a page at head_dim 256, whose registers hold no more); the waves'
+__device__ __forceinline__ f32x4_t mfma16_f16(u32x4_t a, u32x4_t b, f32x4_t c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0,
+                                                0);
+}
+
+// A workgroup: all pairs of a sequence and KV head, up to 16 NC, over one key
+// range, its pages dealt to the four waves in turn. A wave loads its pages
+// straight into registers, the next one during the current one; the waves'
 // results meet in LDS.
-template <int D>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void q8_token_kernel(AttnQ8Params p) {
-  constexpr int NB = D / 32, BK = D == 256 ? 1 : 2, NL = BK * NB;  // 16-byte loads of K (or V) per lane and step
-  constexpr int SB = BK * 32 * D;                                  // bytes of a step's K (or V)
+//
+// 16 pairs are the columns of 16x16x32 products: half the softmax of 32 columns
+// that one decoded token leaves mostly empty. Lane 16 kq + c owns column c, and,
+// with kq = 2 b + h, a page's keys 32 b + 8 i + 4 h + e (i, e < 4). So
+// * S block i (accumulator e) has the key 32 (rho / 8) + 8 i + rho % 8 in its row
+//   rho: K's lane rho reads 16 dims of that key (two steps, dims 64 JJ + 16 kq +
+//   8 step + ..);
+// * V's lane (dim % 16, kq) reads its 16 keys of one dim as they lie, i = 2 step,
+//   2 step + 1, and P needs no exchange.
+template <int D, int NC>
+__global__ __launch_bounds__(256, D == 256 ? 1 : NC == 1 ? 3 : 2) void q8_token_kernel(AttnQ8Params p) {
+  constexpr int NJ = D / 64, NK = 4 * NJ, ND = D / 16;  // K loads (block, 64 dims) and V loads (16 dims) per page
+  constexpr int RS = D + 4;                             // a pair's row in `red`
+  union Lds {
+    uint16_t q[16 * NC * (D + 8)];
+    float red[kWaves * 16 * NC * RS];
+  };
+  __shared__ __attribute__((aligned(16))) Lds lds;
   __shared__ __attribute__((aligned(16))) float scl[kWaves][192];
-  __shared__ float red[kWaves][32][33];
-  __shared__ float mls[kWaves][2][32];
-  const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, h = lane >> 5;
+  __shared__ float mls[kWaves][2][16 * NC];
+  __shared__ float wmax[kWaves];
+  __shared__ uint32_t anc[16 * NC][DTREE_MASK_WORDS];
+  const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, kq = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int Hkv = p.kv.num_kv_heads, g = blockIdx.x % Hkv, b0 = blockIdx.x / Hkv;
   const int part = b0 % p.parts, s = b0 / p.parts;
@@ -331,54 +387,72 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void q8_token_kernel(AttnQ8P
   const int t0 = part * per, t1 = min(rg.tiles, t0 + per);
   if (part >= used) return;
   const int pairs = q.n * p.G;
-  const bool live = c < pairs;
-  const int r = live ? c / p.G : 0, head = g * p.G + (live ? c % p.G : 0);
-  const size_t row = (size_t)q.start + r;
 
-  u32x4_t qf[D / 16];
-  float inv;
-  {
-    float x[NB][16], f, amax = q8_query<D>(p, live, row, head, h, x);
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) amax = fmaxf(amax, __shfl_xor(amax, o));
-    q8_exponent(amax, f, inv);
-    q8_pack<D>(x, f, qf);
-  }
-  const Q8Mask mask = q8_mask(p, q, live, r);
-  f32x16_t o[NB];
-#pragma unroll
-  for (int db = 0; db < NB; ++db)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) o[db][i] = 0.f;
-  float m = kFloor, l = 0.f;
-
-  u32x4_t kb[NL], vb[NL];
+  u32x4_t kb[NK], vb[ND];
   float ksl, vsl;
   auto block = [&](int page) { return ((size_t)max(page, 0) * Hkv + g); };
-  auto page_of = [&](int t) {
-    return t < t1 ? __builtin_amdgcn_readfirstlane(q8_page(p.kv, s, rg.page(t))) : -1;
+  // The wave's i-th page is in lane i % 64 of `ids`: a load in the loop would
+  // have to come back, and with it every load before it, to be used.
+  int ids = -1;
+  auto load_ids = [&](int i) {
+    const int t = t0 + wave + kWaves * (i + lane);
+    ids = t < t1 ? q8_page(p.kv, s, rg.page(t)) : -1;
+  };
+  auto page_of = [&](int i) {
+    if ((i & 63) == 0) load_ids(i);
+    return __builtin_amdgcn_readlane(ids, i & 63);
   };
   // (a resource of no bytes reads as zeros without an access)
-  auto load_k = [&](int page, int half) {
-    const auto rk = buf_rsrc(p.kv.k_pages + block(page) * (DTREE_PAGE * D) + half * SB, page < 0 ? 0 : SB);
+  const int koff = (c >> 3) * (32 * D) + (kq >> 1) * 1024 + ((kq & 1) * 32 + (c & 7)) * 16;
+  const int voff = (kq >> 1) * (32 * D) + ((kq & 1) * 32 + c) * 16;
+  auto load_k = [&](int page) {
+    const auto rk = buf_rsrc(p.kv.k_pages + block(page) * (DTREE_PAGE * D), page < 0 ? 0 : DTREE_PAGE * D);
 #pragma unroll
-    for (int i = 0; i < NL; ++i) kb[i] = buf_ld(rk, 16 * lane + 1024 * i);
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) kb[i * NJ + j] = buf_ld(rk, koff + 128 * i + 2048 * j);
     ksl = page < 0 ? 0.f : p.kv.k_scales[block(page) * DTREE_PAGE + lane];
     vsl = page < 0 ? 0.f : p.kv.v_scales[block(page) * DTREE_PAGE + lane];
   };
-  auto load_v = [&](int page, int half) {
-    const auto rv = buf_rsrc(p.kv.v_pages + block(page) * (DTREE_PAGE * D) + half * SB, page < 0 ? 0 : SB);
+  auto load_v = [&](int page) {
+    const auto rv = buf_rsrc(p.kv.v_pages + block(page) * (DTREE_PAGE * D), page < 0 ? 0 : DTREE_PAGE * D);
 #pragma unroll
-    for (int i = 0; i < NL; ++i) vb[i] = buf_ld(rv, 16 * lane + 1024 * i);
+    for (int i = 0; i < ND; ++i) vb[i] = buf_ld(rv, voff + 1024 * (i >> 1) + 256 * (i & 1));
   };
-  int t = t0 + wave, half = 0, cur = page_of(t);
-  load_k(cur, 0);
-  load_v(cur, 0);
-  while (t < t1) {
-    const int nhalf = BK == 2 ? 0 : half ^ 1, nt = nhalf ? t : t + kWaves;
-    const int next = nhalf ? cur : page_of(nt);
-    const int k0 = DTREE_PAGE * rg.page(t);
-    float* sc = scl[wave];
+  const int steps = max(0, (t1 - t0 - wave + kWaves - 1) / kWaves);  // the wave's pages
+  int cur = page_of(0);
+  load_k(cur);
+  q8_ancestors(p, q, 0, 16 * NC, pairs, anc);
+  const float inv = q8_queries<D, 16 * NC, kWaves>(p, q, g, 0, pairs, lds.q, wmax);
+  load_v(cur);  // (not earlier: the queries' registers)
+  u32x4_t qf[NC][2 * NJ];
+  Q8Mask mask[NC];
+#pragma unroll
+  for (int n = 0; n < NC; ++n) {
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        qf[n][2 * j + k] = *reinterpret_cast<const u32x4_t*>(lds.q + (16 * n + c) * (D + 8) + 64 * j + 16 * kq + 8 * k);
+    const bool live = 16 * n + c < pairs;
+    mask[n] = q8_mask(p, q, live, (16 * n + c) / p.G, anc[16 * n + c]);
+  }
+  f32x4_t o[NC][ND];
+#pragma unroll
+  for (int n = 0; n < NC; ++n)
+#pragma unroll
+    for (int d = 0; d < ND; ++d) o[n][d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  float m[NC], l[NC];
+#pragma unroll
+  for (int n = 0; n < NC; ++n) {
+    m[n] = kFloor;
+    l[n] = 0.f;
+  }
+  const int kkey = 32 * (kq >> 1) + 4 * (kq & 1);  // the lane's keys: kkey + 8 i + e
+  float* sc = scl[wave];
+  for (int i = 0; i < steps; ++i) {
+    const int next = page_of(i + 1);
+    const int k0 = DTREE_PAGE * rg.page(t0 + wave + kWaves * i);
     {
       float k, lv, iv;
       q8_scales(ksl, vsl, inv, k, lv, iv);
@@ -386,83 +460,131 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void q8_token_kernel(AttnQ8P
       sc[64 + lane] = lv;
       sc[128 + lane] = iv;
     }
-    f32x16_t st[BK];
+    f32x4_t st[NC][4];
 #pragma unroll
-    for (int b = 0; b < BK; ++b)
+    for (int n = 0; n < NC; ++n)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) st[b][i] = 0.f;
+      for (int b = 0; b < 4; ++b) st[n][b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int J = 0; J < NB; ++J)
+    for (int b = 0; b < 4; ++b)
 #pragma unroll
-      for (int b = 0; b < BK; ++b) {
+      for (int j = 0; j < NJ; ++j) {
         u32x4_t a0, a1;
-        q8_to_h16(kb[b * NB + J], a0, a1);
-        st[b] = mfma32_f16(a0, qf[2 * J], st[b]);
-        st[b] = mfma32_f16(a1, qf[2 * J + 1], st[b]);
+        q8_to_h16(kb[b * NJ + j], a0, a1);
+#pragma unroll
+        for (int n = 0; n < NC; ++n) {
+          st[n][b] = mfma16_f16(a0, qf[n][2 * j], st[n][b]);
+          st[n][b] = mfma16_f16(a1, qf[n][2 * j + 1], st[n][b]);
+        }
       }
-    load_k(next, nhalf);
+    load_k(next);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
     if (cur >= 0) {
-      const bool masked = mask.tree ? k0 + DTREE_PAGE > q.past
-                                    : k0 + DTREE_PAGE - 1 > q.past ||
-                                          (p.a.window > 0 && k0 + DTREE_PAGE - 1 >= p.a.sink &&
-                                           q.past + q.n - 1 - k0 >= p.a.window);
+      const bool masked = mask[0].tree ? k0 + DTREE_PAGE > q.past
+                                       : k0 + DTREE_PAGE - 1 > q.past ||
+                                             (p.a.window > 0 && k0 + DTREE_PAGE - 1 >= p.a.sink &&
+                                              q.past + q.n - 1 - k0 >= p.a.window);
+      u32x4_t ph[NC][2];
 #pragma unroll
-      for (int b = 0; b < BK; ++b) {
-        u32x4_t ph[2];
-        q8_softmax<NB>(st[b], sc, b + half, h, masked, mask, k0, m, l, o, ph);
+      for (int n = 0; n < NC; ++n) {
+        float mx = kFloor;
 #pragma unroll
-        for (int db = 0; db < NB; ++db) {
-          u32x4_t a0, a1;
-          q8_to_h16(vb[b * NB + db], a0, a1);
-          o[db] = mfma32_f16(a0, ph[0], o[db]);
-          o[db] = mfma32_f16(a1, ph[1], o[db]);
+        for (int b = 0; b < 4; ++b) {
+          const f32x4_t ks = *reinterpret_cast<const f32x4_t*>(sc + kkey + 8 * b);
+          const f32x4_t lv = *reinterpret_cast<const f32x4_t*>(sc + 64 + kkey + 8 * b);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) st[n][b][e] = fmaf(st[n][b][e], ks[e], lv[e]);
+        }
+        if (masked) {
+#pragma unroll
+          for (int b = 0; b < 4; ++b)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (!mask[n].sees(k0 + kkey + 8 * b + e)) st[n][b][e] = -INFINITY;
+        }
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mx = fmaxf(mx, st[n][b][e]);
+        mx = fmaxf(mx, __shfl_xor(mx, 16));
+        mx = fmaxf(mx, __shfl_xor(mx, 32));
+        if (__any(mx > m[n] + (kTop + kSlack))) {
+          const float mn = mx > m[n] + (kTop + kSlack) ? mx - kTop : m[n], alpha = fast_exp2(m[n] - mn);
+          m[n] = mn;
+          l[n] *= alpha;
+#pragma unroll
+          for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[n][d][e] *= alpha;
+        }
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          const f32x4_t iv = *reinterpret_cast<const f32x4_t*>(sc + 128 + kkey + 8 * b);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            st[n][b][e] = fast_exp2(st[n][b][e] - m[n]);
+            l[n] = fmaf(st[n][b][e], iv[e], l[n]);
+          }
+          ph[n][b >> 1][2 * (b & 1)] = pack_h2(st[n][b][0], st[n][b][1]);
+          ph[n][b >> 1][2 * (b & 1) + 1] = pack_h2(st[n][b][2], st[n][b][3]);
+        }
+      }
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        u32x4_t a0, a1;
+        q8_to_h16(vb[d], a0, a1);
+#pragma unroll
+        for (int n = 0; n < NC; ++n) {
+          o[n][d] = mfma16_f16(a0, ph[n][0], o[n][d]);
+          o[n][d] = mfma16_f16(a1, ph[n][1], o[n][d]);
         }
       }
     }
-    load_v(next, nhalf);
+    load_v(next);
     cur = next;
-    half = nhalf;
-    t = nt;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
   }
 
   // the four waves' results
-  l += __shfl_xor(l, 32);
-  if (h == 0) {
-    mls[wave][0][c] = m;
-    mls[wave][1][c] = l;
-  }
-  __syncthreads();
-  float mt = kFloor;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) mt = fmaxf(mt, mls[w][0][c]);
-  const float fac = fast_exp2(m - mt);
-  const int pr = tid >> 3, pd = 4 * (tid & 7);  // this thread's pair and dims of a 32-dim block
-  float ml = kFloor, lt = 0.f;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) ml = fmaxf(ml, mls[w][0][pr]);
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) lt += mls[w][1][pr] * fast_exp2(mls[w][0][pr] - ml);
-  const int po = pr / p.G, ph_ = g * p.G + pr % p.G;
-#pragma unroll
-  for (int db = 0; db < NB; ++db) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) red[wave][c][acc_row(i, h)] = o[db][i] * fac;
-    __syncthreads();
-    if (pr < pairs) {
-      float y[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        y[e] = 0.f;
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) y[e] += red[w][pr][pd + e];
-      }
-      q8_emit(p, used > 1, part, (size_t)q.start + po, ph_, 32 * db + pd, y, ml, lt);
+  for (int n = 0; n < NC; ++n) {
+    l[n] += __shfl_xor(l[n], 16);
+    l[n] += __shfl_xor(l[n], 32);
+    if (kq == 0) {
+      mls[wave][0][16 * n + c] = m[n];
+      mls[wave][1][16 * n + c] = l[n];
     }
-    __syncthreads();
+  }
+  lds_barrier();  // also: every wave has read its queries
+#pragma unroll
+  for (int n = 0; n < NC; ++n) {
+    const int pr = 16 * n + c;
+    if (pr >= pairs) continue;
+    float mt = kFloor;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) mt = fmaxf(mt, mls[w][0][pr]);
+    const float fac = fast_exp2(m[n] - mt);
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+      *reinterpret_cast<f32x4_t*>(lds.red + (wave * 16 * NC + pr) * RS + 16 * d + 4 * kq) =
+          f32x4_t{o[n][d][0] * fac, o[n][d][1] * fac, o[n][d][2] * fac, o[n][d][3] * fac};
+  }
+  lds_barrier();
+  for (int u = tid; u < pairs * (D / 4); u += 256) {
+    const int pr = u / (D / 4), d = 4 * (u % (D / 4));
+    float mt = kFloor, lt = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) mt = fmaxf(mt, mls[w][0][pr]);
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      lt += mls[w][1][pr] * fast_exp2(mls[w][0][pr] - mt);
+      const f32x4_t v = *reinterpret_cast<const f32x4_t*>(lds.red + (w * 16 * NC + pr) * RS + d);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] += v[e];
+    }
+    q8_emit(p, used > 1, part, (size_t)q.start + pr / p.G, g * p.G + pr % p.G, d, y, mt, lt);
   }
 }
 
@@ -476,6 +598,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void q8_rows_kernel(AttnQ8Pa
   __shared__ __attribute__((aligned(16))) unsigned char kvb[2][4 * PB];  // fp16 K, then V
   __shared__ __attribute__((aligned(16))) float scl[2][192];
   __shared__ float wmax[kWaves];
+  __shared__ uint32_t anc[32 * kWaves][DTREE_MASK_WORDS];
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int Hkv = p.kv.num_kv_heads, g = blockIdx.x % Hkv;
@@ -519,19 +642,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void q8_rows_kernel(AttnQ8Pa
     return page >= 0;
   };
   bool here = load(t0), next = false;
+  static_assert(sizeof(kvb) >= 32 * kWaves * (D + 8) * sizeof(uint16_t), "the queries pass through kvb");
+  uint16_t* qs = reinterpret_cast<uint16_t*>(&kvb[0][0]);
+  q8_ancestors(p, q, pair0, 32 * kWaves, pairs, anc);
+  const float inv = q8_queries<D, 32 * kWaves, kWaves>(p, q, g, pair0, pairs, qs, wmax);
   u32x4_t qf[D / 16];
-  float inv;
-  {
-    float x[NB][16], f, amax = q8_query<D>(p, live, row, head, h, x);
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) amax = fmaxf(amax, __shfl_xor(amax, o));
-    if (lane == 0) wmax[wave] = amax;
-    __syncthreads();
-#pragma unroll
-    for (int o = 0; o < kWaves; ++o) amax = fmaxf(amax, wmax[o]);
-    q8_exponent(amax, f, inv);
-    q8_pack<D>(x, f, qf);
-  }
+  for (int i = 0; i < D / 16; ++i)
+    qf[i] = *reinterpret_cast<const u32x4_t*>(qs + (32 * wave + c) * (D + 8) + 32 * (i >> 1) + 16 * h + 8 * (i & 1));
+  lds_barrier();
   auto stage = [&](int buf) {
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
@@ -553,7 +672,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void q8_rows_kernel(AttnQ8Pa
       scl[buf][128 + tid] = iv;
     }
   };
-  const Q8Mask mask = q8_mask(p, q, live, r);
+  const Q8Mask mask = q8_mask(p, q, live, r, anc[32 * wave + c]);
   f32x16_t o[NB];
 #pragma unroll
   for (int db = 0; db < NB; ++db)
@@ -610,37 +729,81 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void q8_rows_kernel(AttnQ8Pa
   }
 }
 
-// Adds the ranges' partial results: D / 4 threads a pair.
-template <int D, bool TOKENS>
+// Adds the ranges' partial results: D / 4 threads for a pair's dims, NG groups of
+// them take its ranges in turn (many ranges of few pairs), and meet in LDS.
+template <int D, bool TOKENS, int NG>
 __global__ __launch_bounds__(256) void q8_join_kernel(AttnQ8Params p) {
-  constexpr int TPP = D / 4;
-  const int s = blockIdx.y, u = blockIdx.x * (256 / TPP) + threadIdx.x / TPP, d = 4 * (threadIdx.x % TPP);
+  constexpr int TPP = D / 4, PPB = 256 / TPP / NG;  // pairs of a workgroup
+  __shared__ __attribute__((aligned(16))) float sums[NG > 1 ? NG : 1][TPP * PPB][4];
+  __shared__ float stat[NG > 1 ? NG : 1][PPB][2];
+  const int tid = threadIdx.x, d = 4 * (tid % TPP), pl = tid / TPP % PPB, grp = tid / (TPP * PPB);
+  const int s = blockIdx.y, u = blockIdx.x * PPB + pl;
   const Q8Seq q = q8_seq(p.kv, s);
   const int r = u / p.a.num_heads, head = u % p.a.num_heads;
-  if (r >= q.n) return;
+  if (blockIdx.x * PPB >= q.n * p.a.num_heads) return;
   int from = 0, to = q.n - 1;  // the rows of its workgroup
   if constexpr (!TOKENS) {
     const int pair0 = (r * p.G + head % p.G) / (32 * kWaves) * (32 * kWaves);
-    from = pair0 / p.G;
+    from = min(pair0 / p.G, q.n - 1);
     to = min(q.n - 1, (pair0 + 32 * kWaves - 1) / p.G);
   }
   const int tiles = q8_range(p, q, from, to).tiles, used = q8_parts(p, tiles);
-  if (used <= 1) return;
-  const size_t row = (size_t)q.start + r, at = row * p.a.num_heads + head;
+  const bool live = r < q.n && used > 1;
+  const size_t row = (size_t)q.start + (live ? r : 0), at = row * p.a.num_heads + head;
   const size_t step = (size_t)p.kv.total_rows * p.a.num_heads;
-  float m = kFloor, l = 0.f;
-  for (int i = 0; i < used; ++i) m = fmaxf(m, p.part_ml[2 * (at + i * step)]);
-  float o[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int i = 0; i < used; ++i) {
-    const f32x2_t ml = *reinterpret_cast<const f32x2_t*>(p.part_ml + 2 * (at + i * step));
-    const f32x4_t v = *reinterpret_cast<const f32x4_t*>(p.part + (at + i * step) * D + d);
-    const float k = fast_exp2(ml[0] - m);
-    l = fmaf(k, ml[1], l);
+  float m = kFloor, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+  if (live) {
+    constexpr int U = 4;  // ranges in flight
+    for (int i0 = grp; i0 < used; i0 += U * NG) {
+      f32x2_t ml[U];
+      f32x4_t v[U];
+      float mx = m;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = fmaf(k, v[e], o[e]);
+      for (int k = 0; k < U; ++k) {
+        const int i = min(i0 + k * NG, used - 1);
+        ml[k] = *reinterpret_cast<const f32x2_t*>(p.part_ml + 2 * (at + i * step));
+        v[k] = *reinterpret_cast<const f32x4_t*>(p.part + (at + i * step) * D + d);
+      }
+#pragma unroll
+      for (int k = 0; k < U; ++k)
+        if (i0 + k * NG < used) mx = fmaxf(mx, ml[k][0]);
+      const float a = fast_exp2(m - mx);
+      m = mx;
+      l *= a;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] *= a;
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        if (i0 + k * NG >= used) continue;
+        const float f = fast_exp2(ml[k][0] - m);
+        l = fmaf(f, ml[k][1], l);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = fmaf(f, v[k][e], o[e]);
+      }
+    }
   }
-  q8_emit(p, false, 0, row, head, d, o, m, l);
+  if constexpr (NG > 1) {
+    if (tid % TPP == 0) {
+      stat[grp][pl][0] = m;
+      stat[grp][pl][1] = l;
+    }
+    *reinterpret_cast<f32x4_t*>(sums[grp][tid % (TPP * PPB)]) = f32x4_t{o[0], o[1], o[2], o[3]};
+    __syncthreads();
+    if (grp) return;
+    float mt = kFloor;
+#pragma unroll
+    for (int k = 0; k < NG; ++k) mt = fmaxf(mt, stat[k][pl][0]);
+    m = mt;
+    l = o[0] = o[1] = o[2] = o[3] = 0.f;
+#pragma unroll
+    for (int k = 0; k < NG; ++k) {
+      const float f = fast_exp2(stat[k][pl][0] - mt);
+      l = fmaf(f, stat[k][pl][1], l);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = fmaf(f, sums[k][tid % (TPP * PPB)][e], o[e]);
+    }
+  }
+  if (live) q8_emit(p, false, 0, row, head, d, o, m, l);
 }
 
 // The launch for a record: which kernel, its grid and key ranges.
@@ -661,7 +824,7 @@ Plan make_plan(const DtreeKvQ8& kv, const DtreeAttnQ8Args& a) {
   const int G = a.num_heads / kv.num_kv_heads;
   Plan pl{};
   const int64_t pairs = (int64_t)std::max(kv.max_rows, a.rows_padded) * G;
-  pl.tokens = pairs <= 32;
+  pl.tokens = pairs <= (kv.head_dim == 256 ? 16 : 32);  // (registers: 32 columns of 256 dims do not fit)
   pl.blocks = pl.tokens ? 1 : (int)((pairs + 32 * kWaves - 1) / (32 * kWaves));
   // pages that one workgroup's rows can see
   const int64_t end = std::min((int64_t)kv.max_past_length + kv.max_rows, (int64_t)kv.ld_page_table * DTREE_PAGE);
@@ -677,17 +840,28 @@ Plan make_plan(const DtreeKvQ8& kv, const DtreeAttnQ8Args& a) {
   return pl;
 }
 
-template <int D>
-int launch(const AttnQ8Params& p, bool tokens, unsigned grid, dim3 join, hipStream_t stream) {
-  if (tokens) q8_token_kernel<D><<<grid, 256, 0, stream>>>(p);
-  else q8_rows_kernel<D><<<grid, 256, 0, stream>>>(p);
-  DTREE_LAUNCH_CHECK("attention_q8 launch");
-  if (p.parts > 1) {
-    if (tokens) q8_join_kernel<D, true><<<join, 256, 0, stream>>>(p);
-    else q8_join_kernel<D, false><<<join, 256, 0, stream>>>(p);
-    DTREE_LAUNCH_CHECK("attention_q8 join launch");
-  }
+template <int D, bool TOKENS>
+int launch_join(const AttnQ8Params& p, hipStream_t stream) {
+  constexpr int NG = 1024 / D;  // groups with one pair a workgroup
+  const int64_t pairs = (int64_t)p.kv.max_rows * p.a.num_heads;
+  // Groups pay where there are ranges for them to share.
+  const bool groups = p.parts >= 2 * NG;
+  const dim3 grid((unsigned)(groups ? pairs : (pairs + NG - 1) / NG), (unsigned)p.kv.num_seqs);
+  if (groups) q8_join_kernel<D, TOKENS, NG><<<grid, 256, 0, stream>>>(p);
+  else q8_join_kernel<D, TOKENS, 1><<<grid, 256, 0, stream>>>(p);
+  DTREE_LAUNCH_CHECK("attention_q8 join launch");
   return DTREE_OK;
+}
+
+template <int D>
+int launch(const AttnQ8Params& p, bool tokens, unsigned grid, hipStream_t stream) {
+  if (!tokens) q8_rows_kernel<D><<<grid, 256, 0, stream>>>(p);
+  else if (D == 256 || std::max(p.kv.max_rows, p.a.rows_padded) * p.G <= 16)
+    q8_token_kernel<D, 1><<<grid, 256, 0, stream>>>(p);
+  else if constexpr (D != 256) q8_token_kernel<D, 2><<<grid, 256, 0, stream>>>(p);
+  DTREE_LAUNCH_CHECK("attention_q8 launch");
+  if (p.parts == 1) return DTREE_OK;
+  return tokens ? launch_join<D, true>(p, stream) : launch_join<D, false>(p, stream);
 }
 
 bool q8_geometry(const DtreeKvQ8& kv, const DtreeAttnQ8Args& a) {
@@ -760,11 +934,10 @@ extern "C" int dtree_attention_q8(const DtreeKvQ8* kv, const DtreeAttnQ8Args* a,
   p.h16 = a->out_layout == DTREE_W_TILED_F16;
   if (p.h16) p.a.out_lo = nullptr;
   const int64_t grid = (int64_t)kv->num_seqs * pl.blocks * pl.parts * kv->num_kv_heads;
-  const int64_t jx = ((int64_t)kv->max_rows * a->num_heads + 1024 / D - 1) / (1024 / D);
-  DTREE_REQUIRE(grid < (int64_t)1 << 31 && jx < (int64_t)1 << 31 && (pl.parts == 1 || kv->num_seqs <= 65535),
+  DTREE_REQUIRE(grid < (int64_t)1 << 31 && (int64_t)kv->max_rows * a->num_heads < (int64_t)1 << 31 &&
+                    (pl.parts == 1 || kv->num_seqs <= 65535),
                 "attention_q8: num_seqs * max_rows too large for one launch");
-  const dim3 join((unsigned)jx, (unsigned)kv->num_seqs);
-  if (D == 64) return launch<64>(p, pl.tokens, (unsigned)grid, join, stream);
-  if (D == 128) return launch<128>(p, pl.tokens, (unsigned)grid, join, stream);
-  return launch<256>(p, pl.tokens, (unsigned)grid, join, stream);
+  if (D == 64) return launch<64>(p, pl.tokens, (unsigned)grid, stream);
+  if (D == 128) return launch<128>(p, pl.tokens, (unsigned)grid, stream);
+  return launch<256>(p, pl.tokens, (unsigned)grid, stream);
 }
