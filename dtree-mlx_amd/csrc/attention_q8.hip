@@ -18,6 +18,7 @@
 // upper part of fp16's range, and taken back in ks.
 // A masked key's t is -inf, whatever its scales and bytes are (u = 0 exactly).
 #include <algorithm>
+#include <type_traits>
 
 #include "kv_q8.h"
 
@@ -32,12 +33,13 @@ constexpr int kWaves = 4;
 struct AttnQ8Params {
   DtreeKvQ8 kv;
   DtreeAttnQ8Args a;
-  int G, blocks;        // heads per group; row blocks per sequence
+  int G, blocks, pairs_wg;  // heads per group; row blocks per sequence, pairs of one
   int parts, per;       // key ranges the grid holds; pages of a range
   int sink_pages;
   float scale_log2;
   float* part; float* part_ml;  // [parts][total_rows][Hq] x D, x (m, l)
   int tiled, h16;
+  int plain;  // out: rows of bf16 alone, 16-byte aligned, no gate
 };
 
 // The pages that the rows from..to of a sequence see between them: the sink's,
@@ -58,103 +60,34 @@ __device__ __forceinline__ int q8_parts(const AttnQ8Params& p, int tiles) {
   return min(p.parts, (tiles + p.per - 1) / p.per);
 }
 
-// 16 int8 -> two fragments of eight fp16, exact: 1024 + 128 + q as fp16 bits,
-// less 1152.
-__device__ __forceinline__ void q8_to_h16(u32x4_t w, u32x4_t& a, u32x4_t& b) {
+// 4 int8 -> 4 fp16, exact: 1024 + 128 + q as fp16 bits, less 1152.
+__device__ __forceinline__ void q8_word_to_h4(uint32_t w, uint32_t& lo, uint32_t& hi) {
   const f16x2_t bias = {(_Float16)1152.f, (_Float16)1152.f};
-  auto two = [&](uint32_t x, uint32_t sel) {
-    const f16x2_t v = __builtin_bit_cast(f16x2_t, __builtin_amdgcn_perm(0x64646464u, x, sel)) - bias;
-    return __builtin_bit_cast(uint32_t, v);
-  };
+  const uint32_t x = w ^ 0x80808080u;
+  lo = __builtin_bit_cast(uint32_t,
+                          __builtin_bit_cast(f16x2_t, __builtin_amdgcn_perm(0x64646464u, x, 0x04010400u)) - bias);
+  hi = __builtin_bit_cast(uint32_t,
+                          __builtin_bit_cast(f16x2_t, __builtin_amdgcn_perm(0x64646464u, x, 0x04030402u)) - bias);
+}
+// 16 int8 -> two fragments of eight fp16.
+__device__ __forceinline__ void q8_to_h16(u32x4_t w, u32x4_t& a, u32x4_t& b) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint32_t x = w[i] ^ 0x80808080u, lo = two(x, 0x04010400u), hi = two(x, 0x04030402u);
-    if (i < 2) {
-      a[2 * i] = lo;
-      a[2 * i + 1] = hi;
-    } else {
-      b[2 * i - 4] = lo;
-      b[2 * i - 3] = hi;
-    }
+    uint32_t lo, hi;
+    q8_word_to_h4(w[i], lo, hi);
+    (i < 2 ? a : b)[2 * (i & 1)] = lo;
+    (i < 2 ? a : b)[2 * (i & 1) + 1] = hi;
   }
 }
 
-// 16 elements of q at dims 16 c .. of a head.
-__device__ __forceinline__ void q8_load16(const AttnQ8Params& p, size_t at, float (&x)[16]) {
-  if (p.a.q_type == DTREE_T_BF16) {
-    const uint16_t* s = static_cast<const uint16_t*>(p.a.q) + at;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const u32x4_t w = ld_u32x4(s + 8 * i);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        x[8 * i + 2 * j] = __uint_as_float(w[j] << 16);
-        x[8 * i + 2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
-      }
-    }
-  } else {
-    const float* s = static_cast<const float*>(p.a.q) + at;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const f32x4_t w = *reinterpret_cast<const f32x4_t*>(s + 4 * i);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) x[4 * i + j] = w[j];
-    }
-  }
-}
-
-// 16 norm weights / 16 table entries, at any address of their type.
-__device__ __forceinline__ void q8_weights16(const uint16_t* w, float (&x)[16]) {
-  u32x4_t v[2];
-  __builtin_memcpy(v, w, sizeof(v));
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const uint32_t b = v[i >> 3][(i >> 1) & 3];
-    x[i] = __uint_as_float((i & 1) ? (b & 0xffff0000u) : (b << 16));
-  }
-}
-__device__ __forceinline__ void q8_table16(const float* t, float (&x)[16]) { __builtin_memcpy(x, t, sizeof(x)); }
-
-// Chunk c (dims 16 c ..) of a row's query head: q_norm, RoPE, the softmax scale
-// in log2 units; the row's D / 16 chunks are neighbouring lanes. Every load comes
-// before the first use (the rotation's other chunk is loaded rather than
-// exchanged).
-template <int D>
-__device__ __forceinline__ void q8_query16(const AttnQ8Params& p, size_t row, int head, int c, float (&x)[16]) {
-  const size_t base = row * p.a.ld_q + (size_t)head * p.a.q_stride;
-  const int half = p.a.rope_dims / 2, hc = half / 16;  // the rotation's halves, hc chunks each
-  const bool turns = c < 2 * hc, low = c < hc, norm = p.a.q_norm != nullptr;
-  const int co = low ? c + hc : c - hc;
-  float o[16], w[16], wo[16], cs[16], sn[16];
-  q8_load16(p, base + 16 * c, x);
-  if (norm) q8_weights16(p.a.q_norm + 16 * c, w);
-  if (turns) {
-    q8_load16(p, base + 16 * co, o);
-    if (norm) q8_weights16(p.a.q_norm + 16 * co, wo);
-    const size_t at = row * half + 16 * (low ? c : co);
-    q8_table16(p.a.rope_cos + at, cs);
-    q8_table16(p.a.rope_sin + at, sn);
-  }
-  float rs = 1.f;
-  if (norm) {
-    float ss = 0.f;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) ss = fmaf(x[i], x[i], ss);
-#pragma unroll
-    for (int k = 1; k < D / 16; k <<= 1) ss += __shfl_xor(ss, k);
-    rs = rsqrtf(ss * (1.0f / D) + p.a.eps);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] *= rs * w[i];
-  }
-  if (turns) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float y = norm ? o[i] * (rs * wo[i]) : o[i];
-      x[i] = low ? x[i] * cs[i] - y * sn[i] : y * sn[i] + x[i] * cs[i];
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < 16; ++i) x[i] *= p.scale_log2;
+// max over the lane and lane ^ 32, without an LDS round trip: v_permlane32_swap of
+// a value with its copy leaves one half's values in one register, the other's in
+// the other. (s_nop: VALU write to permlane read.)
+__device__ __forceinline__ float max_halves(float a) {
+  float b;
+  asm volatile("v_mov_b32 %1, %0\n\ts_nop 1\n\tv_permlane32_swap_b32 %0, %1\n\tv_max_f32 %0, %0, %1"
+               : "+v"(a), "=&v"(b));
+  return a;
 }
 
 // 2^e that takes amax into [2^13, 2^14), and its inverse.
@@ -165,35 +98,109 @@ __device__ __forceinline__ void q8_exponent(float amax, float& f, float& inv) {
   inv = __uint_as_float((uint32_t)(254 - ef) << 23);
 }
 
-// The queries of up to PAIRS pairs from pair0 on, in fp16 at qs[pair][D + 8]
-// (zeros past `pairs`), moved by one power of two for the workgroup; returns its
-// inverse. WAVES waves; the barriers wait for LDS alone.
+// Queries. A pair's D dims are D / 8 neighbouring lanes, each with two pieces of 4
+// dims: lane j of the first R / 8 the halves 4 j .. and R / 2 + 4 j .. of a rotation
+// of R dims, the others 8 dims that do not rotate. A wave's loads are then whole
+// runs of the rows.
+struct Q8Pieces {
+  int at[2];   // first dim of each
+  bool turns;  // the two rotate
+};
+template <int D>
+__device__ __forceinline__ Q8Pieces q8_pieces(int rope_dims, int j) {
+  const int hp = rope_dims / 8;  // pieces of a rotation's half
+  const bool turns = j < hp;
+  return Q8Pieces{{4 * (turns ? j : 2 * j), 4 * (turns ? j + hp : 2 * j + 1)}, turns};
+}
+__device__ __forceinline__ f32x4_t q8_bf4(u32x2_t w) {
+  return f32x4_t{__uint_as_float(w[0] << 16), __uint_as_float(w[0] & 0xffff0000u), __uint_as_float(w[1] << 16),
+                 __uint_as_float(w[1] & 0xffff0000u)};
+}
+
+// The queries of up to PAIRS pairs from pair0 on (q_norm, RoPE, the softmax scale
+// in log2 units), in fp16 at qs[pair][D + 8] (past `pairs`: the last row's, their
+// results unread), moved by one power of two for the workgroup; returns its
+// inverse. WAVES waves; the barriers wait for LDS alone. A row's 1 / rms joins the
+// power of two, after the rotation.
 template <int D, int PAIRS, int WAVES>
 __device__ __forceinline__ float q8_queries(const AttnQ8Params& p, const Q8Seq& q, int g, int pair0, int pairs,
                                             uint16_t* qs, float* wmax) {
-  constexpr int TPR = D / 16, NT = 64 * WAVES, NR = (PAIRS * TPR + NT - 1) / NT;
-  const int tid = threadIdx.x;
-  float x[NR][16], amax = 0.f;
+  constexpr int TPR = D / 8, NT = 64 * WAVES, PPR = NT / TPR, NR = (PAIRS + PPR - 1) / PPR;  // PPR pairs a round
+  const int tid = threadIdx.x, j = tid % TPR;
+  const bool bf = p.a.q_type == DTREE_T_BF16;
+  const int half = p.a.rope_dims / 2;
+  const Q8Pieces pc = q8_pieces<D>(p.a.rope_dims, j);
+  f32x4_t x[NR][2], cs[NR], sn[NR], w[2];
+  // No load in a branch of a lane's own, so that all go out together: lanes
+  // without a rotation read the table's first entries.
+  int m = pair0 + tid / TPR, r = m / p.G, hd = m - r * p.G;
+  const int dr = PPR / p.G, dh = PPR % p.G;
 #pragma unroll
   for (int k = 0; k < NR; ++k) {
-    const int u = tid + NT * k, m = pair0 + u / TPR;
+    const size_t row = (size_t)q.start + min(r, q.n - 1);
+    const size_t base = row * p.a.ld_q + (size_t)(g * p.G + hd) * p.a.q_stride;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) x[k][i] = 0.f;
-    if (m < pairs && u < PAIRS * TPR) {
-      q8_query16<D>(p, (size_t)q.start + m / p.G, g * p.G + m % p.G, u % TPR, x[k]);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float v = fabsf(x[k][i]);
-        amax = v < INFINITY ? fmaxf(amax, v) : amax;  // (what is not finite stays in its row)
-      }
+    for (int i = 0; i < 2; ++i) {
+      if (bf) x[k][i] = q8_bf4(*reinterpret_cast<const u32x2_t*>(static_cast<const uint16_t*>(p.a.q) + base + pc.at[i]));
+      else x[k][i] = *reinterpret_cast<const f32x4_t*>(static_cast<const float*>(p.a.q) + base + pc.at[i]);
     }
+    if (half) {  // (tables and weights at any address of their type)
+      const size_t at = row * half + (pc.turns ? 4 * j : 0);
+      __builtin_memcpy(&cs[k], p.a.rope_cos + at, 16);
+      __builtin_memcpy(&sn[k], p.a.rope_sin + at, 16);
+    }
+    r += dr;
+    hd += dh;
+    if (hd >= p.G) {
+      hd -= p.G;
+      ++r;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    w[i] = f32x4_t{p.scale_log2, p.scale_log2, p.scale_log2, p.scale_log2};
+    if (p.a.q_norm) {
+      u32x2_t v;
+      __builtin_memcpy(&v, p.a.q_norm + pc.at[i], 8);
+      w[i] *= q8_bf4(v);
+    }
+  }
+  float amax = 0.f, rs[NR];
+#pragma unroll
+  for (int k = 0; k < NR; ++k) {
+    rs[k] = 1.f;
+    if (p.a.q_norm) {
+      float ss = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ss = fmaf(x[k][e >> 2][e & 3], x[k][e >> 2][e & 3], ss);
+      ss += dpp<0xB1>(ss);  // TPR lanes: of 2, 4, 8, 16, 32
+      ss += dpp<0x4E>(ss);
+      ss += dpp<0x141>(ss);
+      if constexpr (TPR >= 16) ss += dpp<0x140>(ss);
+      if constexpr (TPR >= 32) ss += swz_xor16(ss);
+      rs[k] = rsqrtf(ss * (1.0f / D) + p.a.eps);
+    }
+    float mx = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float y = x[k][0][e] * w[0][e], z = x[k][1][e] * w[1][e];
+      x[k][0][e] = y;
+      x[k][1][e] = z;
+      if (half) {  // (a select, not sn = 0, which would carry an infinity to another dim)
+        x[k][0][e] = pc.turns ? y * cs[k][e] - z * sn[k][e] : y;
+        x[k][1][e] = pc.turns ? y * sn[k][e] + z * cs[k][e] : z;
+      }
+      mx = fmaxf(mx, fmaxf(fabsf(x[k][0][e]), fabsf(x[k][1][e])));
+    }
+    mx *= rs[k];
+    amax = mx < INFINITY ? fmaxf(amax, mx) : amax;  // (a row that is not finite is NaN whatever its exponent)
   }
   amax = fmaxf(amax, dpp<0xB1>(amax));
   amax = fmaxf(amax, dpp<0x4E>(amax));
   amax = fmaxf(amax, dpp<0x141>(amax));
   amax = fmaxf(amax, dpp<0x140>(amax));
   amax = fmaxf(amax, swz_xor16(amax));
-  amax = fmaxf(amax, __shfl_xor(amax, 32));
+  amax = max_halves(amax);
   if ((tid & 63) == 0) wmax[tid >> 6] = amax;
   lds_barrier();
 #pragma unroll
@@ -202,13 +209,12 @@ __device__ __forceinline__ float q8_queries(const AttnQ8Params& p, const Q8Seq& 
   q8_exponent(amax, f, inv);
 #pragma unroll
   for (int k = 0; k < NR; ++k) {
-    const int u = tid + NT * k;
-    if (u < PAIRS * TPR) {
-      u32x4_t* o = reinterpret_cast<u32x4_t*>(qs + (u / TPR) * (D + 8) + 16 * (u % TPR));
+    const int pl = tid / TPR + k * PPR;
+    if (PAIRS % PPR != 0 && pl >= PAIRS) continue;
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
-        o[j] = u32x4_t{pack_h2(x[k][8 * j] * f, x[k][8 * j + 1] * f), pack_h2(x[k][8 * j + 2] * f, x[k][8 * j + 3] * f),
-                       pack_h2(x[k][8 * j + 4] * f, x[k][8 * j + 5] * f), pack_h2(x[k][8 * j + 6] * f, x[k][8 * j + 7] * f)};
+    for (int i = 0; i < 2; ++i) {
+      const f32x4_t y = x[k][i] * rs[k] * f;
+      *reinterpret_cast<u32x2_t*>(qs + pl * (D + 8) + pc.at[i]) = u32x2_t{pack_h2(y[0], y[1]), pack_h2(y[2], y[3])};
     }
   }
   lds_barrier();
@@ -224,23 +230,24 @@ __device__ __forceinline__ void q8_scales(float ks, float vs, float inv, float& 
   iv = v == v ? 1.f / v : 1.f;
 }
 
-// What a lane's row sees.
-struct Q8Mask {
-  int pos;             // position; -1: the lane has no pair
-  int sink, window;    // window 0: all
-  bool tree;
-  int past, rows;      // draft tree: the prefix, the sequence's rows,
-  const uint32_t* anc;  // and the pair's ancestor words in LDS
-  __device__ __forceinline__ bool sees(int key) const {
-    if (tree) {
-      const int n = key - past;
-      return pos >= 0 && (n < 0 || (n < rows && ((anc[(n >> 5) & 3] >> (n & 31)) & 1u)));
-    }
-    return key <= pos && (window == 0 || key < sink || pos - key < window);
+// The keys key0 .. key0 + 31 that the pair at `pos` (-1: none) sees, a bit each.
+// Draft tree: the cached prefix and `anc`, the pair's ancestor words in LDS.
+__device__ __forceinline__ uint32_t q8_low_bits(int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; }
+__device__ __forceinline__ uint32_t q8_sees(const AttnQ8Params& p, const Q8Seq& q, int pos, int key0,
+                                            const uint32_t* anc) {
+  if (p.a.ancestors) {
+    const int n = key0 - q.past;  // the new row that key0 is
+    if (pos < 0) return 0u;
+    if (n <= -32) return ~0u;
+    if (n < 0) return q8_low_bits(-n) | ((anc[0] & q8_low_bits(q.n)) << -n);
+    if (n >= q.n) return 0u;
+    const int w = n >> 5;  // (at most 128 rows)
+    const uint32_t lo = anc[w], hi = w + 1 < DTREE_MASK_WORDS ? anc[w + 1] : 0u;
+    return __builtin_amdgcn_alignbit(hi, lo, n & 31) & q8_low_bits(q.n - n);
   }
-};
-__device__ __forceinline__ Q8Mask q8_mask(const AttnQ8Params& p, const Q8Seq& q, bool live, int r, const uint32_t* anc) {
-  return Q8Mask{live ? q.past + r : -1, p.a.sink, p.a.window, p.a.ancestors != nullptr, q.past, q.n, anc};
+  uint32_t bits = q8_low_bits(pos - key0 + 1);
+  if (p.a.window > 0) bits &= ~q8_low_bits(pos - p.a.window + 1 - key0) | q8_low_bits(p.a.sink - key0);
+  return bits;
 }
 // The ancestor words of pairs pair0 .. pair0 + n - 1 to LDS (a barrier follows).
 __device__ __forceinline__ void q8_ancestors(const AttnQ8Params& p, const Q8Seq& q, int pair0, int n, int pairs,
@@ -250,50 +257,6 @@ __device__ __forceinline__ void q8_ancestors(const AttnQ8Params& p, const Q8Seq&
     const int m = pair0 + u / DTREE_MASK_WORDS, w = u % DTREE_MASK_WORDS;
     anc[u / DTREE_MASK_WORDS][w] =
         m < pairs ? p.a.ancestors[((size_t)q.start + m / p.G) * DTREE_MASK_WORDS + w] : 0u;
-  }
-}
-
-// One 32-key block: the logits' statistics and weights of a lane's 16 keys
-// (acc_row order), the output rescaled where the maximum has grown. `sc`: the
-// page's ks, log2 vs and 1 / vs in LDS.
-template <int ND>
-__device__ __forceinline__ void q8_softmax(f32x16_t& s, const float* sc, int b, int h, bool masked, const Q8Mask& mask,
-                                           int k0, float& m, float& l, f32x16_t (&o)[ND], u32x4_t (&ph)[2]) {
-  float mx = kFloor;
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const f32x4_t ks = *reinterpret_cast<const f32x4_t*>(sc + 32 * b + 8 * q + 4 * h);
-    const f32x4_t lv = *reinterpret_cast<const f32x4_t*>(sc + 64 + 32 * b + 8 * q + 4 * h);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) s[4 * q + e] = fmaf(s[4 * q + e], ks[e], lv[e]);
-  }
-  if (masked) {
-#pragma unroll
-    for (int r = 0; r < 16; ++r)
-      if (!mask.sees(k0 + 32 * b + acc_row(r, h))) s[r] = -INFINITY;
-  }
-#pragma unroll
-  for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[r]);
-  mx = fmaxf(mx, __shfl_xor(mx, 32));
-  if (__any(mx > m + (kTop + kSlack))) {
-    const float mn = mx > m + (kTop + kSlack) ? mx - kTop : m, alpha = fast_exp2(m - mn);
-    m = mn;
-    l *= alpha;
-#pragma unroll
-    for (int db = 0; db < ND; ++db)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) o[db][r] *= alpha;
-  }
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const f32x4_t iv = *reinterpret_cast<const f32x4_t*>(sc + 128 + 32 * b + 8 * q + 4 * h);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      s[4 * q + e] = fast_exp2(s[4 * q + e] - m);
-      l = fmaf(s[4 * q + e], iv[e], l);
-    }
-    ph[q >> 1][2 * (q & 1)] = pack_h2(s[4 * q], s[4 * q + 1]);
-    ph[q >> 1][2 * (q & 1) + 1] = pack_h2(s[4 * q + 2], s[4 * q + 3]);
   }
 }
 
@@ -326,17 +289,19 @@ __device__ __forceinline__ void q8_store_zero(const AttnQ8Params& p, size_t row,
   store_act4(p.a.out, p.a.out_lo, oi, y, p.h16);
 }
 
-// Four values of a pair (softmax sum l) to `out`, or unscaled to the range's
-// partials.
+// 1 / l, 0 where the row has seen no key.
+__device__ __forceinline__ float q8_inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
+
+// Four values of a pair to `out`, scaled by `inv`, or, of one of several ranges,
+// as they are to its partials, with the range's m and softmax sum l.
 __device__ __forceinline__ void q8_emit(const AttnQ8Params& p, bool split, int part, size_t row, int head, int d,
-                                        const float (&o)[4], float m, float l) {
+                                        const float (&o)[4], float m, float l, float inv) {
   if (split) {
     const size_t u = ((size_t)part * p.kv.total_rows + row) * p.a.num_heads + head;
     *reinterpret_cast<f32x4_t*>(p.part + u * p.kv.head_dim + d) = f32x4_t{o[0], o[1], o[2], o[3]};
     if (d == 0) *reinterpret_cast<f32x2_t*>(p.part_ml + 2 * u) = f32x2_t{m, l};
     return;
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
   float y[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
   q8_store(p, row, head, d, y);
 }
@@ -426,7 +391,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : NC == 1 ? 3 : 2) void q8_token_
   const float inv = q8_queries<D, 16 * NC, kWaves>(p, q, g, 0, pairs, lds.q, wmax);
   load_v(cur);  // (not earlier: the queries' registers)
   u32x4_t qf[NC][2 * NJ];
-  Q8Mask mask[NC];
+  int pos[NC];  // the columns' positions; -1: no pair
 #pragma unroll
   for (int n = 0; n < NC; ++n) {
 #pragma unroll
@@ -434,8 +399,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : NC == 1 ? 3 : 2) void q8_token_
 #pragma unroll
       for (int k = 0; k < 2; ++k)
         qf[n][2 * j + k] = *reinterpret_cast<const u32x4_t*>(lds.q + (16 * n + c) * (D + 8) + 64 * j + 16 * kq + 8 * k);
-    const bool live = 16 * n + c < pairs;
-    mask[n] = q8_mask(p, q, live, (16 * n + c) / p.G, anc[16 * n + c]);
+    pos[n] = 16 * n + c < pairs ? q.past + (16 * n + c) / p.G : -1;
   }
   f32x4_t o[NC][ND];
 #pragma unroll
@@ -481,10 +445,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : NC == 1 ? 3 : 2) void q8_token_
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
     if (cur >= 0) {
-      const bool masked = mask[0].tree ? k0 + DTREE_PAGE > q.past
-                                       : k0 + DTREE_PAGE - 1 > q.past ||
-                                             (p.a.window > 0 && k0 + DTREE_PAGE - 1 >= p.a.sink &&
-                                              q.past + q.n - 1 - k0 >= p.a.window);
+      const bool masked = p.a.ancestors ? k0 + DTREE_PAGE > q.past
+                                        : k0 + DTREE_PAGE - 1 > q.past ||
+                                              (p.a.window > 0 && k0 + DTREE_PAGE - 1 >= p.a.sink &&
+                                               q.past + q.n - 1 - k0 >= p.a.window);
       u32x4_t ph[NC][2];
 #pragma unroll
       for (int n = 0; n < NC; ++n) {
@@ -497,11 +461,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : NC == 1 ? 3 : 2) void q8_token_
           for (int e = 0; e < 4; ++e) st[n][b][e] = fmaf(st[n][b][e], ks[e], lv[e]);
         }
         if (masked) {
+          const uint32_t sees = q8_sees(p, q, pos[n], k0 + (kkey & 32), anc[16 * n + c]) >> (kkey & 31);
 #pragma unroll
           for (int b = 0; b < 4; ++b)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (!mask[n].sees(k0 + kkey + 8 * b + e)) st[n][b][e] = -INFINITY;
+            for (int e = 0; e < 4; ++e) st[n][b][e] = sees & (1u << (8 * b + e)) ? st[n][b][e] : -INFINITY;
         }
 #pragma unroll
         for (int b = 0; b < 4; ++b)
@@ -584,21 +548,40 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : NC == 1 ? 3 : 2) void q8_token_
 #pragma unroll
       for (int e = 0; e < 4; ++e) y[e] += v[e];
     }
-    q8_emit(p, used > 1, part, (size_t)q.start + pr / p.G, g * p.G + pr % p.G, d, y, mt, lt);
+    q8_emit(p, used > 1, part, (size_t)q.start + pr / p.G, g * p.G + pr % p.G, d, y, mt, lt, q8_inverse(lt));
   }
 }
 
-// A workgroup: 4 x 32 pairs of one KV head, a wave each, over one key range. A
-// page is converted to fp16 once for the four waves, on its way from memory to
-// LDS, the next one while the current one is used.
-template <int D>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void q8_rows_kernel(AttnQ8Params p) {
-  constexpr int NB = D / 32, PB = DTREE_PAGE * D;       // bytes of a page's K (or V) as int8
-  constexpr int NC = PB / 16 / 256;                     // 16-byte pieces of it per thread
-  __shared__ __attribute__((aligned(16))) unsigned char kvb[2][4 * PB];  // fp16 K, then V
+// A workgroup: 4 waves of 32 NC pairs of one KV head over one key range. A page is
+// converted to fp16 once for the four waves, on its way from memory to LDS, the
+// next one while the current one is used.
+//
+// A step is 32 keys, half a page: S^T = K Q^T, softmax, O^T += V^T P^T. The matrix
+// cores run S of the next step (block2) while the weights of this step's first 16
+// keys are taken, then PV (block1): of the first 16 keys while the weights of the
+// others are taken, of the others while the next step's logits are scaled, with
+// the next page's conversion in every second block1. A slot is one MFMA, the loads
+// that a later slot needs and a share of the VALU work, in this order
+// (sched_barrier: the compiler keeps it), so that neither unit waits for the other
+// to finish a step.
+template <int D, int NC>
+__global__ __launch_bounds__(256, NC == 1 && D <= 128 ? 2 : 1) void q8_rows_kernel(AttnQ8Params p) {
+  constexpr int NB = D / 32, PB = DTREE_PAGE * D;  // bytes of a page's K (or V) as int8
+  constexpr int NP = PB / 16 / 256;                // 16-byte pieces of it per thread
+  constexpr int NF = D / 16, NS = NF * NC;         // fragments of K (or V) in a step; MFMAs of a block
+  constexpr int RF = 4;                            // fragments loaded ahead
+  constexpr int EV = 16 * NC;                      // a lane's logits of a step
+  constexpr int CP = 32 * NC, WP = kWaves * CP;    // pairs of a wave, of the workgroup
+  constexpr int RS = D + 4;  // a pair's row in `red`
+  union Lds {
+    unsigned char kv[2][4 * PB];  // fp16 K, then V
+    uint16_t q[WP * (D + 8)];
+    float red[kWaves][32 * RS];
+  };
+  __shared__ __attribute__((aligned(16))) Lds lds;
   __shared__ __attribute__((aligned(16))) float scl[2][192];
   __shared__ float wmax[kWaves];
-  __shared__ uint32_t anc[32 * kWaves][DTREE_MASK_WORDS];
+  __shared__ uint32_t anc[WP][DTREE_MASK_WORDS];
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int Hkv = p.kv.num_kv_heads, g = blockIdx.x % Hkv;
@@ -607,63 +590,65 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void q8_rows_kernel(AttnQ8Pa
   bx /= p.parts;
   const int w = p.blocks - 1 - bx % p.blocks, s = bx / p.blocks;  // longest ranges first
   const Q8Seq q = q8_seq(p.kv, s);
-  const int pairs = q.n * p.G, pair0 = 32 * kWaves * w, pair = pair0 + 32 * wave + c;
-  const int r = pair / p.G, head = g * p.G + pair % p.G;
-  if (pair0 >= pairs) {  // rows past the sequence's
-    if (part == 0 && r < p.a.rows_padded && h == 0)
-      for (int d = 0; d < D; d += 4) q8_store_zero(p, r, head, d);
-    return;
+  const int pairs = q.n * p.G, pair0 = WP * w;
+  if (part == 0 && p.a.rows_padded > 0) {  // rows past the sequence's
+    const int end = min(pair0 + WP, p.a.rows_padded * p.G);
+    for (int e = max(pairs - pair0, 0) * (D / 4) + tid; e < (end - pair0) * (D / 4); e += 256) {
+      const int m = pair0 + e / (D / 4);
+      q8_store_zero(p, m / p.G, g * p.G + m % p.G, 4 * (e % (D / 4)));
+    }
   }
-  const int from = pair0 / p.G, to = min(q.n - 1, (pair0 + 32 * kWaves - 1) / p.G);  // the workgroup's rows
+  if (pair0 >= pairs) return;
+  const int from = pair0 / p.G, to = min(q.n - 1, (pair0 + WP - 1) / p.G);  // the workgroup's rows
   const Q8Range rg = q8_range(p, q, from, to);
   const int used = q8_parts(p, rg.tiles), per = (rg.tiles + used - 1) / used;
   const int t0 = part * per, t1 = min(rg.tiles, t0 + per);
   if (part >= used) return;
-  const bool live = pair < pairs;
-  const size_t row = (size_t)q.start + (live ? r : 0);
-  const int wfrom = (pair0 + 32 * wave) / p.G, wto = min(q.n - 1, (pair0 + 32 * wave + 31) / p.G);
-  const bool wlive = pair0 + 32 * wave < pairs;
+  const int wpair = pair0 + CP * wave;
+  // the wave's rows (a wave past the last pair works on zero queries, unread)
+  const int wfrom = min(wpair / p.G, q.n - 1), wto = min(q.n - 1, (wpair + CP - 1) / p.G);
 
-  u32x4_t kr[NC], vr[NC];
+  u32x4_t raw[2 * NP];
   float ksl = 0.f, vsl = 0.f;
-  auto load = [&](int t) {  // page t's pieces of this thread; false: the page is absent
-    const int page = __builtin_amdgcn_readfirstlane(q8_page(p.kv, s, rg.page(t)));
+  // The range's i-th page is in lane i % 64 of `ids` (a load in the loop would
+  // have to come back to be used).
+  int ids = -1;
+  auto load = [&](int i) {  // this thread's pieces of the i-th page; false: the page is absent
+    i = min(i, t1 - t0 - 1);
+    if ((i & 63) == 0) ids = t0 + i + lane < t1 ? q8_page(p.kv, s, rg.page(t0 + i + lane)) : -1;
+    const int page = __builtin_amdgcn_readlane(ids, i & 63);
     const size_t blk = (size_t)max(page, 0) * Hkv + g;
-    const u32x4_t zero = {0, 0, 0, 0};
+    const auto rk = buf_rsrc(p.kv.k_pages + blk * PB, page < 0 ? 0 : PB);
+    const auto rv = buf_rsrc(p.kv.v_pages + blk * PB, page < 0 ? 0 : PB);
 #pragma unroll
-    for (int i = 0; i < NC; ++i) {
-      kr[i] = page >= 0 ? ld_u32x4(p.kv.k_pages + blk * PB + 16 * (tid + 256 * i)) : zero;
-      vr[i] = page >= 0 ? ld_u32x4(p.kv.v_pages + blk * PB + 16 * (tid + 256 * i)) : zero;
+    for (int i = 0; i < NP; ++i) {
+      raw[i] = buf_ld(rk, 16 * tid + 4096 * i);
+      raw[NP + i] = buf_ld(rv, 16 * tid + 4096 * i);
     }
-    if (tid < DTREE_PAGE) {
-      ksl = page >= 0 ? p.kv.k_scales[blk * DTREE_PAGE + tid] : 0.f;
-      vsl = page >= 0 ? p.kv.v_scales[blk * DTREE_PAGE + tid] : 0.f;
-    }
+    const auto sk = buf_rsrc(p.kv.k_scales + blk * DTREE_PAGE, page < 0 ? 0 : 4 * DTREE_PAGE);
+    const auto sv = buf_rsrc(p.kv.v_scales + blk * DTREE_PAGE, page < 0 ? 0 : 4 * DTREE_PAGE);
+    ksl = buf_ldf(sk, 4 * tid);  // (threads past the page's positions read 0)
+    vsl = buf_ldf(sv, 4 * tid);
     return page >= 0;
   };
-  bool here = load(t0), next = false;
-  static_assert(sizeof(kvb) >= 32 * kWaves * (D + 8) * sizeof(uint16_t), "the queries pass through kvb");
-  uint16_t* qs = reinterpret_cast<uint16_t*>(&kvb[0][0]);
-  q8_ancestors(p, q, pair0, 32 * kWaves, pairs, anc);
-  const float inv = q8_queries<D, 32 * kWaves, kWaves>(p, q, g, pair0, pairs, qs, wmax);
-  u32x4_t qf[D / 16];
+  bool here = load(0);
+  q8_ancestors(p, q, pair0, WP, pairs, anc);
+  const float inv = q8_queries<D, WP, kWaves>(p, q, g, pair0, pairs, lds.q, wmax);
+  u32x4_t qf[NC][NF];
+  int pos[NC];  // the lane's positions; -1: no pair
 #pragma unroll
-  for (int i = 0; i < D / 16; ++i)
-    qf[i] = *reinterpret_cast<const u32x4_t*>(qs + (32 * wave + c) * (D + 8) + 32 * (i >> 1) + 16 * h + 8 * (i & 1));
-  lds_barrier();
-  auto stage = [&](int buf) {
+  for (int n = 0; n < NC; ++n) {
+    const int l = CP * wave + 32 * n + c;
+    pos[n] = pair0 + l < pairs ? q.past + (pair0 + l) / p.G : -1;
 #pragma unroll
-    for (int i = 0; i < NC; ++i) {
-      const int u = tid + 256 * i;
-      unsigned char* at = &kvb[buf][(u >> 6) * 2048 + (u & 63) * 16];
-      u32x4_t a0, a1;
-      q8_to_h16(kr[i], a0, a1);
-      *reinterpret_cast<u32x4_t*>(at) = a0;
-      *reinterpret_cast<u32x4_t*>(at + 1024) = a1;
-      q8_to_h16(vr[i], a0, a1);
-      *reinterpret_cast<u32x4_t*>(at + 2 * PB) = a0;
-      *reinterpret_cast<u32x4_t*>(at + 2 * PB + 1024) = a1;
+    for (int i = 0; i < NF; ++i)
+{
+      qf[n][i] = *reinterpret_cast<const u32x4_t*>(lds.q + l * (D + 8) + 32 * (i >> 1) + 16 * h + 8 * (i & 1));
+      if constexpr (NC == 2 || D == 256) asm("" : "+a"(qf[n][i]));
     }
+  }
+  lds_barrier();
+  auto stage_scales = [&](int buf) {
     if (tid < DTREE_PAGE) {
       float k, lv, iv;
       q8_scales(ksl, vsl, inv, k, lv, iv);
@@ -672,60 +657,227 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void q8_rows_kernel(AttnQ8Pa
       scl[buf][128 + tid] = iv;
     }
   };
-  const Q8Mask mask = q8_mask(p, q, live, r, anc[32 * wave + c]);
-  f32x16_t o[NB];
+  // Word j of piece i (K's pieces, then V's) of the raw page; its fragments go out
+  // when they are whole.
+  u32x4_t half;
+  auto stage_word = [&](int buf, int i, int j) {
+    const int u = tid + 256 * (i % NP);
+    uint32_t lo, hi;
+    q8_word_to_h4(raw[i][j], lo, hi);
+    half[2 * (j & 1)] = lo;
+    half[2 * (j & 1) + 1] = hi;
+    if (j & 1)
+      *reinterpret_cast<u32x4_t*>(
+          &lds.kv[buf][(i / NP) * 2 * PB + (u >> 6) * 2048 + (j >> 1) * 1024 + (u & 63) * 16]) = half;
+  };
+  f32x16_t o[NC][NB], sa[NC], sb[NC];  // sa, sb: the logits of even and odd steps
+  u32x4_t ph[NC][2], kf[RF], vf[RF];
+  f32x4_t ks[4], lv[4], iv[4];
+  float m[NC], l[NC], mx[NC];
 #pragma unroll
-  for (int db = 0; db < NB; ++db)
+  for (int n = 0; n < NC; ++n) {
+    m[n] = kFloor;
+    l[n] = 0.f;
+    ph[n][0] = ph[n][1] = u32x4_t{0, 0, 0, 0};
 #pragma unroll
-    for (int i = 0; i < 16; ++i) o[db][i] = 0.f;
-  float m = kFloor, l = 0.f;
-  stage(0);
-  __syncthreads();
-  for (int t = t0; t < t1; ++t) {
-    const int buf = (t - t0) & 1, k0 = DTREE_PAGE * rg.page(t);
-    if (t + 1 < t1) next = load(t + 1);
-    const int wend = q.past + (mask.tree ? q.n - 1 : wto);  // the wave's last key
-    const bool need = here && wlive && k0 <= wend &&
-                      (p.a.window == 0 || k0 < p.a.sink || k0 + DTREE_PAGE - 1 > q.past + wfrom - p.a.window);
-    if (need) {
-      const unsigned char* kp = kvb[buf] + 16 * lane;
-      const unsigned char* vp = kp + 2 * PB;
-      const bool masked = mask.tree ? k0 + DTREE_PAGE > q.past
-                                    : k0 + DTREE_PAGE - 1 > q.past + wfrom ||
-                                          (p.a.window > 0 && k0 + DTREE_PAGE - 1 >= p.a.sink &&
-                                           q.past + wto - k0 >= p.a.window);
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        f32x16_t st;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) st[i] = 0.f;
-#pragma unroll
-        for (int i = 0; i < 2 * NB; ++i)
-          st = mfma32_f16(*reinterpret_cast<const u32x4_t*>(kp + (b * 2 * NB + i) * 1024), qf[i], st);
-        u32x4_t ph[2];
-        q8_softmax<NB>(st, scl[buf], b, h, masked, mask, k0, m, l, o, ph);
-#pragma unroll
-        for (int db = 0; db < NB; ++db)
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-            o[db] = mfma32_f16(*reinterpret_cast<const u32x4_t*>(vp + ((b * NB + db) * 2 + i) * 1024), ph[i], o[db]);
-      }
-    }
-    if (t + 1 < t1) stage(buf ^ 1);
-    here = next;
-    __syncthreads();
-  }
-  l += __shfl_xor(l, 32);
-  if (live) {
+    for (int i = 0; i < 16; ++i) sb[n][i] = -INFINITY;  // the step before the first: no keys
 #pragma unroll
     for (int db = 0; db < NB; ++db)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float y[4] = {o[db][4 * i], o[db][4 * i + 1], o[db][4 * i + 2], o[db][4 * i + 3]};
-        q8_emit(p, used > 1, part, row, head, 32 * db + 8 * i + 4 * h, y, m, l);
+      for (int i = 0; i < 16; ++i) o[n][db][i] = 0.f;
+  }
+  // Fragment f of a half page: K's dims 16 f ..; V's keys 16 (f / NB) .., dims 32 (f % NB) ..
+  auto k_frag = [&](int buf, int b, int f) {
+    return *reinterpret_cast<const u32x4_t*>(&lds.kv[buf][b * PB + 1024 * f + 16 * lane]);
+  };
+  auto v_frag = [&](int buf, int b, int f) {
+    return *reinterpret_cast<const u32x4_t*>(&lds.kv[buf][2 * PB + b * PB + 1024 * (2 * (f % NB) + f / NB) + 16 * lane]);
+  };
+  auto consts = [&](f32x4_t (&x)[4], int buf, int which, int b) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const f32x4_t*>(&scl[buf][64 * which + 32 * b + 8 * i + 4 * h]);
+  };
+  auto weight = [&](f32x16_t (&x)[NC], int n, int r) {
+    x[n][r] = fast_exp2(x[n][r] - m[n]);
+    l[n] = fmaf(x[n][r], iv[r / 4][r % 4], l[n]);
+    if (r & 1) ph[n][r >> 3][(r >> 1) & 3] = pack_h2(x[n][r - 1], x[n][r]);
+  };
+  // PV of the last step (its V: half vh of buffer vb; its logits `old`), the logits
+  // `cur` of this one (half b of buffer buf); STAGE: the raw page to buffer sbuf.
+  auto block1 = [&](f32x16_t (&old)[NC], f32x16_t (&cur)[NC], int vbuf, int vh, int buf, int b, auto stage, int sbuf) {
+    constexpr int ST = NS / 2 > 2 ? NS / 2 - 1 : 1;  // slots of the logits
+    constexpr int SW = 8 * NP / NS;                  // words converted per slot
+    consts(ks, buf, 0, b);
+    consts(lv, buf, 1, b);
+#pragma unroll
+    for (int n = 0; n < NC; ++n) mx[n] = kFloor;
+#pragma unroll
+    for (int k = 0; k < NS; ++k) {
+      const int f = k / NC, n = k % NC;
+      o[n][f % NB] = mfma32_f16(vf[f % RF], ph[n][f / NB], o[n][f % NB]);
+      if (n == NC - 1 && f + RF < NF) vf[f % RF] = v_frag(vbuf, vh, f + RF);
+      if constexpr (decltype(stage)::value) {
+#pragma unroll
+        for (int i = k * SW; i < (k + 1) * SW; ++i) stage_word(sbuf, i / 4, i % 4);
       }
-  } else if (part == 0 && r < p.a.rows_padded && h == 0) {
-    for (int d = 0; d < D; d += 4) q8_store_zero(p, r, head, d);
+      if (k < NS / 2) {
+#pragma unroll
+        for (int e = k * EV / NS; e < (k + 1) * EV / NS; ++e) weight(old, e % NC, 8 + e / NC);
+      } else {
+        const int j = k - NS / 2;
+        if (j < ST) {
+#pragma unroll
+          for (int e = j * EV / ST; e < (j + 1) * EV / ST; ++e) {
+            const int r = e / NC, en = e % NC;
+            cur[en][r] = fmaf(cur[en][r], ks[r / 4][r % 4], lv[r / 4][r % 4]);
+            mx[en] = fmaxf(mx[en], cur[en][r]);
+          }
+        }
+        if (j == NS / 2 - 1) {
+#pragma unroll
+          for (int en = 0; en < NC; ++en) mx[en] = max_halves(mx[en]);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  // What the rows may not see; the output rescaled where a row's maximum has grown.
+  auto limits = [&](f32x16_t (&cur)[NC], bool masked, bool there, int key0) {
+    if (masked) {
+#pragma unroll
+      for (int n = 0; n < NC; ++n) {
+        const uint32_t sees = there ? q8_sees(p, q, pos[n], key0, anc[CP * wave + 32 * n + c]) >> (4 * h) : 0u;
+        mx[n] = kFloor;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          cur[n][r] = sees & (1u << acc_row(r, 0)) ? cur[n][r] : -INFINITY;
+          mx[n] = fmaxf(mx[n], cur[n][r]);
+        }
+        mx[n] = max_halves(mx[n]);
+      }
+    }
+    bool grown = false;
+#pragma unroll
+    for (int n = 0; n < NC; ++n) grown |= mx[n] > m[n] + (kTop + kSlack);
+    if (__any(grown)) {
+#pragma unroll
+      for (int n = 0; n < NC; ++n) {
+        const float mn = mx[n] > m[n] + (kTop + kSlack) ? mx[n] - kTop : m[n], alpha = fast_exp2(m[n] - mn);
+        m[n] = mn;
+        l[n] *= alpha;
+#pragma unroll
+        for (int db = 0; db < NB; ++db)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[n][db][r] *= alpha;
+      }
+    }
+  };
+  auto k_ahead = [&](int buf, int b) {
+#pragma unroll
+    for (int f = 0; f < RF; ++f) kf[f] = k_frag(buf, b, f);
+  };
+  // S of the next step (half b of buffer buf) to `next`, the weights of `cur`'s
+  // first 16 keys, the first V fragments (half vh of vbuf) of the next block1.
+  auto block2 = [&](f32x16_t (&cur)[NC], f32x16_t (&next)[NC], int buf, int b, int vbuf, int vh) {
+#pragma unroll
+    for (int n = 0; n < NC; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) next[n][r] = 0.f;
+#pragma unroll
+    for (int k = 0; k < NS; ++k) {
+      const int f = k / NC, n = k % NC;
+      next[n] = mfma32_f16(kf[f % RF], qf[n][f], next[n]);
+      if (n == NC - 1 && f + RF < NF) kf[f % RF] = k_frag(buf, b, f + RF);
+      if (n == NC - 1 && f + RF >= NF) vf[f + RF - NF] = v_frag(vbuf, vh, f + RF - NF);
+#pragma unroll
+      for (int e = k * (EV / 2) / NS; e < (k + 1) * (EV / 2) / NS; ++e) weight(cur, e % NC, e / NC);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int n = 0; n < NC; ++n) asm volatile("" : "+v"(ph[n][0]), "+v"(l[n]));  // taken here, not sunk to their use
+  };
+  auto hidden = [&](int k0) {  // does a page hold keys that some row may not see
+    return p.a.ancestors ? k0 + DTREE_PAGE > q.past
+                         : k0 + DTREE_PAGE - 1 > q.past + wfrom ||
+                               (p.a.window > 0 && k0 + DTREE_PAGE - 1 >= p.a.sink && q.past + wto - k0 >= p.a.window);
+  };
+  stage_scales(0);
+#pragma unroll
+  for (int i = 0; i < 2 * NP; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) stage_word(0, i, j);
+  bool next = load(1);
+  lds_barrier();
+  // S of the first step. PV of none before it: zero weights times the first page.
+  consts(iv, 0, 2, 0);
+  k_ahead(0, 0);
+  block2(sb, sa, 0, 0, 0, 0);
+  int vbuf = 0, vh = 0;  // where the last step's V is
+  for (int t = t0; t < t1; ++t) {
+    const int buf = (t - t0) & 1, k0 = DTREE_PAGE * rg.page(t);
+    const bool masked = !here || hidden(k0);
+    block1(sb, sa, vbuf, vh, buf, 0, std::false_type{}, 0);
+    k_ahead(buf, 1);
+    consts(iv, buf, 2, 0);
+    limits(sa, masked, here, k0);
+    block2(sa, sb, buf, 1, buf, 0);
+    lds_barrier();  // the other buffer's last readers are done
+    stage_scales(buf ^ 1);
+    block1(sa, sb, buf, 0, buf, 1, std::true_type{}, buf ^ 1);
+    lds_barrier();  // page t + 1 is there
+    k_ahead(buf ^ 1, 0);
+    consts(iv, buf, 2, 1);
+    limits(sb, masked, here, k0 + 32);
+    const bool soon = load(t + 2 - t0);
+    block2(sb, sa, buf ^ 1, 0, buf, 1);
+    vbuf = buf;
+    vh = 1;
+    here = next;
+    next = soon;
+  }
+  block1(sb, sa, vbuf, vh, vbuf, 0, std::false_type{}, 0);
+  lds_barrier();  // every wave has read the pages
+  // The outputs through LDS, each wave its own part: rows of D values, 8 a lane.
+  const bool plain = used == 1 && p.plain;
+#pragma unroll
+  for (int n = 0; n < NC; ++n) {
+    const float lt = l[n] + __shfl_xor(l[n], 32);
+    if (wpair + 32 * n >= pairs) break;
+    float* red = lds.red[wave];
+#pragma unroll
+    for (int db = 0; db < NB; ++db)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<f32x4_t*>(red + c * RS + 32 * db + 8 * i + 4 * h) =
+            f32x4_t{o[n][db][4 * i], o[n][db][4 * i + 1], o[n][db][4 * i + 2], o[n][db][4 * i + 3]};
+    if (h == 0) {  // the pair's row, head, m and l or 1 / l behind its values
+      const int pair = wpair + 32 * n + c, row = pair / p.G;
+      *reinterpret_cast<f32x4_t*>(red + c * RS + D) =
+          f32x4_t{m[n], used > 1 ? lt : q8_inverse(lt), __int_as_float(row), __int_as_float(pair - row * p.G)};
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    const int nl = min(32, pairs - wpair - 32 * n) * (D / 8);
+#pragma unroll 2
+    for (int e = lane; e < nl; e += 64) {
+      const int pl = e / (D / 8), d = 8 * (e % (D / 8));
+      const f32x4_t x0 = *reinterpret_cast<const f32x4_t*>(red + pl * RS + d);
+      const f32x4_t x1 = *reinterpret_cast<const f32x4_t*>(red + pl * RS + d + 4);
+      const f32x4_t of = *reinterpret_cast<const f32x4_t*>(red + pl * RS + D);
+      const size_t row = (size_t)q.start + __float_as_int(of[2]);
+      const int head = g * p.G + __float_as_int(of[3]);
+      if (plain) {  // rows of bf16, 16 bytes a lane
+        const f32x4_t y0 = x0 * of[1], y1 = x1 * of[1];
+        *reinterpret_cast<u32x4_t*>(p.a.out + row * p.a.ld_out + head * D + d) =
+            u32x4_t{pack_bf2(y0[0], y0[1]), pack_bf2(y0[2], y0[3]), pack_bf2(y1[0], y1[1]), pack_bf2(y1[2], y1[3])};
+      } else {
+        const float a0[4] = {x0[0], x0[1], x0[2], x0[3]}, a1[4] = {x1[0], x1[1], x1[2], x1[3]};
+        q8_emit(p, used > 1, part, row, head, d, a0, of[0], of[1], of[1]);
+        q8_emit(p, used > 1, part, row, head, d + 4, a1, of[0], of[1], of[1]);
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
   }
 }
 
@@ -743,9 +895,9 @@ __global__ __launch_bounds__(256) void q8_join_kernel(AttnQ8Params p) {
   if (blockIdx.x * PPB >= q.n * p.a.num_heads) return;
   int from = 0, to = q.n - 1;  // the rows of its workgroup
   if constexpr (!TOKENS) {
-    const int pair0 = (r * p.G + head % p.G) / (32 * kWaves) * (32 * kWaves);
+    const int pair0 = (r * p.G + head % p.G) / p.pairs_wg * p.pairs_wg;
     from = min(pair0 / p.G, q.n - 1);
-    to = min(q.n - 1, (pair0 + 32 * kWaves - 1) / p.G);
+    to = min(q.n - 1, (pair0 + p.pairs_wg - 1) / p.G);
   }
   const int tiles = q8_range(p, q, from, to).tiles, used = q8_parts(p, tiles);
   const bool live = r < q.n && used > 1;
@@ -803,12 +955,13 @@ __global__ __launch_bounds__(256) void q8_join_kernel(AttnQ8Params p) {
       for (int e = 0; e < 4; ++e) o[e] = fmaf(f, sums[k][tid % (TPP * PPB)][e], o[e]);
     }
   }
-  if (live) q8_emit(p, false, 0, row, head, d, o, m, l);
+  if (live) q8_emit(p, false, 0, row, head, d, o, m, l, q8_inverse(l));
 }
 
 // The launch for a record: which kernel, its grid and key ranges.
 struct Plan {
   bool tokens;
+  int nc;  // column blocks: 16 pairs (tokens) or 32 (rows) each
   int blocks, parts, per;
 };
 
@@ -817,20 +970,22 @@ size_t part_bytes(const DtreeKvQ8& kv, const DtreeAttnQ8Args& a) {
 }
 
 // Workgroups the key ranges are cut for, and the fewest pages of a range.
-constexpr int kFillTokens = 2048, kFillRows = 512;
+constexpr int kFillTokens = 4096, kFillRows = 512;
 constexpr int kMinTokens = 16, kMinRows = 4;
 
 Plan make_plan(const DtreeKvQ8& kv, const DtreeAttnQ8Args& a) {
-  const int G = a.num_heads / kv.num_kv_heads;
+  const int G = a.num_heads / kv.num_kv_heads, D = kv.head_dim;
   Plan pl{};
   const int64_t pairs = (int64_t)std::max(kv.max_rows, a.rows_padded) * G;
-  pl.tokens = pairs <= (kv.head_dim == 256 ? 16 : 32);  // (registers: 32 columns of 256 dims do not fit)
-  pl.blocks = pl.tokens ? 1 : (int)((pairs + 32 * kWaves - 1) / (32 * kWaves));
+  pl.tokens = pairs <= (D == 256 ? 16 : 32);  // (registers: 32 columns of 256 dims do not fit)
+  pl.nc = pl.tokens ? (pairs <= 16 ? 1 : 2) : (D == 256 || pairs <= 32 * kWaves ? 1 : 2);
+  const int wp = 32 * kWaves * pl.nc;  // pairs of a workgroup of rows
+  pl.blocks = pl.tokens ? 1 : (int)((pairs + wp - 1) / wp);
   // pages that one workgroup's rows can see
   const int64_t end = std::min((int64_t)kv.max_past_length + kv.max_rows, (int64_t)kv.ld_page_table * DTREE_PAGE);
   int64_t tiles = (end + DTREE_PAGE - 1) / DTREE_PAGE;
   if (a.window > 0) {
-    const int64_t span = pl.tokens ? kv.max_rows : std::min(kv.max_rows, 32 * kWaves / G + 2);
+    const int64_t span = pl.tokens ? kv.max_rows : std::min(kv.max_rows, wp / G + 2);
     tiles = std::min(tiles, ((int64_t)a.sink + DTREE_PAGE - 1) / DTREE_PAGE + (a.window + span) / DTREE_PAGE + 2);
   }
   const int64_t units = (int64_t)kv.num_seqs * kv.num_kv_heads * pl.blocks;
@@ -854,14 +1009,17 @@ int launch_join(const AttnQ8Params& p, hipStream_t stream) {
 }
 
 template <int D>
-int launch(const AttnQ8Params& p, bool tokens, unsigned grid, hipStream_t stream) {
-  if (!tokens) q8_rows_kernel<D><<<grid, 256, 0, stream>>>(p);
-  else if (D == 256 || std::max(p.kv.max_rows, p.a.rows_padded) * p.G <= 16)
-    q8_token_kernel<D, 1><<<grid, 256, 0, stream>>>(p);
-  else if constexpr (D != 256) q8_token_kernel<D, 2><<<grid, 256, 0, stream>>>(p);
+int launch(const AttnQ8Params& p, const Plan& pl, unsigned grid, hipStream_t stream) {
+  if (pl.nc == 1) {
+    if (pl.tokens) q8_token_kernel<D, 1><<<grid, 256, 0, stream>>>(p);
+    else q8_rows_kernel<D, 1><<<grid, 256, 0, stream>>>(p);
+  } else if constexpr (D != 256) {
+    if (pl.tokens) q8_token_kernel<D, 2><<<grid, 256, 0, stream>>>(p);
+    else q8_rows_kernel<D, 2><<<grid, 256, 0, stream>>>(p);
+  }
   DTREE_LAUNCH_CHECK("attention_q8 launch");
   if (p.parts == 1) return DTREE_OK;
-  return tokens ? launch_join<D, true>(p, stream) : launch_join<D, false>(p, stream);
+  return pl.tokens ? launch_join<D, true>(p, stream) : launch_join<D, false>(p, stream);
 }
 
 bool q8_geometry(const DtreeKvQ8& kv, const DtreeAttnQ8Args& a) {
@@ -924,6 +1082,7 @@ extern "C" int dtree_attention_q8(const DtreeKvQ8* kv, const DtreeAttnQ8Args* a,
   p.a = *a;
   p.G = a->num_heads / kv->num_kv_heads;
   p.blocks = pl.blocks;
+  p.pairs_wg = 32 * kWaves * pl.nc;
   p.parts = pl.parts;
   p.per = pl.per;
   p.sink_pages = (a->sink + DTREE_PAGE - 1) / DTREE_PAGE;
@@ -933,11 +1092,12 @@ extern "C" int dtree_attention_q8(const DtreeKvQ8* kv, const DtreeAttnQ8Args* a,
   p.tiled = tiled;
   p.h16 = a->out_layout == DTREE_W_TILED_F16;
   if (p.h16) p.a.out_lo = nullptr;
+  p.plain = !tiled && !p.a.out_lo && !a->gated && ((uintptr_t)a->out & 15) == 0 && a->ld_out % 8 == 0;
   const int64_t grid = (int64_t)kv->num_seqs * pl.blocks * pl.parts * kv->num_kv_heads;
   DTREE_REQUIRE(grid < (int64_t)1 << 31 && (int64_t)kv->max_rows * a->num_heads < (int64_t)1 << 31 &&
                     (pl.parts == 1 || kv->num_seqs <= 65535),
                 "attention_q8: num_seqs * max_rows too large for one launch");
-  if (D == 64) return launch<64>(p, pl.tokens, (unsigned)grid, stream);
-  if (D == 128) return launch<128>(p, pl.tokens, (unsigned)grid, stream);
-  return launch<256>(p, pl.tokens, (unsigned)grid, stream);
+  if (D == 64) return launch<64>(p, pl, (unsigned)grid, stream);
+  if (D == 128) return launch<128>(p, pl, (unsigned)grid, stream);
+  return launch<256>(p, pl, (unsigned)grid, stream);
 }
