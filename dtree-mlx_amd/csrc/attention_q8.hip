@@ -90,7 +90,7 @@ __device__ __forceinline__ float max_halves(float a) {
   return a;
 }
 
-// 2^e that takes amax into [2^13, 2^14), and its inverse.
+// 2^e that takes a bound on the values into [2^13, 2^14), and its inverse.
 __device__ __forceinline__ void q8_exponent(float amax, float& f, float& inv) {
   const int e = (int)(__float_as_uint(amax) >> 23);
   const int ef = amax > 0.f ? min(max(267 - e, 1), 253) : 127;
@@ -117,108 +117,152 @@ __device__ __forceinline__ f32x4_t q8_bf4(u32x2_t w) {
                  __uint_as_float(w[1] & 0xffff0000u)};
 }
 
+// Max over the TPR = D / 8 lanes of a pair.
+template <int TPR>
+__device__ __forceinline__ float q8_max_lanes(float a) {
+  a = fmaxf(a, dpp<0xB1>(a));
+  a = fmaxf(a, dpp<0x4E>(a));
+  a = fmaxf(a, dpp<0x141>(a));
+  if constexpr (TPR >= 16) a = fmaxf(a, dpp<0x140>(a));
+  if constexpr (TPR >= 32) a = fmaxf(a, swz_xor16(a));
+  return a;
+}
+
 // The queries of up to PAIRS pairs from pair0 on (q_norm, RoPE, the softmax scale
 // in log2 units), in fp16 at qs[pair][D + 8] (past `pairs`: the last row's, their
-// results unread), moved by one power of two for the workgroup; returns its
-// inverse. WAVES waves; the barriers wait for LDS alone. A row's 1 / rms joins the
-// power of two, after the rotation.
-template <int D, int PAIRS, int WAVES>
-__device__ __forceinline__ float q8_queries(const AttnQ8Params& p, const Q8Seq& q, int g, int pair0, int pairs,
-                                            uint16_t* qs, float* wmax) {
-  constexpr int TPR = D / 8, NT = 64 * WAVES, PPR = NT / TPR, NR = (PAIRS + PPR - 1) / PPR;  // PPR pairs a round
+// results unread), moved by one power of two for the workgroup, whose inverse is
+// returned: from a bound on the values, sqrt(2 D) max |w| behind an RMSNorm, else
+// sqrt(2) times the largest finite one. W waves; the barriers wait for LDS alone.
+// No load is in a branch, so that a batch's loads go out together: lanes without a
+// rotation read a table's first entries, calls without one the row.
+template <int D, int PAIRS, int W, bool BF>
+__device__ __forceinline__ float q8_queries_of(const AttnQ8Params& p, const Q8Seq& q, int g, int pair0, uint16_t* qs,
+                                               float* wmax) {
+  constexpr int TPR = D / 8, NT = 64 * W, PPR = NT / TPR;  // PPR pairs a round
+  constexpr int NR = (PAIRS + PPR - 1) / PPR, BR = NR < 8 ? NR : 8;  // rounds; rounds in flight
+  constexpr int SZ = BF ? 2 : 4;
+  static_assert(NR % BR == 0, "whole batches of rounds");
   const int tid = threadIdx.x, j = tid % TPR;
-  const bool bf = p.a.q_type == DTREE_T_BF16;
   const int half = p.a.rope_dims / 2;
   const Q8Pieces pc = q8_pieces<D>(p.a.rope_dims, j);
-  f32x4_t x[NR][2], cs[NR], sn[NR], w[2];
-  // No load in a branch of a lane's own, so that all go out together: lanes
-  // without a rotation read the table's first entries.
-  int m = pair0 + tid / TPR, r = m / p.G, hd = m - r * p.G;
+  // Pair to pair in steps of PPR: dr rows and dh heads on, one row more where the
+  // heads wrap; past the last row it stays there.
   const int dr = PPR / p.G, dh = PPR % p.G;
-#pragma unroll
-  for (int k = 0; k < NR; ++k) {
-    const size_t row = (size_t)q.start + min(r, q.n - 1);
-    const size_t base = row * p.a.ld_q + (size_t)(g * p.G + hd) * p.a.q_stride;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      if (bf) x[k][i] = q8_bf4(*reinterpret_cast<const u32x2_t*>(static_cast<const uint16_t*>(p.a.q) + base + pc.at[i]));
-      else x[k][i] = *reinterpret_cast<const f32x4_t*>(static_cast<const float*>(p.a.q) + base + pc.at[i]);
-    }
-    if (half) {  // (tables and weights at any address of their type)
-      const size_t at = row * half + (pc.turns ? 4 * j : 0);
-      __builtin_memcpy(&cs[k], p.a.rope_cos + at, 16);
-      __builtin_memcpy(&sn[k], p.a.rope_sin + at, 16);
+  const int r0 = (pair0 + tid / TPR) / p.G, h0 = pair0 + tid / TPR - r0 * p.G;
+  const char* const base0 = static_cast<const char*>(p.a.q) + (size_t)q.start * p.a.ld_q * SZ;
+  int r = r0, hd = h0;
+  auto load = [&](u32x4_t& x0, u32x4_t& x1, size_t& row, const char*& base) {
+    const int rr = min(r, q.n - 1);
+    row = (size_t)q.start + rr;
+    base = base0 + ((size_t)rr * (unsigned)p.a.ld_q + (unsigned)((g * p.G + hd) * p.a.q_stride)) * SZ;
+    if constexpr (BF) {
+      const u32x2_t a = *reinterpret_cast<const u32x2_t*>(base + 2 * pc.at[0]);
+      const u32x2_t b = *reinterpret_cast<const u32x2_t*>(base + 2 * pc.at[1]);
+      x0 = u32x4_t{a[0], a[1], 0, 0};
+      x1 = u32x4_t{b[0], b[1], 0, 0};
+    } else {
+      x0 = ld_u32x4(base + 4 * pc.at[0]);
+      x1 = ld_u32x4(base + 4 * pc.at[1]);
     }
     r += dr;
     hd += dh;
-    if (hd >= p.G) {
-      hd -= p.G;
-      ++r;
-    }
-  }
+    const bool wrap = hd >= p.G;
+    hd -= wrap ? p.G : 0;
+    r += wrap ? 1 : 0;
+  };
+  auto value = [](u32x4_t x) {
+    if constexpr (BF) return q8_bf4(u32x2_t{x[0], x[1]});
+    else return __builtin_bit_cast(f32x4_t, x);
+  };
+  const bool norm = p.a.q_norm != nullptr;
+  f32x4_t w0 = {p.scale_log2, p.scale_log2, p.scale_log2, p.scale_log2}, w1 = w0;
+  float f, inv, bound = 0.f;
+  if (norm) {
+    u32x2_t a, b;  // (tables and weights at any address of their type)
+    __builtin_memcpy(&a, p.a.q_norm + pc.at[0], 8);
+    __builtin_memcpy(&b, p.a.q_norm + pc.at[1], 8);
+    w0 *= q8_bf4(a);
+    w1 *= q8_bf4(b);
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    w[i] = f32x4_t{p.scale_log2, p.scale_log2, p.scale_log2, p.scale_log2};
-    if (p.a.q_norm) {
-      u32x2_t v;
-      __builtin_memcpy(&v, p.a.q_norm + pc.at[i], 8);
-      w[i] *= q8_bf4(v);
+    for (int e = 0; e < 4; ++e) {
+      const float m = fmaxf(fabsf(w0[e]), fabsf(w1[e]));
+      bound = m < INFINITY ? fmaxf(bound, m) : bound;
     }
-  }
-  float amax = 0.f, rs[NR];
+    bound = q8_max_lanes<TPR>(bound) * sqrtf(2.f * D);
+  } else {
+#pragma unroll 1
+    for (int k = 0; k < NR; ++k) {
+      u32x4_t x0, x1;
+      size_t row;
+      const char* base;
+      load(x0, x1, row, base);
+      const f32x4_t a = value(x0), b = value(x1);
 #pragma unroll
-  for (int k = 0; k < NR; ++k) {
-    rs[k] = 1.f;
-    if (p.a.q_norm) {
+      for (int e = 0; e < 4; ++e) {
+        bound = fabsf(a[e]) < INFINITY ? fmaxf(bound, fabsf(a[e])) : bound;  // (what is not finite stays in its row)
+        bound = fabsf(b[e]) < INFINITY ? fmaxf(bound, fabsf(b[e])) : bound;
+      }
+    }
+    r = r0;
+    hd = h0;
+    bound = max_halves(q8_max_lanes<32>(bound));
+    if ((tid & 63) == 0) wmax[tid >> 6] = bound;
+    lds_barrier();
+#pragma unroll
+    for (int k = 0; k < W; ++k) bound = fmaxf(bound, wmax[k]);
+    bound *= p.scale_log2 * 1.4142136f;
+  }
+  q8_exponent(bound, f, inv);
+#pragma unroll 1
+  for (int k0 = 0; k0 < NR; k0 += BR) {
+    u32x4_t x[BR][2];
+    f32x4_t cs[BR], sn[BR];
+#pragma unroll
+    for (int k = 0; k < BR; ++k) {
+      size_t row;
+      const char* base;
+      load(x[k][0], x[k][1], row, base);
+      const size_t at = 4 * (row * half + (pc.turns ? 4 * j : 0));
+      const char* tc = half ? reinterpret_cast<const char*>(p.a.rope_cos) + at : base;
+      const char* ts = half ? reinterpret_cast<const char*>(p.a.rope_sin) + at : base;
+      __builtin_memcpy(&cs[k], tc, 16);
+      __builtin_memcpy(&sn[k], ts, 16);
+    }
+#pragma unroll
+    for (int k = 0; k < BR; ++k) {
+      const f32x4_t x0 = value(x[k][0]), x1 = value(x[k][1]);
       float ss = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) ss = fmaf(x[k][e >> 2][e & 3], x[k][e >> 2][e & 3], ss);
-      ss += dpp<0xB1>(ss);  // TPR lanes: of 2, 4, 8, 16, 32
+      for (int e = 0; e < 4; ++e) ss = fmaf(x0[e], x0[e], fmaf(x1[e], x1[e], ss));
+      ss += dpp<0xB1>(ss);
       ss += dpp<0x4E>(ss);
       ss += dpp<0x141>(ss);
       if constexpr (TPR >= 16) ss += dpp<0x140>(ss);
       if constexpr (TPR >= 32) ss += swz_xor16(ss);
-      rs[k] = rsqrtf(ss * (1.0f / D) + p.a.eps);
-    }
-    float mx = 0.f;
+      const float rs = norm ? f * __builtin_amdgcn_rsqf(ss * (1.0f / D) + p.a.eps) : f;  // (1 ulp; fp16 follows)
+      f32x4_t y, z;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float y = x[k][0][e] * w[0][e], z = x[k][1][e] * w[1][e];
-      x[k][0][e] = y;
-      x[k][1][e] = z;
-      if (half) {  // (a select, not sn = 0, which would carry an infinity to another dim)
-        x[k][0][e] = pc.turns ? y * cs[k][e] - z * sn[k][e] : y;
-        x[k][1][e] = pc.turns ? y * sn[k][e] + z * cs[k][e] : z;
+      for (int e = 0; e < 4; ++e) {
+        const float a = x0[e] * w0[e], b = x1[e] * w1[e];
+        // (a select, not sn = 0, which would carry an infinity to another dim)
+        y[e] = (pc.turns ? a * cs[k][e] - b * sn[k][e] : a) * rs;
+        z[e] = (pc.turns ? a * sn[k][e] + b * cs[k][e] : b) * rs;
       }
-      mx = fmaxf(mx, fmaxf(fabsf(x[k][0][e]), fabsf(x[k][1][e])));
-    }
-    mx *= rs[k];
-    amax = mx < INFINITY ? fmaxf(amax, mx) : amax;  // (a row that is not finite is NaN whatever its exponent)
-  }
-  amax = fmaxf(amax, dpp<0xB1>(amax));
-  amax = fmaxf(amax, dpp<0x4E>(amax));
-  amax = fmaxf(amax, dpp<0x141>(amax));
-  amax = fmaxf(amax, dpp<0x140>(amax));
-  amax = fmaxf(amax, swz_xor16(amax));
-  amax = max_halves(amax);
-  if ((tid & 63) == 0) wmax[tid >> 6] = amax;
-  lds_barrier();
-#pragma unroll
-  for (int k = 0; k < WAVES; ++k) amax = fmaxf(amax, wmax[k]);
-  float f, inv;
-  q8_exponent(amax, f, inv);
-#pragma unroll
-  for (int k = 0; k < NR; ++k) {
-    const int pl = tid / TPR + k * PPR;
-    if (PAIRS % PPR != 0 && pl >= PAIRS) continue;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const f32x4_t y = x[k][i] * rs[k] * f;
-      *reinterpret_cast<u32x2_t*>(qs + pl * (D + 8) + pc.at[i]) = u32x2_t{pack_h2(y[0], y[1]), pack_h2(y[2], y[3])};
+      const int pl = tid / TPR + (k0 + k) * PPR;
+      if (PAIRS % PPR == 0 || pl < PAIRS) {
+        *reinterpret_cast<u32x2_t*>(qs + pl * (D + 8) + pc.at[0]) = u32x2_t{pack_h2(y[0], y[1]), pack_h2(y[2], y[3])};
+        *reinterpret_cast<u32x2_t*>(qs + pl * (D + 8) + pc.at[1]) = u32x2_t{pack_h2(z[0], z[1]), pack_h2(z[2], z[3])};
+      }
     }
   }
   lds_barrier();
   return inv;
+}
+template <int D, int PAIRS, int W>
+__device__ __forceinline__ float q8_queries(const AttnQ8Params& p, const Q8Seq& q, int g, int pair0, uint16_t* qs,
+                                            float* wmax) {
+  return p.a.q_type == DTREE_T_BF16 ? q8_queries_of<D, PAIRS, W, true>(p, q, g, pair0, qs, wmax)
+                                    : q8_queries_of<D, PAIRS, W, false>(p, q, g, pair0, qs, wmax);
 }
 
 // (ks, log2 vs, 1 / vs) of a key. A NaN reaches a row that sees the key through
@@ -325,7 +369,7 @@ __device__ __forceinline__ f32x4_t mfma16_f16(u32x4_t a, u32x4_t b, f32x4_t c) {
 // * V's lane (dim % 16, kq) reads its 16 keys of one dim as they lie, i = 2 step,
 //   2 step + 1, and P needs no exchange.
 template <int D, int NC>
-__global__ __launch_bounds__(256, D == 256 ? 1 : NC == 1 ? 3 : 2) void q8_token_kernel(AttnQ8Params p) {
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void q8_token_kernel(AttnQ8Params p) {
   constexpr int NJ = D / 64, NK = 4 * NJ, ND = D / 16;  // K loads (block, 64 dims) and V loads (16 dims) per page
   constexpr int RS = D + 4;                             // a pair's row in `red`
   union Lds {
@@ -388,7 +432,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : NC == 1 ? 3 : 2) void q8_token_
   int cur = page_of(0);
   load_k(cur);
   q8_ancestors(p, q, 0, 16 * NC, pairs, anc);
-  const float inv = q8_queries<D, 16 * NC, kWaves>(p, q, g, 0, pairs, lds.q, wmax);
+  const float inv = q8_queries<D, 16 * NC, kWaves>(p, q, g, 0, lds.q, wmax);
   load_v(cur);  // (not earlier: the queries' registers)
   u32x4_t qf[NC][2 * NJ];
   int pos[NC];  // the columns' positions; -1: no pair
@@ -552,8 +596,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : NC == 1 ? 3 : 2) void q8_token_
   }
 }
 
-// A workgroup: 4 waves of 32 NC pairs of one KV head over one key range. A page is
-// converted to fp16 once for the four waves, on its way from memory to LDS, the
+// A workgroup: W waves of 32 pairs of one KV head over one key range. A page is
+// converted to fp16 once for all of them, on its way from memory to LDS, the
 // next one while the current one is used.
 //
 // A step is 32 keys, half a page: S^T = K Q^T, softmax, O^T += V^T P^T. The matrix
@@ -564,23 +608,22 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : NC == 1 ? 3 : 2) void q8_token_
 // that a later slot needs and a share of the VALU work, in this order
 // (sched_barrier: the compiler keeps it), so that neither unit waits for the other
 // to finish a step.
-template <int D, int NC>
-__global__ __launch_bounds__(256, NC == 1 && D <= 128 ? 2 : 1) void q8_rows_kernel(AttnQ8Params p) {
+template <int D, int W>
+__global__ __launch_bounds__(64 * W, D <= 128 ? 8 / W : 1) void q8_rows_kernel(AttnQ8Params p) {
   constexpr int NB = D / 32, PB = DTREE_PAGE * D;  // bytes of a page's K (or V) as int8
-  constexpr int NP = PB / 16 / 256;                // 16-byte pieces of it per thread
-  constexpr int NF = D / 16, NS = NF * NC;         // fragments of K (or V) in a step; MFMAs of a block
+  constexpr int NT = 64 * W, NP = PB / 16 / NT;    // 16-byte pieces of it per thread
+  constexpr int NF = D / 16;                       // fragments of K (or V) in a step, MFMAs of a block
   constexpr int RF = 4;                            // fragments loaded ahead
-  constexpr int EV = 16 * NC;                      // a lane's logits of a step
-  constexpr int CP = 32 * NC, WP = kWaves * CP;    // pairs of a wave, of the workgroup
+  constexpr int WP = 32 * W;                       // pairs of the workgroup
   constexpr int RS = D + 4;  // a pair's row in `red`
   union Lds {
     unsigned char kv[2][4 * PB];  // fp16 K, then V
     uint16_t q[WP * (D + 8)];
-    float red[kWaves][32 * RS];
+    float red[W][32 * RS];
   };
   __shared__ __attribute__((aligned(16))) Lds lds;
   __shared__ __attribute__((aligned(16))) float scl[2][192];
-  __shared__ float wmax[kWaves];
+  __shared__ float wmax[W];
   __shared__ uint32_t anc[WP][DTREE_MASK_WORDS];
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -593,7 +636,7 @@ __global__ __launch_bounds__(256, NC == 1 && D <= 128 ? 2 : 1) void q8_rows_kern
   const int pairs = q.n * p.G, pair0 = WP * w;
   if (part == 0 && p.a.rows_padded > 0) {  // rows past the sequence's
     const int end = min(pair0 + WP, p.a.rows_padded * p.G);
-    for (int e = max(pairs - pair0, 0) * (D / 4) + tid; e < (end - pair0) * (D / 4); e += 256) {
+    for (int e = max(pairs - pair0, 0) * (D / 4) + tid; e < (end - pair0) * (D / 4); e += NT) {
       const int m = pair0 + e / (D / 4);
       q8_store_zero(p, m / p.G, g * p.G + m % p.G, 4 * (e % (D / 4)));
     }
@@ -604,9 +647,9 @@ __global__ __launch_bounds__(256, NC == 1 && D <= 128 ? 2 : 1) void q8_rows_kern
   const int used = q8_parts(p, rg.tiles), per = (rg.tiles + used - 1) / used;
   const int t0 = part * per, t1 = min(rg.tiles, t0 + per);
   if (part >= used) return;
-  const int wpair = pair0 + CP * wave;
+  const int wpair = pair0 + 32 * wave;
   // the wave's rows (a wave past the last pair works on zero queries, unread)
-  const int wfrom = min(wpair / p.G, q.n - 1), wto = min(q.n - 1, (wpair + CP - 1) / p.G);
+  const int wfrom = min(wpair / p.G, q.n - 1), wto = min(q.n - 1, (wpair + 31) / p.G);
 
   u32x4_t raw[2 * NP];
   float ksl = 0.f, vsl = 0.f;
@@ -622,8 +665,8 @@ __global__ __launch_bounds__(256, NC == 1 && D <= 128 ? 2 : 1) void q8_rows_kern
     const auto rv = buf_rsrc(p.kv.v_pages + blk * PB, page < 0 ? 0 : PB);
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
-      raw[i] = buf_ld(rk, 16 * tid + 4096 * i);
-      raw[NP + i] = buf_ld(rv, 16 * tid + 4096 * i);
+      raw[i] = buf_ld(rk, 16 * tid + 16 * NT * i);
+      raw[NP + i] = buf_ld(rv, 16 * tid + 16 * NT * i);
     }
     const auto sk = buf_rsrc(p.kv.k_scales + blk * DTREE_PAGE, page < 0 ? 0 : 4 * DTREE_PAGE);
     const auto sv = buf_rsrc(p.kv.v_scales + blk * DTREE_PAGE, page < 0 ? 0 : 4 * DTREE_PAGE);
@@ -633,19 +676,14 @@ __global__ __launch_bounds__(256, NC == 1 && D <= 128 ? 2 : 1) void q8_rows_kern
   };
   bool here = load(0);
   q8_ancestors(p, q, pair0, WP, pairs, anc);
-  const float inv = q8_queries<D, WP, kWaves>(p, q, g, pair0, pairs, lds.q, wmax);
-  u32x4_t qf[NC][NF];
-  int pos[NC];  // the lane's positions; -1: no pair
+  const float inv = q8_queries<D, WP, W>(p, q, g, pair0, lds.q, wmax);
+  u32x4_t qf[NF];
+  const int pos = wpair + c < pairs ? q.past + (wpair + c) / p.G : -1;  // -1: the lane has no pair
 #pragma unroll
-  for (int n = 0; n < NC; ++n) {
-    const int l = CP * wave + 32 * n + c;
-    pos[n] = pair0 + l < pairs ? q.past + (pair0 + l) / p.G : -1;
-#pragma unroll
-    for (int i = 0; i < NF; ++i)
-{
-      qf[n][i] = *reinterpret_cast<const u32x4_t*>(lds.q + l * (D + 8) + 32 * (i >> 1) + 16 * h + 8 * (i & 1));
-      if constexpr (NC == 2 || D == 256) asm("" : "+a"(qf[n][i]));
-    }
+  for (int i = 0; i < NF; ++i) {
+    qf[i] = *reinterpret_cast<const u32x4_t*>(lds.q + (32 * wave + c) * (D + 8) + 32 * (i >> 1) + 16 * h + 8 * (i & 1));
+    // (an MFMA reads its B operand from either file: not the one the softmax needs)
+    if constexpr (D == 256) asm("" : "+a"(qf[i]));
   }
   lds_barrier();
   auto stage_scales = [&](int buf) {
@@ -661,7 +699,7 @@ __global__ __launch_bounds__(256, NC == 1 && D <= 128 ? 2 : 1) void q8_rows_kern
   // when they are whole.
   u32x4_t half;
   auto stage_word = [&](int buf, int i, int j) {
-    const int u = tid + 256 * (i % NP);
+    const int u = tid + NT * (i % NP);
     uint32_t lo, hi;
     q8_word_to_h4(raw[i][j], lo, hi);
     half[2 * (j & 1)] = lo;
@@ -670,22 +708,17 @@ __global__ __launch_bounds__(256, NC == 1 && D <= 128 ? 2 : 1) void q8_rows_kern
       *reinterpret_cast<u32x4_t*>(
           &lds.kv[buf][(i / NP) * 2 * PB + (u >> 6) * 2048 + (j >> 1) * 1024 + (u & 63) * 16]) = half;
   };
-  f32x16_t o[NC][NB], sa[NC], sb[NC];  // sa, sb: the logits of even and odd steps
-  u32x4_t ph[NC][2], kf[RF], vf[RF];
+  f32x16_t o[NB], sa, sb;  // sa, sb: the logits of even and odd steps
+  u32x4_t ph[2], kf[RF], vf[RF];
   f32x4_t ks[4], lv[4], iv[4];
-  float m[NC], l[NC], mx[NC];
+  float m = kFloor, l = 0.f, mx;
+  ph[0] = ph[1] = u32x4_t{0, 0, 0, 0};
 #pragma unroll
-  for (int n = 0; n < NC; ++n) {
-    m[n] = kFloor;
-    l[n] = 0.f;
-    ph[n][0] = ph[n][1] = u32x4_t{0, 0, 0, 0};
+  for (int i = 0; i < 16; ++i) sb[i] = -INFINITY;  // the step before the first: no keys
 #pragma unroll
-    for (int i = 0; i < 16; ++i) sb[n][i] = -INFINITY;  // the step before the first: no keys
+  for (int db = 0; db < NB; ++db)
 #pragma unroll
-    for (int db = 0; db < NB; ++db)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) o[n][db][i] = 0.f;
-  }
+    for (int i = 0; i < 16; ++i) o[db][i] = 0.f;
   // Fragment f of a half page: K's dims 16 f ..; V's keys 16 (f / NB) .., dims 32 (f % NB) ..
   auto k_frag = [&](int buf, int b, int f) {
     return *reinterpret_cast<const u32x4_t*>(&lds.kv[buf][b * PB + 1024 * f + 16 * lane]);
@@ -697,79 +730,64 @@ __global__ __launch_bounds__(256, NC == 1 && D <= 128 ? 2 : 1) void q8_rows_kern
 #pragma unroll
     for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const f32x4_t*>(&scl[buf][64 * which + 32 * b + 8 * i + 4 * h]);
   };
-  auto weight = [&](f32x16_t (&x)[NC], int n, int r) {
-    x[n][r] = fast_exp2(x[n][r] - m[n]);
-    l[n] = fmaf(x[n][r], iv[r / 4][r % 4], l[n]);
-    if (r & 1) ph[n][r >> 3][(r >> 1) & 3] = pack_h2(x[n][r - 1], x[n][r]);
+  auto weight = [&](f32x16_t& x, int r) {
+    x[r] = fast_exp2(x[r] - m);
+    l = fmaf(x[r], iv[r / 4][r % 4], l);
+    if (r & 1) ph[r >> 3][(r >> 1) & 3] = pack_h2(x[r - 1], x[r]);
   };
-  // PV of the last step (its V: half vh of buffer vb; its logits `old`), the logits
+  // PV of the last step (its V: half vh of buffer vbuf; its logits `old`), the logits
   // `cur` of this one (half b of buffer buf); STAGE: the raw page to buffer sbuf.
-  auto block1 = [&](f32x16_t (&old)[NC], f32x16_t (&cur)[NC], int vbuf, int vh, int buf, int b, auto stage, int sbuf) {
-    constexpr int ST = NS / 2 > 2 ? NS / 2 - 1 : 1;  // slots of the logits
-    constexpr int SW = 8 * NP / NS;                  // words converted per slot
+  auto block1 = [&](f32x16_t& old, f32x16_t& cur, int vbuf, int vh, int buf, int b, auto stage, int sbuf) {
+    constexpr int ST = NF / 2 > 2 ? NF / 2 - 1 : 1;  // slots of the logits
+    constexpr int SW = 8 * NP / NF;                  // words converted per slot
     consts(ks, buf, 0, b);
     consts(lv, buf, 1, b);
+    mx = kFloor;
 #pragma unroll
-    for (int n = 0; n < NC; ++n) mx[n] = kFloor;
-#pragma unroll
-    for (int k = 0; k < NS; ++k) {
-      const int f = k / NC, n = k % NC;
-      o[n][f % NB] = mfma32_f16(vf[f % RF], ph[n][f / NB], o[n][f % NB]);
-      if (n == NC - 1 && f + RF < NF) vf[f % RF] = v_frag(vbuf, vh, f + RF);
+    for (int k = 0; k < NF; ++k) {
+      o[k % NB] = mfma32_f16(vf[k % RF], ph[k / NB], o[k % NB]);
+      if (k + RF < NF) vf[k % RF] = v_frag(vbuf, vh, k + RF);
       if constexpr (decltype(stage)::value) {
 #pragma unroll
         for (int i = k * SW; i < (k + 1) * SW; ++i) stage_word(sbuf, i / 4, i % 4);
       }
-      if (k < NS / 2) {
+      if (k < NF / 2) {
 #pragma unroll
-        for (int e = k * EV / NS; e < (k + 1) * EV / NS; ++e) weight(old, e % NC, 8 + e / NC);
+        for (int r = 8 + k * 16 / NF; r < 8 + (k + 1) * 16 / NF; ++r) weight(old, r);
       } else {
-        const int j = k - NS / 2;
+        const int j = k - NF / 2;
         if (j < ST) {
 #pragma unroll
-          for (int e = j * EV / ST; e < (j + 1) * EV / ST; ++e) {
-            const int r = e / NC, en = e % NC;
-            cur[en][r] = fmaf(cur[en][r], ks[r / 4][r % 4], lv[r / 4][r % 4]);
-            mx[en] = fmaxf(mx[en], cur[en][r]);
+          for (int r = j * 16 / ST; r < (j + 1) * 16 / ST; ++r) {
+            cur[r] = fmaf(cur[r], ks[r / 4][r % 4], lv[r / 4][r % 4]);
+            mx = fmaxf(mx, cur[r]);
           }
         }
-        if (j == NS / 2 - 1) {
-#pragma unroll
-          for (int en = 0; en < NC; ++en) mx[en] = max_halves(mx[en]);
-        }
+        if (j == NF / 2 - 1) mx = max_halves(mx);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
   };
   // What the rows may not see; the output rescaled where a row's maximum has grown.
-  auto limits = [&](f32x16_t (&cur)[NC], bool masked, bool there, int key0) {
+  auto limits = [&](f32x16_t& cur, bool masked, bool there, int key0) {
     if (masked) {
+      const uint32_t sees = there ? q8_sees(p, q, pos, key0, anc[32 * wave + c]) >> (4 * h) : 0u;
+      mx = kFloor;
 #pragma unroll
-      for (int n = 0; n < NC; ++n) {
-        const uint32_t sees = there ? q8_sees(p, q, pos[n], key0, anc[CP * wave + 32 * n + c]) >> (4 * h) : 0u;
-        mx[n] = kFloor;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          cur[n][r] = sees & (1u << acc_row(r, 0)) ? cur[n][r] : -INFINITY;
-          mx[n] = fmaxf(mx[n], cur[n][r]);
-        }
-        mx[n] = max_halves(mx[n]);
+      for (int r = 0; r < 16; ++r) {
+        cur[r] = sees & (1u << acc_row(r, 0)) ? cur[r] : -INFINITY;
+        mx = fmaxf(mx, cur[r]);
       }
+      mx = max_halves(mx);
     }
-    bool grown = false;
+    if (__any(mx > m + (kTop + kSlack))) {
+      const float mn = mx > m + (kTop + kSlack) ? mx - kTop : m, alpha = fast_exp2(m - mn);
+      m = mn;
+      l *= alpha;
 #pragma unroll
-    for (int n = 0; n < NC; ++n) grown |= mx[n] > m[n] + (kTop + kSlack);
-    if (__any(grown)) {
+      for (int db = 0; db < NB; ++db)
 #pragma unroll
-      for (int n = 0; n < NC; ++n) {
-        const float mn = mx[n] > m[n] + (kTop + kSlack) ? mx[n] - kTop : m[n], alpha = fast_exp2(m[n] - mn);
-        m[n] = mn;
-        l[n] *= alpha;
-#pragma unroll
-        for (int db = 0; db < NB; ++db)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) o[n][db][r] *= alpha;
-      }
+        for (int r = 0; r < 16; ++r) o[db][r] *= alpha;
     }
   };
   auto k_ahead = [&](int buf, int b) {
@@ -778,23 +796,19 @@ __global__ __launch_bounds__(256, NC == 1 && D <= 128 ? 2 : 1) void q8_rows_kern
   };
   // S of the next step (half b of buffer buf) to `next`, the weights of `cur`'s
   // first 16 keys, the first V fragments (half vh of vbuf) of the next block1.
-  auto block2 = [&](f32x16_t (&cur)[NC], f32x16_t (&next)[NC], int buf, int b, int vbuf, int vh) {
+  auto block2 = [&](f32x16_t& cur, f32x16_t& next, int buf, int b, int vbuf, int vh) {
 #pragma unroll
-    for (int n = 0; n < NC; ++n)
+    for (int r = 0; r < 16; ++r) next[r] = 0.f;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) next[n][r] = 0.f;
+    for (int k = 0; k < NF; ++k) {
+      next = mfma32_f16(kf[k % RF], qf[k], next);
+      if (k + RF < NF) kf[k % RF] = k_frag(buf, b, k + RF);
+      else vf[k + RF - NF] = v_frag(vbuf, vh, k + RF - NF);
 #pragma unroll
-    for (int k = 0; k < NS; ++k) {
-      const int f = k / NC, n = k % NC;
-      next[n] = mfma32_f16(kf[f % RF], qf[n][f], next[n]);
-      if (n == NC - 1 && f + RF < NF) kf[f % RF] = k_frag(buf, b, f + RF);
-      if (n == NC - 1 && f + RF >= NF) vf[f + RF - NF] = v_frag(vbuf, vh, f + RF - NF);
-#pragma unroll
-      for (int e = k * (EV / 2) / NS; e < (k + 1) * (EV / 2) / NS; ++e) weight(cur, e % NC, e / NC);
+      for (int r = k * 8 / NF; r < (k + 1) * 8 / NF; ++r) weight(cur, r);
       __builtin_amdgcn_sched_barrier(0);
     }
-#pragma unroll
-    for (int n = 0; n < NC; ++n) asm volatile("" : "+v"(ph[n][0]), "+v"(l[n]));  // taken here, not sunk to their use
+    asm volatile("" : "+v"(ph[0]), "+v"(l));  // taken here, not sunk to their use
   };
   auto hidden = [&](int k0) {  // does a page hold keys that some row may not see
     return p.a.ancestors ? k0 + DTREE_PAGE > q.past
@@ -839,45 +853,39 @@ __global__ __launch_bounds__(256, NC == 1 && D <= 128 ? 2 : 1) void q8_rows_kern
   lds_barrier();  // every wave has read the pages
   // The outputs through LDS, each wave its own part: rows of D values, 8 a lane.
   const bool plain = used == 1 && p.plain;
+  const float lt = l + __shfl_xor(l, 32);
+  float* red = lds.red[wave];
 #pragma unroll
-  for (int n = 0; n < NC; ++n) {
-    const float lt = l[n] + __shfl_xor(l[n], 32);
-    if (wpair + 32 * n >= pairs) break;
-    float* red = lds.red[wave];
+  for (int db = 0; db < NB; ++db)
 #pragma unroll
-    for (int db = 0; db < NB; ++db)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        *reinterpret_cast<f32x4_t*>(red + c * RS + 32 * db + 8 * i + 4 * h) =
-            f32x4_t{o[n][db][4 * i], o[n][db][4 * i + 1], o[n][db][4 * i + 2], o[n][db][4 * i + 3]};
-    if (h == 0) {  // the pair's row, head, m and l or 1 / l behind its values
-      const int pair = wpair + 32 * n + c, row = pair / p.G;
-      *reinterpret_cast<f32x4_t*>(red + c * RS + D) =
-          f32x4_t{m[n], used > 1 ? lt : q8_inverse(lt), __int_as_float(row), __int_as_float(pair - row * p.G)};
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    const int nl = min(32, pairs - wpair - 32 * n) * (D / 8);
+    for (int i = 0; i < 4; ++i)
+      *reinterpret_cast<f32x4_t*>(red + c * RS + 32 * db + 8 * i + 4 * h) =
+          f32x4_t{o[db][4 * i], o[db][4 * i + 1], o[db][4 * i + 2], o[db][4 * i + 3]};
+  if (h == 0) {  // the pair's row, head, m and l or 1 / l behind its values
+    const int row = (wpair + c) / p.G;
+    *reinterpret_cast<f32x4_t*>(red + c * RS + D) = f32x4_t{m, used > 1 ? lt : q8_inverse(lt), __int_as_float(row),
+                                                            __int_as_float(wpair + c - row * p.G)};
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  const int nl = min(32, pairs - wpair) * (D / 8);
 #pragma unroll 2
-    for (int e = lane; e < nl; e += 64) {
-      const int pl = e / (D / 8), d = 8 * (e % (D / 8));
-      const f32x4_t x0 = *reinterpret_cast<const f32x4_t*>(red + pl * RS + d);
-      const f32x4_t x1 = *reinterpret_cast<const f32x4_t*>(red + pl * RS + d + 4);
-      const f32x4_t of = *reinterpret_cast<const f32x4_t*>(red + pl * RS + D);
-      const size_t row = (size_t)q.start + __float_as_int(of[2]);
-      const int head = g * p.G + __float_as_int(of[3]);
-      if (plain) {  // rows of bf16, 16 bytes a lane
-        const f32x4_t y0 = x0 * of[1], y1 = x1 * of[1];
-        *reinterpret_cast<u32x4_t*>(p.a.out + row * p.a.ld_out + head * D + d) =
-            u32x4_t{pack_bf2(y0[0], y0[1]), pack_bf2(y0[2], y0[3]), pack_bf2(y1[0], y1[1]), pack_bf2(y1[2], y1[3])};
-      } else {
-        const float a0[4] = {x0[0], x0[1], x0[2], x0[3]}, a1[4] = {x1[0], x1[1], x1[2], x1[3]};
-        q8_emit(p, used > 1, part, row, head, d, a0, of[0], of[1], of[1]);
-        q8_emit(p, used > 1, part, row, head, d + 4, a1, of[0], of[1], of[1]);
-      }
+  for (int e = lane; e < nl; e += 64) {
+    const int pl = e / (D / 8), d = 8 * (e % (D / 8));
+    const f32x4_t x0 = *reinterpret_cast<const f32x4_t*>(red + pl * RS + d);
+    const f32x4_t x1 = *reinterpret_cast<const f32x4_t*>(red + pl * RS + d + 4);
+    const f32x4_t of = *reinterpret_cast<const f32x4_t*>(red + pl * RS + D);
+    const size_t row = (size_t)q.start + __float_as_int(of[2]);
+    const int head = g * p.G + __float_as_int(of[3]);
+    if (plain) {  // rows of bf16, 16 bytes a lane
+      const f32x4_t y0 = x0 * of[1], y1 = x1 * of[1];
+      *reinterpret_cast<u32x4_t*>(p.a.out + row * p.a.ld_out + head * D + d) =
+          u32x4_t{pack_bf2(y0[0], y0[1]), pack_bf2(y0[2], y0[3]), pack_bf2(y1[0], y1[1]), pack_bf2(y1[2], y1[3])};
+    } else {
+      const float a0[4] = {x0[0], x0[1], x0[2], x0[3]}, a1[4] = {x1[0], x1[1], x1[2], x1[3]};
+      q8_emit(p, used > 1, part, row, head, d, a0, of[0], of[1], of[1]);
+      q8_emit(p, used > 1, part, row, head, d + 4, a1, of[0], of[1], of[1]);
     }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
   }
 }
 
@@ -961,7 +969,8 @@ __global__ __launch_bounds__(256) void q8_join_kernel(AttnQ8Params p) {
 // The launch for a record: which kernel, its grid and key ranges.
 struct Plan {
   bool tokens;
-  int nc;  // column blocks: 16 pairs (tokens) or 32 (rows) each
+  int nc;     // tokens: column blocks of 16 pairs
+  int waves;  // rows: waves of 32 pairs
   int blocks, parts, per;
 };
 
@@ -978,8 +987,9 @@ Plan make_plan(const DtreeKvQ8& kv, const DtreeAttnQ8Args& a) {
   Plan pl{};
   const int64_t pairs = (int64_t)std::max(kv.max_rows, a.rows_padded) * G;
   pl.tokens = pairs <= (D == 256 ? 16 : 32);  // (registers: 32 columns of 256 dims do not fit)
-  pl.nc = pl.tokens ? (pairs <= 16 ? 1 : 2) : (D == 256 || pairs <= 32 * kWaves ? 1 : 2);
-  const int wp = 32 * kWaves * pl.nc;  // pairs of a workgroup of rows
+  pl.nc = pairs <= 16 ? 1 : 2;
+  pl.waves = D == 128 && pairs > 128 ? 8 : 4;
+  const int wp = 32 * pl.waves;  // pairs of a workgroup of rows
   pl.blocks = pl.tokens ? 1 : (int)((pairs + wp - 1) / wp);
   // pages that one workgroup's rows can see
   const int64_t end = std::min((int64_t)kv.max_past_length + kv.max_rows, (int64_t)kv.ld_page_table * DTREE_PAGE);
@@ -1010,12 +1020,13 @@ int launch_join(const AttnQ8Params& p, hipStream_t stream) {
 
 template <int D>
 int launch(const AttnQ8Params& p, const Plan& pl, unsigned grid, hipStream_t stream) {
-  if (pl.nc == 1) {
-    if (pl.tokens) q8_token_kernel<D, 1><<<grid, 256, 0, stream>>>(p);
-    else q8_rows_kernel<D, 1><<<grid, 256, 0, stream>>>(p);
-  } else if constexpr (D != 256) {
-    if (pl.tokens) q8_token_kernel<D, 2><<<grid, 256, 0, stream>>>(p);
-    else q8_rows_kernel<D, 2><<<grid, 256, 0, stream>>>(p);
+  if (pl.tokens) {
+    if (pl.nc == 1) q8_token_kernel<D, 1><<<grid, 256, 0, stream>>>(p);
+    else if constexpr (D != 256) q8_token_kernel<D, 2><<<grid, 256, 0, stream>>>(p);
+  } else if (pl.waves == 4) {
+    q8_rows_kernel<D, 4><<<grid, 256, 0, stream>>>(p);
+  } else if constexpr (D == 128) {
+    q8_rows_kernel<D, 8><<<grid, 512, 0, stream>>>(p);
   }
   DTREE_LAUNCH_CHECK("attention_q8 launch");
   if (p.parts == 1) return DTREE_OK;
@@ -1082,7 +1093,7 @@ extern "C" int dtree_attention_q8(const DtreeKvQ8* kv, const DtreeAttnQ8Args* a,
   p.a = *a;
   p.G = a->num_heads / kv->num_kv_heads;
   p.blocks = pl.blocks;
-  p.pairs_wg = 32 * kWaves * pl.nc;
+  p.pairs_wg = 32 * pl.waves;
   p.parts = pl.parts;
   p.per = pl.per;
   p.sink_pages = (a->sink + DTREE_PAGE - 1) / DTREE_PAGE;
