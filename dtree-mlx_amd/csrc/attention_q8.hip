@@ -33,11 +33,12 @@ constexpr int kWaves = 4;
 struct AttnQ8Params {
   DtreeKvQ8 kv;
   DtreeAttnQ8Args a;
+  float* part;    // [parts][total_rows][Hq][D], of every key range
+  float* part_ml;  // and (m, l) of the same
   int G, blocks, pairs_wg;  // heads per group; row blocks per sequence, pairs of one
-  int parts, per;       // key ranges the grid holds; pages of a range
+  int parts, per;           // key ranges the grid holds; pages of a range
   int sink_pages;
   float scale_log2;
-  float* part; float* part_ml;  // [parts][total_rows][Hq] x D, x (m, l)
   int tiled, h16;
   int plain;  // out: rows of bf16 alone, 16-byte aligned, no gate
 };
@@ -96,25 +97,6 @@ __device__ __forceinline__ void q8_exponent(float amax, float& f, float& inv) {
   const int ef = amax > 0.f ? min(max(267 - e, 1), 253) : 127;
   f = __uint_as_float((uint32_t)ef << 23);
   inv = __uint_as_float((uint32_t)(254 - ef) << 23);
-}
-
-// Queries. A pair's D dims are D / 8 neighbouring lanes, each with two pieces of 4
-// dims: lane j of the first R / 8 the halves 4 j .. and R / 2 + 4 j .. of a rotation
-// of R dims, the others 8 dims that do not rotate. A wave's loads are then whole
-// runs of the rows.
-struct Q8Pieces {
-  int at[2];   // first dim of each
-  bool turns;  // the two rotate
-};
-template <int D>
-__device__ __forceinline__ Q8Pieces q8_pieces(int rope_dims, int j) {
-  const int hp = rope_dims / 8;  // pieces of a rotation's half
-  const bool turns = j < hp;
-  return Q8Pieces{{4 * (turns ? j : 2 * j), 4 * (turns ? j + hp : 2 * j + 1)}, turns};
-}
-__device__ __forceinline__ f32x4_t q8_bf4(u32x2_t w) {
-  return f32x4_t{__uint_as_float(w[0] << 16), __uint_as_float(w[0] & 0xffff0000u), __uint_as_float(w[1] << 16),
-                 __uint_as_float(w[1] & 0xffff0000u)};
 }
 
 // Max over the TPR = D / 8 lanes of a pair.
@@ -327,10 +309,10 @@ __device__ __forceinline__ void q8_store(const AttnQ8Params& p, size_t row, int 
   store_act4(p.a.out, p.a.out_lo, oi, y, p.h16);
 }
 __device__ __forceinline__ void q8_store_zero(const AttnQ8Params& p, size_t row, int head, int d) {
-  float y[4] = {0.f, 0.f, 0.f, 0.f};
   const int col = head * p.kv.head_dim + d;
   const size_t oi = p.tiled ? tiled_index((int)row, col, p.a.ld_out) : row * p.a.ld_out + col;
-  store_act4(p.a.out, p.a.out_lo, oi, y, p.h16);
+  *reinterpret_cast<u32x2_t*>(p.a.out + oi) = u32x2_t{0, 0};  // (0 in bf16 and in fp16)
+  if (p.a.out_lo) *reinterpret_cast<u32x2_t*>(p.a.out_lo + oi) = u32x2_t{0, 0};
 }
 
 // 1 / l, 0 where the row has seen no key.
@@ -430,9 +412,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void q8_token_kernel(AttnQ8P
   };
   const int steps = max(0, (t1 - t0 - wave + kWaves - 1) / kWaves);  // the wave's pages
   int cur = page_of(0);
-  load_k(cur);
+  if constexpr (NC == 1) load_k(cur);
   q8_ancestors(p, q, 0, 16 * NC, pairs, anc);
   const float inv = q8_queries<D, 16 * NC, kWaves>(p, q, g, 0, lds.q, wmax);
+  if constexpr (NC == 2) load_k(cur);
   load_v(cur);  // (not earlier: the queries' registers)
   u32x4_t qf[NC][2 * NJ];
   int pos[NC];  // the columns' positions; -1: no pair

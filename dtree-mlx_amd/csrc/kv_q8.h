@@ -40,8 +40,24 @@ __device__ __forceinline__ int q8_page(const DtreeKvQ8& kv, int s, int i) {
   return page >= 0 && page < kv.num_pages ? page : -1;
 }
 
-// Pages that max_rows positions from anywhere in a page can touch.
-__host__ __forceinline__ int q8_span_pages(const DtreeKvQ8& kv) { return (kv.max_rows + DTREE_PAGE - 2) / DTREE_PAGE + 1; }
+// A projection row's head as D / 8 neighbouring lanes with two pieces of 4 dims
+// each: lane j of the first R / 8 has the halves 4 j .. and R / 2 + 4 j .. of a
+// rotation of R dims, the others 8 dims that do not rotate. A wave's loads are then
+// whole runs of the rows.
+struct Q8Pieces {
+  int at[2];   // first dim of each
+  bool turns;  // the two rotate
+};
+template <int D>
+__device__ __forceinline__ Q8Pieces q8_pieces(int rope_dims, int j) {
+  const int hp = rope_dims / 8;  // pieces of a rotation's half
+  const bool turns = j < hp;
+  return Q8Pieces{{4 * (turns ? j : 2 * j), 4 * (turns ? j + hp : 2 * j + 1)}, turns};
+}
+__device__ __forceinline__ f32x4_t q8_bf4(u32x2_t w) {
+  return f32x4_t{__uint_as_float(w[0] << 16), __uint_as_float(w[0] & 0xffff0000u), __uint_as_float(w[1] << 16),
+                 __uint_as_float(w[1] & 0xffff0000u)};
+}
 
 // Host check of the record, common to the entries (`what`: the entry's name).
 int q8_check(const DtreeKvQ8* kv, const char* what);

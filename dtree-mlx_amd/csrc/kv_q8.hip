@@ -7,10 +7,10 @@
 // of its value, so q is the nearest integer but for borders met by less than
 // that, and two programs that follow the definition store the same bytes.
 //
-// All three are bound by the bytes they move (a decode step's by the launch).
-// A workgroup owns one page of one kv head. K rows are written by D / 16 threads
-// each, 16 dims (one 16-byte store) a thread; V's 16 bytes belong to 16 rows of
-// one dim and go through LDS.
+// All three are bound by the bytes they move (a decode step's by the launch). A
+// workgroup owns half a page (32 positions, whole 16-byte pieces of K and of V) of
+// one kv head. The rows' side is read and written in runs of their dims, the
+// pages' side in runs of their pieces, and LDS, rows of bytes, lies between.
 #include <cmath>
 
 #include "kv_q8.h"
@@ -18,165 +18,222 @@
 namespace dtree {
 namespace {
 
+constexpr int kHalf = DTREE_PAGE / 2;
+
+// Half pages that max_rows positions from anywhere in one can touch.
+int span_halves(const DtreeKvQ8& kv) { return (kv.max_rows + kHalf - 2) / kHalf + 1; }
+
+// This workgroup's half page: its page, the sequence's row in its slot 0, its live
+// slots lo .. hi - 1 (none: lo >= hi).
+struct Half {
+  int page, b, first, lo, hi;
+  size_t row0;  // buffer row of the sequence's row 0
+};
+__device__ __forceinline__ Half q8_half(const DtreeKvQ8& kv, int block, int span) {
+  const int s = block / span;
+  const Q8Seq q = q8_seq(kv, s);
+  const int i = q.past / kHalf + block % span;
+  Half w{-1, i & 1, i * kHalf - q.past, 0, 0, (size_t)q.start};
+  w.lo = max(0, -w.first);
+  w.hi = min(kHalf, q.n - w.first);
+  if (w.lo < w.hi) w.page = q8_page(kv, s, i >> 1);
+  return w;
+}
+
+// Four rows' words of four bytes -> four columns' words.
+__device__ __forceinline__ void transpose4(uint32_t (&w)[4]) {
+  const uint32_t t0 = __builtin_amdgcn_perm(w[1], w[0], 0x05010400u), t1 = __builtin_amdgcn_perm(w[1], w[0], 0x07030602u);
+  const uint32_t u0 = __builtin_amdgcn_perm(w[3], w[2], 0x05010400u), u1 = __builtin_amdgcn_perm(w[3], w[2], 0x07030602u);
+  w[0] = __builtin_amdgcn_perm(u0, t0, 0x05040100u);
+  w[1] = __builtin_amdgcn_perm(u0, t0, 0x07060302u);
+  w[2] = __builtin_amdgcn_perm(u1, t1, 0x05040100u);
+  w[3] = __builtin_amdgcn_perm(u1, t1, 0x07060302u);
+}
+
 struct Q8AppendParams {
   DtreeKvQ8 kv;
   const void* k; const void* v;
-  int ld_k, ld_v, span;
-  const uint16_t* k_norm; double eps;
-  const float* cos; const float* sin; int half;  // rotated pairs
+  int ld_k, ld_v, span, rope_dims;
+  const uint16_t* k_norm;
+  const float* cos; const float* sin;
+  double eps;
 };
 
-// 16 consecutive elements of a row.
-template <bool BF16>
-__device__ __forceinline__ void load16(const void* base, size_t at, float (&x)[16]) {
-  if constexpr (BF16) {
-    const uint16_t* p = static_cast<const uint16_t*>(base) + at;
+template <int CTRL>
+__device__ __forceinline__ double dpp64(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)dpp_i<CTRL>((int)(uint32_t)b), hi = (uint32_t)dpp_i<CTRL>((int)(uint32_t)(b >> 32));
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double swz64_xor16(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)swz_xor16_i((int)(uint32_t)b), hi = (uint32_t)swz_xor16_i((int)(uint32_t)(b >> 32));
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+// Sum or maximum over TPR neighbouring lanes, in each of them.
+template <int TPR, class F>
+__device__ __forceinline__ double over_row(double v, F f) {
+  v = f(v, dpp64<0xB1>(v));
+  v = f(v, dpp64<0x4E>(v));
+  v = f(v, dpp64<0x141>(v));
+  if constexpr (TPR >= 16) v = f(v, dpp64<0x140>(v));
+  if constexpr (TPR >= 32) v = f(v, swz64_xor16(v));
+  return v;
+}
+// 1 / sqrt(a) and 1 / a, two Newton steps (2^-52) on the hardware's estimates.
+__device__ __forceinline__ double rsqrt64(double a) {
+  double r = __builtin_amdgcn_rsq(a);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const u32x4_t w = ld_u32x4(p + 8 * i);
+  for (int i = 0; i < 2; ++i) r = fma(r * fma(-a * r, r, 1.0), 0.5, r);
+  return r;
+}
+__device__ __forceinline__ double rcp64(double a) {
+  double r = __builtin_amdgcn_rcp(a);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        x[8 * i + 2 * j] = __uint_as_float(w[j] << 16);
-        x[8 * i + 2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
-      }
-    }
-  } else {
-    const float* p = static_cast<const float*>(base) + at;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const f32x4_t w = *reinterpret_cast<const f32x4_t*>(p + 4 * i);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) x[4 * i + j] = w[j];
-    }
-  }
+  for (int i = 0; i < 2; ++i) r = fma(fma(-a, r, 1.0), r, r);
+  return r;
 }
 
-// Quantises a row held by TPR neighbouring lanes, 16 elements each: the bytes,
-// and the row's scale in every lane. Not finite anywhere: scale NaN, bytes 0.
+// A row's bytes (this lane's two pieces) and scale. Not finite anywhere (or beyond
+// what an fp32 scale can stand for): scale NaN, bytes 0.
 template <int TPR>
-__device__ __forceinline__ u32x4_t quantise16(const double (&x)[16], float& scale) {
+__device__ __forceinline__ void quantise(const double (&x)[8], uint32_t (&w)[2], float& scale) {
   constexpr double kMost = 4.3e40;  // fp32's largest times 127, less a little
   double amax = 0.;
   bool bad = false;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
+  for (int i = 0; i < 8; ++i) {
     const double a = fabs(x[i]);
     bad |= !(a <= kMost);
     amax = fmax(amax, a);
   }
-  if (bad) amax = INFINITY;
+  amax = over_row<TPR>(bad ? (double)INFINITY : amax, [](double a, double b) { return fmax(a, b); });
+  const bool fine = amax <= kMost;
+  scale = fine ? (float)(amax * (1.0 / 127.0)) : NAN;
+  const double inv = scale > 0.f ? rcp64((double)scale) : 0.;
 #pragma unroll
-  for (int o = 1; o < TPR; o <<= 1) amax = fmax(amax, __shfl_xor(amax, o));
-  if (amax > kMost) {
-    scale = NAN;
-    return u32x4_t{0, 0, 0, 0};
-  }
-  scale = (float)(amax / 127.0);
-  const double inv = scale > 0.f ? 1.0 / (double)scale : 0.;
-  u32x4_t w;
+  for (int i = 0; i < 2; ++i) {
+    w[i] = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    uint32_t b = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      // (a subnormal scale may have been rounded by more than 1 / 254)
-      const double q = fmin(fmax(rint(x[4 * i + j] * inv), -127.), 127.);
-      b |= (uint32_t)((int)q & 0xff) << (8 * j);
+    for (int e = 0; e < 4; ++e) {
+      // (clamped: a subnormal scale may have been rounded by more than 1 / 254)
+      const int q = fine ? (int)fmin(fmax(rint(x[4 * i + e] * inv), -127.), 127.) : 0;
+      w[i] |= (uint32_t)(q & 0xff) << (8 * e);
     }
-    w[i] = b;
   }
-  return w;
 }
 
-// Waves 0 and 1 take K rows, waves 2 and 3 V rows, at once.
 template <int D, bool BF16>
 __global__ __launch_bounds__(256) void q8_append_kernel(Q8AppendParams p) {
-  constexpr int TPR = D / 16, RPP = 128 / TPR;  // threads a row; rows a pass
-  __shared__ uint32_t vt[D][17];                // V bytes [dim][slot], a word of padding
-  const int g = blockIdx.x % p.kv.num_kv_heads, b = blockIdx.x / p.kv.num_kv_heads;
-  const int s = b / p.span;
-  const Q8Seq q = q8_seq(p.kv, s);
-  if (q.n == 0) return;
-  const int pg = q.past / DTREE_PAGE + b % p.span;
-  const int first = pg * DTREE_PAGE - q.past;  // the sequence's row in slot 0
-  const int lo = max(0, -first), hi = min(DTREE_PAGE, q.n - first);  // live slots
-  if (lo >= hi) return;
-  const int page = q8_page(p.kv, s, pg);
-  if (page < 0) return;
-  const size_t blk = (size_t)page * p.kv.num_kv_heads + g;
-  const int tid = threadIdx.x, t = tid & 127, j = t % TPR;
-  for (int slot = lo + t / TPR; slot < hi; slot += RPP) {
-    const size_t row = q.start + first + slot;
-    double x[16];
-    float y[16], scale;
-    if (tid < 128) {
-      load16<BF16>(p.k, row * p.ld_k + g * D + 16 * j, y);
+  constexpr int TPR = D / 8, RPP = 256 / TPR;  // lanes a row; rows a pass
+  constexpr int LS = D / 4 + 4;                // words of a row in LDS, 16-byte pieces on their own banks
+  __shared__ __attribute__((aligned(16))) uint32_t lds[2][kHalf][LS];  // K rows, V rows
+  const int g = blockIdx.x % p.kv.num_kv_heads;
+  const Half w = q8_half(p.kv, blockIdx.x / p.kv.num_kv_heads, p.span);
+  if (w.page < 0) return;
+  const size_t blk = (size_t)w.page * p.kv.num_kv_heads + g;
+  const int tid = threadIdx.x, j = tid % TPR, n = w.hi - w.lo, half = p.rope_dims / 2;
+  const Q8Pieces pc = q8_pieces<D>(p.rope_dims, j);
+  const int at0 = g * D + pc.at[0], at1 = g * D + pc.at[1];
+  // K rows, then V rows
+  for (int i = tid / TPR; i < 2 * n; i += RPP) {
+    const bool is_k = i < n;
+    const int slot = w.lo + (is_k ? i : i - n);
+    const size_t row = w.row0 + w.first + slot;
+    const size_t base = row * (is_k ? p.ld_k : p.ld_v);
+    f32x4_t x0, x1;
+    if constexpr (BF16) {
+      const uint16_t* s = static_cast<const uint16_t*>(is_k ? p.k : p.v) + base;
+      x0 = q8_bf4(*reinterpret_cast<const u32x2_t*>(s + at0));
+      x1 = q8_bf4(*reinterpret_cast<const u32x2_t*>(s + at1));
+    } else {
+      const float* s = static_cast<const float*>(is_k ? p.k : p.v) + base;
+      x0 = *reinterpret_cast<const f32x4_t*>(s + at0);
+      x1 = *reinterpret_cast<const f32x4_t*>(s + at1);
+    }
+    double x[8];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] = y[i];
-      double rs = 1.;
+    for (int e = 0; e < 4; ++e) {
+      x[e] = x0[e];
+      x[4 + e] = x1[e];
+    }
+    if (is_k) {
+      f32x4_t cs, sn;
+      if (pc.turns) {  // (tables and weights at any address of their type)
+        __builtin_memcpy(&cs, p.cos + row * half + 4 * j, 16);
+        __builtin_memcpy(&sn, p.sin + row * half + 4 * j, 16);
+      }
       if (p.k_norm) {
+        u32x2_t a, b;
+        __builtin_memcpy(&a, p.k_norm + pc.at[0], 8);
+        __builtin_memcpy(&b, p.k_norm + pc.at[1], 8);
+        const f32x4_t w0 = q8_bf4(a), w1 = q8_bf4(b);
         double ss = 0.;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) ss = fma(x[i], x[i], ss);
+        for (int e = 0; e < 8; ++e) ss = fma(x[e], x[e], ss);
+        ss = over_row<TPR>(ss, [](double a, double b) { return a + b; });
+        const double rs = rsqrt64(ss * (1.0 / D) + p.eps);
 #pragma unroll
-        for (int o = 1; o < TPR; o <<= 1) ss += __shfl_xor(ss, o);
-        rs = 1. / sqrt(ss * (1.0 / D) + p.eps);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] *= rs * (double)bf2f(p.k_norm[16 * j + i]);
-      }
-      const int hc = p.half / 16;  // chunks of 16 dims in a half of the rotated ones
-      if (j < 2 * hc) {            // the rotation's other half, loaded once more
-        const bool low = j < hc;
-        const int jo = low ? j + hc : j - hc;
-        load16<BF16>(p.k, row * p.ld_k + g * D + 16 * jo, y);
-        const size_t at = row * p.half + 16 * (low ? j : jo);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const double o = p.k_norm ? (double)y[i] * (rs * (double)bf2f(p.k_norm[16 * jo + i])) : (double)y[i];
-          const double cs = p.cos[at + i], sn = p.sin[at + i];
-          x[i] = low ? x[i] * cs - o * sn : o * sn + x[i] * cs;
+        for (int e = 0; e < 4; ++e) {
+          x[e] *= rs * w0[e];
+          x[4 + e] *= rs * w1[e];
         }
       }
-      const u32x4_t w = quantise16<TPR>(x, scale);
-      *reinterpret_cast<u32x4_t*>(p.kv.k_pages + blk * (DTREE_PAGE * D) + q8_k_off(slot, 16 * j, D)) = w;
-      if (j == 0) p.kv.k_scales[blk * DTREE_PAGE + slot] = scale;
-    } else {
-      load16<BF16>(p.v, row * p.ld_v + g * D + 16 * j, y);
+      if (pc.turns) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] = y[i];
-      const u32x4_t w = quantise16<TPR>(x, scale);
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        reinterpret_cast<uint8_t*>(&vt[16 * j + i][0])[slot] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
-      if (j == 0) p.kv.v_scales[blk * DTREE_PAGE + slot] = scale;
+        for (int e = 0; e < 4; ++e) {
+          const double a = x[e], b = x[4 + e];
+          x[e] = a * cs[e] - b * sn[e];
+          x[4 + e] = a * sn[e] + b * cs[e];
+        }
+      }
     }
+    uint32_t q[2];
+    float scale;
+    quantise<TPR>(x, q, scale);
+    uint32_t* o = lds[is_k ? 0 : 1][slot];
+    o[pc.at[0] / 4] = q[0];
+    o[pc.at[1] / 4] = q[1];
+    if (j == 0) (is_k ? p.kv.k_scales : p.kv.v_scales)[blk * DTREE_PAGE + w.b * kHalf + slot] = scale;
   }
   __syncthreads();
-  // V: 16-byte pieces (32-slot half, 32 dims, 4-slot parity, dim); what other
-  // rows own of a piece stays.
-  int8_t* vp = p.kv.v_pages + blk * (DTREE_PAGE * D);
+  int8_t* kp = p.kv.k_pages + blk * (DTREE_PAGE * D) + w.b * kHalf * D;
+  int8_t* vp = p.kv.v_pages + blk * (DTREE_PAGE * D) + w.b * kHalf * D;
+  // K: piece u = (dims 16 (u / 32) .., slot u % 32)
 #pragma unroll
-  for (int u = tid; u < 4 * D; u += 256) {
-    const int dl = u & 31, h = (u >> 5) & 1, db = (u >> 6) % (D / 32), b2 = (u >> 6) / (D / 32);
-    const int s0 = 32 * b2 + 4 * h, d = 32 * db + dl;  // the piece's slots: s0 + 8 i + 0 .. 3
-    if (s0 + 27 < lo || s0 >= hi) continue;
-    u32x4_t w;
+  for (int u = tid; u < 2 * D; u += 256) {
+    const int slot = u & 31;
+    if (slot >= w.lo && slot < w.hi)
+      *reinterpret_cast<u32x4_t*>(kp + 16 * u) = ld_u32x4(&lds[0][slot][4 * (u >> 5)]);
+  }
+  // V: four dims of a 4-slot parity; what other rows own of a piece stays.
+  for (int u = tid; u < D / 2; u += 256) {
+    const int dq = u % (D / 4), h = u / (D / 4), d = 4 * dq;
+    uint32_t v[4][4];  // [slots 8 i + 4 h ..][dims d ..]
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = vt[d][s0 / 4 + 2 * i];
-    int8_t* o = vp + (u << 4);
-    if (s0 >= lo && s0 + 27 < hi) {
-      *reinterpret_cast<u32x4_t*>(o) = w;
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[i][e] = lds[1][8 * i + 4 * h + e][dq];
+      transpose4(v[i]);
+    }
+    int8_t* o = vp + (((d >> 5) * 64 + 32 * h + (d & 31)) << 4);
+    if (w.lo <= 4 * h && w.hi >= 28 + 4 * h) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) *reinterpret_cast<u32x4_t*>(o + 16 * e) = u32x4_t{v[0][e], v[1][e], v[2][e], v[3][e]};
       continue;
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int sl = s0 + 8 * i;
-      if (sl >= lo && sl + 3 < hi) {
-        reinterpret_cast<uint32_t*>(o)[i] = w[i];
-      } else {
+      const int sl = 8 * i + 4 * h;
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (sl + e >= lo && sl + e < hi) o[4 * i + e] = (int8_t)(w[i] >> (8 * e));
+      for (int e = 0; e < 4; ++e) {
+        if (sl >= w.lo && sl + 3 < w.hi) {
+          *reinterpret_cast<uint32_t*>(o + 16 * e + 4 * i) = v[i][e];
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (sl + k >= w.lo && sl + k < w.hi) o[16 * e + 4 * i + k] = (int8_t)(v[i][e] >> (8 * k));
+        }
       }
     }
   }
@@ -188,70 +245,65 @@ struct Q8ReadParams {
   int ld_k, ld_v, span;
 };
 
-template <bool BF16>
-__device__ __forceinline__ void store16(void* base, size_t at, u32x4_t w, float scale) {
-  float y[16];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) y[i] = (float)((int)(w[i >> 2] << (24 - 8 * (i & 3))) >> 24) * scale;
-  if constexpr (BF16) {
-    uint16_t* o = static_cast<uint16_t*>(base) + at;
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-      *reinterpret_cast<u32x4_t*>(o + 8 * i) = u32x4_t{pack_bf2(y[8 * i], y[8 * i + 1]), pack_bf2(y[8 * i + 2], y[8 * i + 3]),
-                                                       pack_bf2(y[8 * i + 4], y[8 * i + 5]), pack_bf2(y[8 * i + 6], y[8 * i + 7])};
-  } else {
-    float* o = static_cast<float*>(base) + at;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      *reinterpret_cast<f32x4_t*>(o + 4 * i) = f32x4_t{y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]};
-  }
-}
-
 template <int D, bool BF16>
 __global__ __launch_bounds__(256) void q8_read_kernel(Q8ReadParams p) {
-  constexpr int TPR = D / 16;
-  __shared__ uint32_t vt[D][17];
-  const int g = blockIdx.x % p.kv.num_kv_heads, b = blockIdx.x / p.kv.num_kv_heads;
-  const int s = b / p.span;
-  const Q8Seq q = q8_seq(p.kv, s);
-  if (q.n == 0) return;
-  const int pg = q.past / DTREE_PAGE + b % p.span;
-  const int first = pg * DTREE_PAGE - q.past;
-  const int lo = max(0, -first), hi = min(DTREE_PAGE, q.n - first);
-  if (lo >= hi) return;
-  const int page = q8_page(p.kv, s, pg), tid = threadIdx.x;
-  const size_t blk = (size_t)max(page, 0) * p.kv.num_kv_heads + g;
-  const int8_t* kb = p.kv.k_pages + blk * (DTREE_PAGE * D);
-  const int8_t* vb = p.kv.v_pages + blk * (DTREE_PAGE * D);
+  constexpr int EPT = BF16 ? 8 : 4, TPR = D / EPT, RPP = 256 / TPR;  // 16 bytes out a lane
+  constexpr int LS = D / 4 + 4;
+  __shared__ __attribute__((aligned(16))) uint32_t lds[2][kHalf][LS];
+  __shared__ float sc[2][kHalf];
+  const int g = blockIdx.x % p.kv.num_kv_heads;
+  const Half w = q8_half(p.kv, blockIdx.x / p.kv.num_kv_heads, p.span);
+  if (w.lo >= w.hi) return;
+  const bool here = w.page >= 0;
+  const size_t blk = (size_t)max(w.page, 0) * p.kv.num_kv_heads + g;
+  const int tid = threadIdx.x;
+  const int8_t* kb = p.kv.k_pages + blk * (DTREE_PAGE * D) + w.b * kHalf * D;
+  const int8_t* vb = p.kv.v_pages + blk * (DTREE_PAGE * D) + w.b * kHalf * D;
   const u32x4_t zero = {0, 0, 0, 0};
+  if (tid < 2 * kHalf) {
+    const float* s = (tid < kHalf ? p.kv.k_scales : p.kv.v_scales) + blk * DTREE_PAGE + w.b * kHalf;
+    sc[tid / kHalf][tid % kHalf] = here ? s[tid % kHalf] : 0.f;
+  }
+  if (p.k) {
+#pragma unroll
+    for (int u = tid; u < 2 * D; u += 256)
+      *reinterpret_cast<u32x4_t*>(&lds[0][u & 31][4 * (u >> 5)]) = here ? ld_u32x4(kb + 16 * u) : zero;
+  }
   if (p.v) {
+    for (int u = tid; u < D / 2; u += 256) {
+      const int dq = u % (D / 4), h = u / (D / 4), d = 4 * dq;
+      const int8_t* o = vb + (((d >> 5) * 64 + 32 * h + (d & 31)) << 4);
+      u32x4_t v[4];  // [dim d + e][slots 8 i + 4 h ..]
 #pragma unroll
-    for (int u = tid; u < 4 * D; u += 256) {
-      const int dl = u & 31, h = (u >> 5) & 1, db = (u >> 6) % (D / 32), b2 = (u >> 6) / (D / 32);
-      const u32x4_t w = page >= 0 ? ld_u32x4(vb + (u << 4)) : zero;
+      for (int e = 0; e < 4; ++e) v[e] = here ? ld_u32x4(o + 16 * e) : zero;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) vt[32 * db + dl][8 * b2 + h + 2 * i] = w[i];
+      for (int i = 0; i < 4; ++i) {
+        uint32_t t[4] = {v[0][i], v[1][i], v[2][i], v[3][i]};
+        transpose4(t);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) lds[1][8 * i + 4 * h + e][dq] = t[e];
+      }
     }
   }
   __syncthreads();
-  for (int slot = lo + tid / TPR; slot < hi; slot += 256 / TPR) {
-    const int j = tid % TPR;
-    const size_t row = q.start + first + slot;
-    if (p.k)
-      store16<BF16>(p.k, row * p.ld_k + g * D + 16 * j, page >= 0 ? ld_u32x4(kb + q8_k_off(slot, 16 * j, D)) : zero,
-                    page >= 0 ? p.kv.k_scales[blk * DTREE_PAGE + slot] : 0.f);
-    if (p.v) {
-      u32x4_t w;
+  const int n = w.hi - w.lo, j = tid % TPR;
+  const int from = p.k ? 0 : n, to = p.v ? 2 * n : n;  // K rows, then V rows
+  for (int i = from + tid / TPR; i < to; i += RPP) {
+    const bool is_k = i < n;
+    const int slot = w.lo + (is_k ? i : i - n), which = is_k ? 0 : 1;
+    const size_t at = (w.row0 + w.first + slot) * (is_k ? p.ld_k : p.ld_v) + g * D + EPT * j;
+    const float scale = sc[which][slot];
+    float y[EPT];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t x = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          x |= (uint32_t) reinterpret_cast<const uint8_t*>(&vt[16 * j + 4 * i + e][0])[slot] << (8 * e);
-        w[i] = x;
-      }
-      store16<BF16>(p.v, row * p.ld_v + g * D + 16 * j, w, page >= 0 ? p.kv.v_scales[blk * DTREE_PAGE + slot] : 0.f);
+    for (int e = 0; e < EPT; ++e) {
+      const uint32_t x = lds[which][slot][EPT / 4 * j + e / 4];
+      y[e] = (float)((int)(x << (24 - 8 * (e & 3))) >> 24) * scale;
     }
+    void* out = is_k ? p.k : p.v;
+    if constexpr (BF16)
+      *reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(out) + at) =
+          u32x4_t{pack_bf2(y[0], y[1]), pack_bf2(y[2], y[3]), pack_bf2(y[4], y[5]), pack_bf2(y[6], y[7])};
+    else *reinterpret_cast<f32x4_t*>(static_cast<float*>(out) + at) = f32x4_t{y[0], y[1], y[2], y[3]};
   }
 }
 
@@ -357,7 +409,7 @@ static int row_buffer_check(const DtreeKvQ8* kv, const void* p, int ld, int type
 }
 
 static int grid_of(const DtreeKvQ8* kv, const std::string& what, unsigned* grid) {
-  const int64_t n = (int64_t)kv->num_seqs * q8_span_pages(*kv) * kv->num_kv_heads;
+  const int64_t n = (int64_t)kv->num_seqs * span_halves(*kv) * kv->num_kv_heads;
   DTREE_REQUIRE(n < (int64_t)1 << 31, what + ": num_seqs * max_rows too large for one launch");
   *grid = (unsigned)n;
   return DTREE_OK;
@@ -377,8 +429,7 @@ extern "C" int dtree_kv_q8_append(const DtreeKvQ8* kv, const void* k, const void
   DTREE_REQUIRE(eps >= 0.f, "kv_q8_append: eps");
   unsigned grid;
   if (int rc = grid_of(kv, "kv_q8_append", &grid)) return rc;
-  const Q8AppendParams p{*kv, k, v, ld_k, ld_v, q8_span_pages(*kv), k_norm, (double)eps, rope_cos, rope_sin,
-                         rope_dims / 2};
+  const Q8AppendParams p{*kv, k, v, ld_k, ld_v, span_halves(*kv), rope_dims, k_norm, rope_cos, rope_sin, (double)eps};
   const bool bf = type == DTREE_T_BF16;
   if (kv->head_dim == 64) {
     if (bf) q8_append_kernel<64, true><<<grid, 256, 0, stream>>>(p);
@@ -405,7 +456,7 @@ extern "C" int dtree_kv_q8_read(const DtreeKvQ8* kv, void* k, void* v, int32_t t
     if (int rc = row_buffer_check(kv, v, ld_v, type, "kv_q8_read: v")) return rc;
   unsigned grid;
   if (int rc = grid_of(kv, "kv_q8_read", &grid)) return rc;
-  const Q8ReadParams p{*kv, k, v, ld_k, ld_v, q8_span_pages(*kv)};
+  const Q8ReadParams p{*kv, k, v, ld_k, ld_v, span_halves(*kv)};
   const bool bf = type == DTREE_T_BF16;
   if (kv->head_dim == 64) {
     if (bf) q8_read_kernel<64, true><<<grid, 256, 0, stream>>>(p);
