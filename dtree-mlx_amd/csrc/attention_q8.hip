@@ -961,9 +961,11 @@ size_t part_bytes(const DtreeKvQ8& kv, const DtreeAttnQ8Args& a) {
   return (size_t)kv.total_rows * a.num_heads * (kv.head_dim + 2) * sizeof(float);
 }
 
-// Workgroups the key ranges are cut for, and the fewest pages of a range.
-constexpr int kFillTokens = 4096, kFillRows = 512;
+// Workgroups of tokens that the key ranges are cut for (some hold few pages where
+// the sequences differ), and the fewest pages of a range.
+constexpr int kFillTokens = 4096;
 constexpr int kMinTokens = 16, kMinRows = 4;
+constexpr int kLongPages = 32;
 
 Plan make_plan(const DtreeKvQ8& kv, const DtreeAttnQ8Args& a) {
   const int G = a.num_heads / kv.num_kv_heads, D = kv.head_dim;
@@ -971,18 +973,21 @@ Plan make_plan(const DtreeKvQ8& kv, const DtreeAttnQ8Args& a) {
   const int64_t pairs = (int64_t)std::max(kv.max_rows, a.rows_padded) * G;
   pl.tokens = pairs <= (D == 256 ? 16 : 32);  // (registers: 32 columns of 256 dims do not fit)
   pl.nc = pairs <= 16 ? 1 : 2;
-  pl.waves = D == 128 && pairs > 128 ? 8 : 4;
-  const int wp = 32 * pl.waves;  // pairs of a workgroup of rows
-  pl.blocks = pl.tokens ? 1 : (int)((pairs + wp - 1) / wp);
   // pages that one workgroup's rows can see
   const int64_t end = std::min((int64_t)kv.max_past_length + kv.max_rows, (int64_t)kv.ld_page_table * DTREE_PAGE);
-  int64_t tiles = (end + DTREE_PAGE - 1) / DTREE_PAGE;
-  if (a.window > 0) {
-    const int64_t span = pl.tokens ? kv.max_rows : std::min(kv.max_rows, wp / G + 2);
-    tiles = std::min(tiles, ((int64_t)a.sink + DTREE_PAGE - 1) / DTREE_PAGE + (a.window + span) / DTREE_PAGE + 2);
-  }
+  const int64_t all = (end + DTREE_PAGE - 1) / DTREE_PAGE;
+  auto pages = [&](int64_t rows) {
+    if (a.window == 0) return all;
+    return std::min(all, ((int64_t)a.sink + DTREE_PAGE - 1) / DTREE_PAGE + (a.window + rows) / DTREE_PAGE + 2);
+  };
+  pl.waves = D == 128 && pairs > 128 && pages(256 / G + 2) >= kLongPages ? 8 : 4;
+  const int wp = 32 * pl.waves;  // pairs of a workgroup of rows
+  pl.blocks = pl.tokens ? 1 : (int)((pairs + wp - 1) / wp);
+  const int64_t tiles = pages(pl.tokens ? kv.max_rows : std::min(kv.max_rows, wp / G + 2));
   const int64_t units = (int64_t)kv.num_seqs * kv.num_kv_heads * pl.blocks;
-  const int64_t most = std::max<int64_t>(1, (pl.tokens ? kFillTokens : kFillRows) / units);
+  // rows: as many workgroups as the CUs hold at once
+  const int fill = pl.tokens ? kFillTokens : D == 256 || pl.waves == 8 ? 256 : 512;
+  const int64_t most = std::max<int64_t>(1, fill / units);
   pl.per = (int)std::max<int64_t>(pl.tokens ? kMinTokens : kMinRows, (tiles + most - 1) / most);
   pl.parts = (int)((tiles + pl.per - 1) / pl.per);
   return pl;

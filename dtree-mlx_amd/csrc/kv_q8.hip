@@ -12,6 +12,7 @@
 // one kv head. The rows' side is read and written in runs of their dims, the
 // pages' side in runs of their pieces, and LDS, rows of bytes, lies between.
 #include <cmath>
+#include <type_traits>
 
 #include "kv_q8.h"
 
@@ -129,27 +130,45 @@ __global__ __launch_bounds__(256) void q8_append_kernel(Q8AppendParams p) {
   constexpr int LS = D / 4 + 4;                // words of a row in LDS, 16-byte pieces on their own banks
   __shared__ __attribute__((aligned(16))) uint32_t lds[2][kHalf][LS];  // K rows, V rows
   const int g = blockIdx.x % p.kv.num_kv_heads;
-  const Half w = q8_half(p.kv, blockIdx.x / p.kv.num_kv_heads, p.span);
-  if (w.page < 0) return;
-  const size_t blk = (size_t)w.page * p.kv.num_kv_heads + g;
-  const int tid = threadIdx.x, j = tid % TPR, n = w.hi - w.lo, half = p.rope_dims / 2;
+  const int tid = threadIdx.x, j = tid % TPR, half = p.rope_dims / 2;
   const Q8Pieces pc = q8_pieces<D>(p.rope_dims, j);
-  const int at0 = g * D + pc.at[0], at1 = g * D + pc.at[1];
+  f32x4_t w0 = {1.f, 1.f, 1.f, 1.f}, w1 = w0;
+  if (p.k_norm) {  // (tables and weights at any address of their type)
+    u32x2_t a, b;
+    __builtin_memcpy(&a, p.k_norm + pc.at[0], 8);
+    __builtin_memcpy(&b, p.k_norm + pc.at[1], 8);
+    w0 = q8_bf4(a);
+    w1 = q8_bf4(b);
+  }
+  const Half w = q8_half(p.kv, blockIdx.x / p.kv.num_kv_heads, p.span);
+  if (w.lo >= w.hi) return;
+  const size_t blk = (size_t)w.page * p.kv.num_kv_heads + g;
+  const int n = w.hi - w.lo, at0 = g * D + pc.at[0], at1 = g * D + pc.at[1];
   // K rows, then V rows
   for (int i = tid / TPR; i < 2 * n; i += RPP) {
     const bool is_k = i < n;
     const int slot = w.lo + (is_k ? i : i - n);
     const size_t row = w.row0 + w.first + slot;
     const size_t base = row * (is_k ? p.ld_k : p.ld_v);
-    f32x4_t x0, x1;
+    // One round of loads: what does not rotate reads its row in the tables' place.
+    using T = std::conditional_t<BF16, uint16_t, float>;
+    const T* src = static_cast<const T*>(is_k ? p.k : p.v) + base;
+    const bool turns = is_k && pc.turns;
+    const size_t tab = row * half + 4 * j;
+    const void* tc = turns ? static_cast<const void*>(p.cos + tab) : src + g * D;
+    const void* ts = turns ? static_cast<const void*>(p.sin + tab) : src + g * D;
+    f32x4_t x0, x1, cs, sn;
     if constexpr (BF16) {
-      const uint16_t* s = static_cast<const uint16_t*>(is_k ? p.k : p.v) + base;
-      x0 = q8_bf4(*reinterpret_cast<const u32x2_t*>(s + at0));
-      x1 = q8_bf4(*reinterpret_cast<const u32x2_t*>(s + at1));
+      const u32x2_t a = *reinterpret_cast<const u32x2_t*>(src + at0), b = *reinterpret_cast<const u32x2_t*>(src + at1);
+      __builtin_memcpy(&cs, tc, 16);
+      __builtin_memcpy(&sn, ts, 16);
+      x0 = q8_bf4(a);
+      x1 = q8_bf4(b);
     } else {
-      const float* s = static_cast<const float*>(is_k ? p.k : p.v) + base;
-      x0 = *reinterpret_cast<const f32x4_t*>(s + at0);
-      x1 = *reinterpret_cast<const f32x4_t*>(s + at1);
+      x0 = *reinterpret_cast<const f32x4_t*>(src + at0);
+      x1 = *reinterpret_cast<const f32x4_t*>(src + at1);
+      __builtin_memcpy(&cs, tc, 16);
+      __builtin_memcpy(&sn, ts, 16);
     }
     double x[8];
 #pragma unroll
@@ -157,35 +176,24 @@ __global__ __launch_bounds__(256) void q8_append_kernel(Q8AppendParams p) {
       x[e] = x0[e];
       x[4 + e] = x1[e];
     }
-    if (is_k) {
-      f32x4_t cs, sn;
-      if (pc.turns) {  // (tables and weights at any address of their type)
-        __builtin_memcpy(&cs, p.cos + row * half + 4 * j, 16);
-        __builtin_memcpy(&sn, p.sin + row * half + 4 * j, 16);
+    if (is_k && p.k_norm) {
+      double ss = 0.;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ss = fma(x[e], x[e], ss);
+      ss = over_row<TPR>(ss, [](double a, double b) { return a + b; });
+      const double rs = rsqrt64(ss * (1.0 / D) + p.eps);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[e] *= rs * w0[e];
+        x[4 + e] *= rs * w1[e];
       }
-      if (p.k_norm) {
-        u32x2_t a, b;
-        __builtin_memcpy(&a, p.k_norm + pc.at[0], 8);
-        __builtin_memcpy(&b, p.k_norm + pc.at[1], 8);
-        const f32x4_t w0 = q8_bf4(a), w1 = q8_bf4(b);
-        double ss = 0.;
+    }
+    if (turns) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss = fma(x[e], x[e], ss);
-        ss = over_row<TPR>(ss, [](double a, double b) { return a + b; });
-        const double rs = rsqrt64(ss * (1.0 / D) + p.eps);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          x[e] *= rs * w0[e];
-          x[4 + e] *= rs * w1[e];
-        }
-      }
-      if (pc.turns) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const double a = x[e], b = x[4 + e];
-          x[e] = a * cs[e] - b * sn[e];
-          x[4 + e] = a * sn[e] + b * cs[e];
-        }
+      for (int e = 0; e < 4; ++e) {
+        const double a = x[e], b = x[4 + e];
+        x[e] = a * cs[e] - b * sn[e];
+        x[4 + e] = a * sn[e] + b * cs[e];
       }
     }
     uint32_t q[2];
@@ -194,9 +202,10 @@ __global__ __launch_bounds__(256) void q8_append_kernel(Q8AppendParams p) {
     uint32_t* o = lds[is_k ? 0 : 1][slot];
     o[pc.at[0] / 4] = q[0];
     o[pc.at[1] / 4] = q[1];
-    if (j == 0) (is_k ? p.kv.k_scales : p.kv.v_scales)[blk * DTREE_PAGE + w.b * kHalf + slot] = scale;
+    if (j == 0 && w.page >= 0) (is_k ? p.kv.k_scales : p.kv.v_scales)[blk * DTREE_PAGE + w.b * kHalf + slot] = scale;
   }
   __syncthreads();
+  if (w.page < 0) return;  // (not before: the page's number comes behind the rows)
   int8_t* kp = p.kv.k_pages + blk * (DTREE_PAGE * D) + w.b * kHalf * D;
   int8_t* vp = p.kv.v_pages + blk * (DTREE_PAGE * D) + w.b * kHalf * D;
   // K: piece u = (dims 16 (u / 32) .., slot u % 32)
