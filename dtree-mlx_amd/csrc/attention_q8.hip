@@ -599,13 +599,17 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 8 / W : 1) void q8_rows_kernel(A
   constexpr int RF = 4;                            // fragments loaded ahead
   constexpr int WP = 32 * W;                       // pairs of the workgroup
   constexpr int RS = D + 4;  // a pair's row in `red`
+  // Three pages where LDS has room beside the outputs: the next page can then be
+  // staged while the last one's V is read, with one barrier a page, and its K read
+  // ahead; with two it waits for that between two barriers.
+  constexpr int NBUF = D == 64 || W == 8 ? 3 : 2;
   union Lds {
-    unsigned char kv[2][4 * PB];  // fp16 K, then V
+    unsigned char kv[NBUF][4 * PB];  // fp16 K, then V
     uint16_t q[WP * (D + 8)];
     float red[W][32 * RS];
   };
   __shared__ __attribute__((aligned(16))) Lds lds;
-  __shared__ __attribute__((aligned(16))) float scl[2][192];
+  __shared__ __attribute__((aligned(16))) float scl[NBUF][192];
   __shared__ float wmax[W];
   __shared__ uint32_t anc[WP][DTREE_MASK_WORDS];
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, h = lane >> 5;
@@ -719,17 +723,18 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 8 / W : 1) void q8_rows_kernel(A
     if (r & 1) ph[r >> 3][(r >> 1) & 3] = pack_h2(x[r - 1], x[r]);
   };
   // PV of the last step (its V: half vh of buffer vbuf; its logits `old`), the logits
-  // `cur` of this one (half b of buffer buf); STAGE: the raw page to buffer sbuf.
-  auto block1 = [&](f32x16_t& old, f32x16_t& cur, int vbuf, int vh, int buf, int b, auto stage, int sbuf) {
+  // `cur` of this one (half b of buffer buf, whose 1 / vs it loads). STAGE: the raw
+  // page to buffer sbuf. AHEAD: the first K fragments (half kh of kbuf) of block2.
+  auto block1 = [&](f32x16_t& old, f32x16_t& cur, int vbuf, int vh, int buf, int b, auto stage, int sbuf, auto ahead,
+                    int kbuf, int kh) {
     constexpr int ST = NF / 2 > 2 ? NF / 2 - 1 : 1;  // slots of the logits
     constexpr int SW = 8 * NP / NF;                  // words converted per slot
-    consts(ks, buf, 0, b);
-    consts(lv, buf, 1, b);
     mx = kFloor;
 #pragma unroll
     for (int k = 0; k < NF; ++k) {
       o[k % NB] = mfma32_f16(vf[k % RF], ph[k / NB], o[k % NB]);
       if (k + RF < NF) vf[k % RF] = v_frag(vbuf, vh, k + RF);
+      else if constexpr (decltype(ahead)::value) kf[k + RF - NF] = k_frag(kbuf, kh, k + RF - NF);
       if constexpr (decltype(stage)::value) {
 #pragma unroll
         for (int i = k * SW; i < (k + 1) * SW; ++i) stage_word(sbuf, i / 4, i % 4);
@@ -746,6 +751,7 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 8 / W : 1) void q8_rows_kernel(A
             mx = fmaxf(mx, cur[r]);
           }
         }
+        if (j == 0) consts(iv, buf, 2, b);
         if (j == NF / 2 - 1) mx = max_halves(mx);
       }
       __builtin_amdgcn_sched_barrier(0);
@@ -777,8 +783,9 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 8 / W : 1) void q8_rows_kernel(A
 #pragma unroll
     for (int f = 0; f < RF; ++f) kf[f] = k_frag(buf, b, f);
   };
-  // S of the next step (half b of buffer buf) to `next`, the weights of `cur`'s
-  // first 16 keys, the first V fragments (half vh of vbuf) of the next block1.
+  // S of the next step (half b of buffer buf, whose ks and log2 vs it loads) to
+  // `next`, the weights of `cur`'s first 16 keys, the first V fragments (half vh of
+  // vbuf) of the next block1.
   auto block2 = [&](f32x16_t& cur, f32x16_t& next, int buf, int b, int vbuf, int vh) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) next[r] = 0.f;
@@ -787,6 +794,8 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 8 / W : 1) void q8_rows_kernel(A
       next = mfma32_f16(kf[k % RF], qf[k], next);
       if (k + RF < NF) kf[k % RF] = k_frag(buf, b, k + RF);
       else vf[k + RF - NF] = v_frag(vbuf, vh, k + RF - NF);
+      if (k == 0) consts(ks, buf, 0, b);
+      if (k == NF / 4) consts(lv, buf, 1, b);
 #pragma unroll
       for (int r = k * 8 / NF; r < (k + 1) * 8 / NF; ++r) weight(cur, r);
       __builtin_amdgcn_sched_barrier(0);
@@ -809,30 +818,41 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 8 / W : 1) void q8_rows_kernel(A
   consts(iv, 0, 2, 0);
   k_ahead(0, 0);
   block2(sb, sa, 0, 0, 0, 0);
-  int vbuf = 0, vh = 0;  // where the last step's V is
+  int vbuf = 0, vh = 0, buf = 0;  // where the last step's V is; this page
+  constexpr std::true_type yes{};
+  constexpr std::false_type no{};
   for (int t = t0; t < t1; ++t) {
-    const int buf = (t - t0) & 1, k0 = DTREE_PAGE * rg.page(t);
+    const int k0 = DTREE_PAGE * rg.page(t), then = buf + 1 == NBUF ? 0 : buf + 1;  // the next page's buffer
     const bool masked = !here || hidden(k0);
-    block1(sb, sa, vbuf, vh, buf, 0, std::false_type{}, 0);
-    k_ahead(buf, 1);
-    consts(iv, buf, 2, 0);
-    limits(sa, masked, here, k0);
-    block2(sa, sb, buf, 1, buf, 0);
-    lds_barrier();  // the other buffer's last readers are done
-    stage_scales(buf ^ 1);
-    block1(sa, sb, buf, 0, buf, 1, std::true_type{}, buf ^ 1);
-    lds_barrier();  // page t + 1 is there
-    k_ahead(buf ^ 1, 0);
-    consts(iv, buf, 2, 1);
+    bool soon;
+    if constexpr (NBUF == 3) {
+      stage_scales(then);
+      block1(sb, sa, vbuf, vh, buf, 0, yes, then, yes, buf, 1);
+      soon = load(t + 2 - t0);
+      limits(sa, masked, here, k0);
+      block2(sa, sb, buf, 1, buf, 0);
+      lds_barrier();  // page t + 1 is there, and the last readers of page t - 1 are done
+      block1(sa, sb, buf, 0, buf, 1, no, 0, yes, then, 0);
+    } else {
+      block1(sb, sa, vbuf, vh, buf, 0, no, 0, yes, buf, 1);
+      limits(sa, masked, here, k0);
+      block2(sa, sb, buf, 1, buf, 0);
+      lds_barrier();  // the other buffer's last readers are done
+      stage_scales(then);
+      block1(sa, sb, buf, 0, buf, 1, yes, then, no, 0, 0);
+      lds_barrier();  // page t + 1 is there
+      k_ahead(then, 0);
+      soon = load(t + 2 - t0);
+    }
     limits(sb, masked, here, k0 + 32);
-    const bool soon = load(t + 2 - t0);
-    block2(sb, sa, buf ^ 1, 0, buf, 1);
+    block2(sb, sa, then, 0, buf, 1);
     vbuf = buf;
     vh = 1;
+    buf = then;
     here = next;
     next = soon;
   }
-  block1(sb, sa, vbuf, vh, vbuf, 0, std::false_type{}, 0);
+  block1(sb, sa, vbuf, vh, vbuf, 0, no, 0, no, 0, 0);
   lds_barrier();  // every wave has read the pages
   // The outputs through LDS, each wave its own part: rows of D values, 8 a lane.
   const bool plain = used == 1 && p.plain;
