@@ -588,9 +588,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void q8_token_kernel(AttnQ8P
 // keys are taken, then PV (block1): of the first 16 keys while the weights of the
 // others are taken, of the others while the next step's logits are scaled, with
 // the next page's conversion in every second block1. A slot is one MFMA, the loads
-// that a later slot needs and a share of the VALU work, in this order
-// (sched_barrier: the compiler keeps it), so that neither unit waits for the other
-// to finish a step.
+// that a later slot needs and a share of the VALU work, and the code is written in
+// that order: with each product before or behind all of its softmax, neither unit
+// was busy for half the time. Two waves a SIMD: one of 64 pairs, with half the LDS
+// reads, took 8 % longer, since a wave alone issues one instruction at a time.
 template <int D, int W>
 __global__ __launch_bounds__(64 * W, D <= 128 ? 8 / W : 1) void q8_rows_kernel(AttnQ8Params p) {
   constexpr int NB = D / 32, PB = DTREE_PAGE * D;  // bytes of a page's K (or V) as int8
@@ -754,7 +755,6 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 8 / W : 1) void q8_rows_kernel(A
         if (j == 0) consts(iv, buf, 2, b);
         if (j == NF / 2 - 1) mx = max_halves(mx);
       }
-      __builtin_amdgcn_sched_barrier(0);
     }
   };
   // What the rows may not see; the output rescaled where a row's maximum has grown.
@@ -798,7 +798,6 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 8 / W : 1) void q8_rows_kernel(A
       if (k == NF / 4) consts(lv, buf, 1, b);
 #pragma unroll
       for (int r = k * 8 / NF; r < (k + 1) * 8 / NF; ++r) weight(cur, r);
-      __builtin_amdgcn_sched_barrier(0);
     }
     asm volatile("" : "+v"(ph[0]), "+v"(l));  // taken here, not sunk to their use
   };
@@ -981,10 +980,17 @@ size_t part_bytes(const DtreeKvQ8& kv, const DtreeAttnQ8Args& a) {
   return (size_t)kv.total_rows * a.num_heads * (kv.head_dim + 2) * sizeof(float);
 }
 
-// Workgroups of tokens that the key ranges are cut for (some hold few pages where
-// the sequences differ), and the fewest pages of a range.
-constexpr int kFillTokens = 4096;
-constexpr int kMinTokens = 16, kMinRows = 4;
+// Pages of a key range. Tokens: up to kOneRange pages are one range (17 pages, 8
+// workgroups: 10.2 us, in two ranges 11.0 with the join; 16 x 20 pages 12.1, 12.8).
+// More are cut so that the ranges are as many as the CUs hold at once, two
+// workgroups each, if all sequences are as long as the longest (1 x 1025 pages:
+// 32.9 us with 16 pages a range, 36.8 with 8; 1 x 125: 13.0 with 8, 16.3 with 32),
+// but not longer than kRagged where sequences differ (32 of up to 129: 31.4 us with
+// 16), and no more of them than kMost. Rows: as many workgroups as the CUs hold.
+constexpr int kOneRange = 24, kMinTokens = 8, kRagged = 16, kMost = 4096, kResident = 512;
+constexpr int kMinRows = 4;
+// 8 waves share a page's conversion where they read many (64 pages: 171 us, 4 waves
+// 181); 4 start sooner and leave less of a CU idle at the end (20: 45 us, 8 waves 50).
 constexpr int kLongPages = 32;
 
 Plan make_plan(const DtreeKvQ8& kv, const DtreeAttnQ8Args& a) {
@@ -1005,10 +1011,17 @@ Plan make_plan(const DtreeKvQ8& kv, const DtreeAttnQ8Args& a) {
   pl.blocks = pl.tokens ? 1 : (int)((pairs + wp - 1) / wp);
   const int64_t tiles = pages(pl.tokens ? kv.max_rows : std::min(kv.max_rows, wp / G + 2));
   const int64_t units = (int64_t)kv.num_seqs * kv.num_kv_heads * pl.blocks;
-  // rows: as many workgroups as the CUs hold at once
-  const int fill = pl.tokens ? kFillTokens : D == 256 || pl.waves == 8 ? 256 : 512;
-  const int64_t most = std::max<int64_t>(1, fill / units);
-  pl.per = (int)std::max<int64_t>(pl.tokens ? kMinTokens : kMinRows, (tiles + most - 1) / most);
+  auto cut = [](int64_t n, int64_t into) { return (n + into - 1) / into; };
+  int64_t per;
+  if (pl.tokens) {
+    per = std::max<int64_t>(kMinTokens, cut(tiles * units, kResident));
+    if (kv.num_seqs > 1) per = std::min<int64_t>(per, kRagged);
+    per = tiles <= kOneRange ? tiles : std::max(per, cut(tiles, std::max<int64_t>(1, kMost / units)));
+  } else {
+    const int64_t fill = D == 256 || pl.waves == 8 ? kResident / 2 : kResident;
+    per = std::max<int64_t>(kMinRows, cut(tiles, std::max<int64_t>(1, fill / units)));
+  }
+  pl.per = (int)per;
   pl.parts = (int)((tiles + pl.per - 1) / pl.per);
   return pl;
 }
@@ -1017,8 +1030,7 @@ template <int D, bool TOKENS>
 int launch_join(const AttnQ8Params& p, hipStream_t stream) {
   constexpr int NG = 1024 / D;  // groups with one pair a workgroup
   const int64_t pairs = (int64_t)p.kv.max_rows * p.a.num_heads;
-  // Groups pay where there are ranges for them to share.
-  const bool groups = p.parts >= 2 * NG;
+  const bool groups = p.parts >= NG;  // a range for each
   const dim3 grid((unsigned)(groups ? pairs : (pairs + NG - 1) / NG), (unsigned)p.kv.num_seqs);
   if (groups) q8_join_kernel<D, TOKENS, NG><<<grid, 256, 0, stream>>>(p);
   else q8_join_kernel<D, TOKENS, 1><<<grid, 256, 0, stream>>>(p);
