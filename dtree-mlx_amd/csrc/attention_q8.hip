@@ -111,17 +111,17 @@ __device__ __forceinline__ float q8_max_lanes(float a) {
 }
 
 // The queries of up to PAIRS pairs from pair0 on (q_norm, RoPE, the softmax scale
-// in log2 units), in fp16 at qs[pair][D + 8] (past `pairs`: the last row's, their
+// in log2 units), in fp16 at qs[pair][D + 8] (past `pairs` anything, their
 // results unread), moved by one power of two for the workgroup, whose inverse is
 // returned: from a bound on the values, sqrt(2 D) max |w| behind an RMSNorm, else
 // sqrt(2) times the largest finite one. W waves; the barriers wait for LDS alone.
 // No load is in a branch, so that a batch's loads go out together: lanes without a
 // rotation read a table's first entries, calls without one the row.
 template <int D, int PAIRS, int W, bool BF>
-__device__ __forceinline__ float q8_queries_of(const AttnQ8Params& p, const Q8Seq& q, int g, int pair0, uint16_t* qs,
-                                               float* wmax) {
-  constexpr int TPR = D / 8, NT = 64 * W, PPR = NT / TPR;  // PPR pairs a round
-  constexpr int NR = (PAIRS + PPR - 1) / PPR, BR = NR < 8 ? NR : 8;  // rounds; rounds in flight
+__device__ __forceinline__ float q8_queries_of(const AttnQ8Params& p, const Q8Seq& q, int g, int pair0, int pairs,
+                                               uint16_t* qs, float* wmax) {
+  constexpr int TPR = D / 8, NT = 64 * W, PPR = NT / TPR, kFlight = 8;  // PPR pairs a round
+  constexpr int NR = (PAIRS + PPR - 1) / PPR, BR = NR < kFlight ? NR : kFlight;  // rounds; rounds in flight
   constexpr int SZ = BF ? 2 : 4;
   static_assert(NR % BR == 0, "whole batches of rounds");
   const int tid = threadIdx.x, j = tid % TPR;
@@ -156,6 +156,7 @@ __device__ __forceinline__ float q8_queries_of(const AttnQ8Params& p, const Q8Se
     if constexpr (BF) return q8_bf4(u32x2_t{x[0], x[1]});
     else return __builtin_bit_cast(f32x4_t, x);
   };
+  const int rounds = min(NR, (pairs - pair0 + PPR - 1) / PPR);  // (what is behind them stays as LDS has it)
   const bool norm = p.a.q_norm != nullptr;
   f32x4_t w0 = {p.scale_log2, p.scale_log2, p.scale_log2, p.scale_log2}, w1 = w0;
   float f, inv, bound = 0.f;
@@ -173,7 +174,7 @@ __device__ __forceinline__ float q8_queries_of(const AttnQ8Params& p, const Q8Se
     bound = q8_max_lanes<TPR>(bound) * sqrtf(2.f * D);
   } else {
 #pragma unroll 1
-    for (int k = 0; k < NR; ++k) {
+    for (int k = 0; k < rounds; ++k) {
       u32x4_t x0, x1;
       size_t row;
       const char* base;
@@ -196,7 +197,7 @@ __device__ __forceinline__ float q8_queries_of(const AttnQ8Params& p, const Q8Se
   }
   q8_exponent(bound, f, inv);
 #pragma unroll 1
-  for (int k0 = 0; k0 < NR; k0 += BR) {
+  for (int k0 = 0; k0 < rounds; k0 += BR) {
     u32x4_t x[BR][2];
     f32x4_t cs[BR], sn[BR];
 #pragma unroll
@@ -241,10 +242,10 @@ __device__ __forceinline__ float q8_queries_of(const AttnQ8Params& p, const Q8Se
   return inv;
 }
 template <int D, int PAIRS, int W>
-__device__ __forceinline__ float q8_queries(const AttnQ8Params& p, const Q8Seq& q, int g, int pair0, uint16_t* qs,
-                                            float* wmax) {
-  return p.a.q_type == DTREE_T_BF16 ? q8_queries_of<D, PAIRS, W, true>(p, q, g, pair0, qs, wmax)
-                                    : q8_queries_of<D, PAIRS, W, false>(p, q, g, pair0, qs, wmax);
+__device__ __forceinline__ float q8_queries(const AttnQ8Params& p, const Q8Seq& q, int g, int pair0, int pairs,
+                                            uint16_t* qs, float* wmax) {
+  return p.a.q_type == DTREE_T_BF16 ? q8_queries_of<D, PAIRS, W, true>(p, q, g, pair0, pairs, qs, wmax)
+                                    : q8_queries_of<D, PAIRS, W, false>(p, q, g, pair0, pairs, qs, wmax);
 }
 
 // (ks, log2 vs, 1 / vs) of a key. A NaN reaches a row that sees the key through
@@ -286,25 +287,20 @@ __device__ __forceinline__ void q8_ancestors(const AttnQ8Params& p, const Q8Seq&
   }
 }
 
+// The output gate's logits at dims d .. of a pair (0 without a gate, unused).
+__device__ __forceinline__ f32x4_t q8_gate(const AttnQ8Params& p, size_t row, int head, int d) {
+  if (!p.a.gated) return f32x4_t{0.f, 0.f, 0.f, 0.f};
+  const size_t at = row * p.a.ld_q + (size_t)head * p.a.q_stride + p.kv.head_dim + d;
+  if (p.a.q_type == DTREE_T_BF16)
+    return q8_bf4(*reinterpret_cast<const u32x2_t*>(static_cast<const uint16_t*>(p.a.q) + at));
+  return *reinterpret_cast<const f32x4_t*>(static_cast<const float*>(p.a.q) + at);
+}
 // Four values of dims d .. of a pair's output, gated, stored.
-__device__ __forceinline__ void q8_store(const AttnQ8Params& p, size_t row, int head, int d, float (&y)[4]) {
-  const int D = p.kv.head_dim;
-  if (p.a.gated) {
-    const size_t at = row * p.a.ld_q + (size_t)head * p.a.q_stride + D + d;
-    float gt[4];
-    if (p.a.q_type == DTREE_T_BF16) {
-      const u32x2_t w = *reinterpret_cast<const u32x2_t*>(static_cast<const uint16_t*>(p.a.q) + at);
+__device__ __forceinline__ void q8_store(const AttnQ8Params& p, size_t row, int head, int d, f32x4_t o, f32x4_t gate) {
+  float y[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) gt[e] = __uint_as_float((e & 1) ? (w[e >> 1] & 0xffff0000u) : (w[e >> 1] << 16));
-    } else {
-      const f32x4_t w = *reinterpret_cast<const f32x4_t*>(static_cast<const float*>(p.a.q) + at);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) gt[e] = w[e];
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] = y[e] / (1.0f + __expf(-gt[e]));
-  }
-  const int col = head * D + d;
+  for (int e = 0; e < 4; ++e) y[e] = p.a.gated ? o[e] * __builtin_amdgcn_rcpf(1.0f + __expf(-gate[e])) : o[e];
+  const int col = head * p.kv.head_dim + d;
   const size_t oi = p.tiled ? tiled_index((int)row, col, p.a.ld_out) : row * p.a.ld_out + col;
   store_act4(p.a.out, p.a.out_lo, oi, y, p.h16);
 }
@@ -318,18 +314,13 @@ __device__ __forceinline__ void q8_store_zero(const AttnQ8Params& p, size_t row,
 // 1 / l, 0 where the row has seen no key.
 __device__ __forceinline__ float q8_inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
 
-// Four values of a pair to `out`, scaled by `inv`, or, of one of several ranges,
-// as they are to its partials, with the range's m and softmax sum l.
-__device__ __forceinline__ void q8_emit(const AttnQ8Params& p, bool split, int part, size_t row, int head, int d,
-                                        const float (&o)[4], float m, float l, float inv) {
-  if (split) {
-    const size_t u = ((size_t)part * p.kv.total_rows + row) * p.a.num_heads + head;
-    *reinterpret_cast<f32x4_t*>(p.part + u * p.kv.head_dim + d) = f32x4_t{o[0], o[1], o[2], o[3]};
-    if (d == 0) *reinterpret_cast<f32x2_t*>(p.part_ml + 2 * u) = f32x2_t{m, l};
-    return;
-  }
-  float y[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
-  q8_store(p, row, head, d, y);
+// Four values of a pair of one of several ranges, with the range's m and softmax
+// sum l, to the partials.
+__device__ __forceinline__ void q8_partial(const AttnQ8Params& p, int part, size_t row, int head, int d, f32x4_t o,
+                                           float m, float l) {
+  const size_t u = ((size_t)part * p.kv.total_rows + row) * p.a.num_heads + head;
+  *reinterpret_cast<f32x4_t*>(p.part + u * p.kv.head_dim + d) = o;
+  if (d == 0) *reinterpret_cast<f32x2_t*>(p.part_ml + 2 * u) = f32x2_t{m, l};
 }
 
 __device__ __forceinline__ f32x4_t mfma16_f16(u32x4_t a, u32x4_t b, f32x4_t c) {
@@ -414,7 +405,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void q8_token_kernel(AttnQ8P
   int cur = page_of(0);
   if constexpr (NC == 1) load_k(cur);
   q8_ancestors(p, q, 0, 16 * NC, pairs, anc);
-  const float inv = q8_queries<D, 16 * NC, kWaves>(p, q, g, 0, lds.q, wmax);
+  const float inv = q8_queries<D, 16 * NC, kWaves>(p, q, g, 0, pairs, lds.q, wmax);
   if constexpr (NC == 2) load_k(cur);
   load_v(cur);  // (not earlier: the queries' registers)
   u32x4_t qf[NC][2 * NJ];
@@ -564,18 +555,20 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void q8_token_kernel(AttnQ8P
   }
   lds_barrier();
   for (int u = tid; u < pairs * (D / 4); u += 256) {
-    const int pr = u / (D / 4), d = 4 * (u % (D / 4));
-    float mt = kFloor, lt = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
+    const int pr = u / (D / 4), d = 4 * (u % (D / 4)), head = g * p.G + pr % p.G;
+    const size_t row = (size_t)q.start + pr / p.G;
+    const f32x4_t gate = q8_gate(p, row, head, d);
+    float mt = kFloor, lt = 0.f;
+    f32x4_t y = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) mt = fmaxf(mt, mls[w][0][pr]);
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
       lt += mls[w][1][pr] * fast_exp2(mls[w][0][pr] - mt);
-      const f32x4_t v = *reinterpret_cast<const f32x4_t*>(lds.red + (w * 16 * NC + pr) * RS + d);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] += v[e];
+      y += *reinterpret_cast<const f32x4_t*>(lds.red + (w * 16 * NC + pr) * RS + d);
     }
-    q8_emit(p, used > 1, part, (size_t)q.start + pr / p.G, g * p.G + pr % p.G, d, y, mt, lt, q8_inverse(lt));
+    if (used > 1) q8_partial(p, part, row, head, d, y, mt, lt);
+    else q8_store(p, row, head, d, y * q8_inverse(lt), gate);
   }
 }
 
@@ -607,7 +600,7 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 8 / W : 1) void q8_rows_kernel(A
   union Lds {
     unsigned char kv[NBUF][4 * PB];  // fp16 K, then V
     uint16_t q[WP * (D + 8)];
-    float red[W][32 * RS];
+    float red[WP * RS];
   };
   __shared__ __attribute__((aligned(16))) Lds lds;
   __shared__ __attribute__((aligned(16))) float scl[NBUF][192];
@@ -664,7 +657,7 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 8 / W : 1) void q8_rows_kernel(A
   };
   bool here = load(0);
   q8_ancestors(p, q, pair0, WP, pairs, anc);
-  const float inv = q8_queries<D, WP, W>(p, q, g, pair0, lds.q, wmax);
+  const float inv = q8_queries<D, WP, W>(p, q, g, pair0, pairs, lds.q, wmax);
   u32x4_t qf[NF];
   const int pos = wpair + c < pairs ? q.past + (wpair + c) / p.G : -1;  // -1: the lane has no pair
 #pragma unroll
@@ -853,10 +846,11 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 8 / W : 1) void q8_rows_kernel(A
   }
   block1(sb, sa, vbuf, vh, vbuf, 0, no, 0, no, 0, 0);
   lds_barrier();  // every wave has read the pages
-  // The outputs through LDS, each wave its own part: rows of D values, 8 a lane.
+  // The outputs through LDS: rows of D values, 8 a thread, whichever wave they are of.
+  constexpr int U = 4;
   const bool plain = used == 1 && p.plain;
   const float lt = l + __shfl_xor(l, 32);
-  float* red = lds.red[wave];
+  float* red = lds.red + 32 * wave * RS;
 #pragma unroll
   for (int db = 0; db < NB; ++db)
 #pragma unroll
@@ -868,25 +862,41 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 8 / W : 1) void q8_rows_kernel(A
     *reinterpret_cast<f32x4_t*>(red + c * RS + D) = f32x4_t{m, used > 1 ? lt : q8_inverse(lt), __int_as_float(row),
                                                             __int_as_float(wpair + c - row * p.G)};
   }
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  const int nl = min(32, pairs - wpair) * (D / 8);
-#pragma unroll 2
-  for (int e = lane; e < nl; e += 64) {
-    const int pl = e / (D / 8), d = 8 * (e % (D / 8));
-    const f32x4_t x0 = *reinterpret_cast<const f32x4_t*>(red + pl * RS + d);
-    const f32x4_t x1 = *reinterpret_cast<const f32x4_t*>(red + pl * RS + d + 4);
-    const f32x4_t of = *reinterpret_cast<const f32x4_t*>(red + pl * RS + D);
-    const size_t row = (size_t)q.start + __float_as_int(of[2]);
-    const int head = g * p.G + __float_as_int(of[3]);
-    if (plain) {  // rows of bf16, 16 bytes a lane
-      const f32x4_t y0 = x0 * of[1], y1 = x1 * of[1];
-      *reinterpret_cast<u32x4_t*>(p.a.out + row * p.a.ld_out + head * D + d) =
-          u32x4_t{pack_bf2(y0[0], y0[1]), pack_bf2(y0[2], y0[3]), pack_bf2(y1[0], y1[1]), pack_bf2(y1[2], y1[3])};
-    } else {
-      const float a0[4] = {x0[0], x0[1], x0[2], x0[3]}, a1[4] = {x1[0], x1[1], x1[2], x1[3]};
-      q8_emit(p, used > 1, part, row, head, d, a0, of[0], of[1], of[1]);
-      q8_emit(p, used > 1, part, row, head, d + 4, a1, of[0], of[1], of[1]);
+  lds_barrier();
+  red = lds.red;
+  const int nl = min(WP, pairs - pair0) * (D / 8);
+  for (int e0 = tid; e0 < nl; e0 += NT * U) {
+    f32x4_t gate[U][2];
+    if (used == 1 && p.a.gated) {  // U pieces' gates at once: a store holds back the loads behind it
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        const int e = min(e0 + NT * k, nl - 1), pl = e / (D / 8), d = 8 * (e % (D / 8));
+        const f32x4_t of = *reinterpret_cast<const f32x4_t*>(red + pl * RS + D);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          gate[k][i] = q8_gate(p, (size_t)q.start + __float_as_int(of[2]), g * p.G + __float_as_int(of[3]), d + 4 * i);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int e = e0 + NT * k, pl = e / (D / 8), d = 8 * (e % (D / 8));
+      if (e >= nl) break;
+      const f32x4_t x0 = *reinterpret_cast<const f32x4_t*>(red + pl * RS + d);
+      const f32x4_t x1 = *reinterpret_cast<const f32x4_t*>(red + pl * RS + d + 4);
+      const f32x4_t of = *reinterpret_cast<const f32x4_t*>(red + pl * RS + D);
+      const size_t row = (size_t)q.start + __float_as_int(of[2]);
+      const int head = g * p.G + __float_as_int(of[3]);
+      if (plain) {  // rows of bf16, 16 bytes a lane
+        const f32x4_t y0 = x0 * of[1], y1 = x1 * of[1];
+        *reinterpret_cast<u32x4_t*>(p.a.out + row * p.a.ld_out + head * D + d) =
+            u32x4_t{pack_bf2(y0[0], y0[1]), pack_bf2(y0[2], y0[3]), pack_bf2(y1[0], y1[1]), pack_bf2(y1[2], y1[3])};
+      } else if (used > 1) {
+        q8_partial(p, part, row, head, d, x0, of[0], of[1]);
+        q8_partial(p, part, row, head, d + 4, x1, of[0], of[1]);
+      } else {
+        q8_store(p, row, head, d, x0 * of[1], gate[k][0]);
+        q8_store(p, row, head, d + 4, x1 * of[1], gate[k][1]);
+      }
     }
   }
 }
@@ -914,7 +924,9 @@ __global__ __launch_bounds__(256) void q8_join_kernel(AttnQ8Params p) {
   const size_t row = (size_t)q.start + (live ? r : 0), at = row * p.a.num_heads + head;
   const size_t step = (size_t)p.kv.total_rows * p.a.num_heads;
   float m = kFloor, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+  f32x4_t gate = {0.f, 0.f, 0.f, 0.f};
   if (live) {
+    gate = q8_gate(p, row, head, d);
     constexpr int U = 4;  // ranges in flight
     for (int i0 = grp; i0 < used; i0 += U * NG) {
       f32x2_t ml[U];
@@ -965,7 +977,7 @@ __global__ __launch_bounds__(256) void q8_join_kernel(AttnQ8Params p) {
       for (int e = 0; e < 4; ++e) o[e] = fmaf(f, sums[k][tid % (TPP * PPB)][e], o[e]);
     }
   }
-  if (live) q8_emit(p, false, 0, row, head, d, o, m, l, q8_inverse(l));
+  if (live) q8_store(p, row, head, d, f32x4_t{o[0], o[1], o[2], o[3]} * q8_inverse(l), gate);
 }
 
 // The launch for a record: which kernel, its grid and key ranges.
