@@ -26,11 +26,11 @@ class Qwen3TreeModel:
     """A Qwen3 target resident on one GPU (weights + verify engine)."""
 
     def __init__(self, cfg: Qwen3Config, weights: Qwen3Weights, max_past: int = 4096, layer_ids=(),
-                 max_nodes: int = 32, split_k: dict | None = None):
+                 max_nodes: int = 32, split_k: dict | None = None, kv_bits: int = 16):
         self.args = cfg
         self.weights = weights
         self.engine = Qwen3TreeEngine(cfg, weights, max_past=max_past, max_nodes=max_nodes,
-                                      layer_ids=layer_ids, split_k=split_k)
+                                      layer_ids=layer_ids, split_k=split_k, kv_bits=kv_bits)
 
     @property
     def layers(self):
@@ -63,11 +63,11 @@ class Qwen35TreeModel:
     """A Qwen3.5 hybrid target resident on one GPU (weights + verify engine)."""
 
     def __init__(self, cfg: Qwen35Config, weights: Qwen35Weights, max_past: int = 4096, layer_ids=(),
-                 max_nodes: int = 32, split_k: dict | None = None):
+                 max_nodes: int = 32, split_k: dict | None = None, kv_bits: int = 16):
         self.args = cfg
         self.weights = weights
         self.engine = Qwen35TreeEngine(cfg, weights, max_past=max_past, max_nodes=max_nodes,
-                                       layer_ids=layer_ids, split_k=split_k)
+                                       layer_ids=layer_ids, split_k=split_k, kv_bits=kv_bits)
         self.model = _Qwen35TextModel(self)
 
     @property
@@ -475,10 +475,11 @@ class LoadedTargetModel:
 
 def load_target_model(spec: str | Qwen3Config | Qwen35Config = "random:qwen3-4b", seed: int = 0,
                       max_past: int = 4096, device: str = "cuda", layer_ids=(), norm_jitter: float = 0.0,
-                      quant: str = "bf16") -> LoadedTargetModel:
+                      quant: str = "bf16", kv_bits: int = 16) -> LoadedTargetModel:
     """Random-init target (no checkpoint download: weights ~ N(0, 0.02), seeded).
     ``spec`` is "random:qwen3-4b", "random:qwen35-4b" or a Qwen3Config /
-    Qwen35Config (adapters.py:822-846 resolves a model name instead)."""
+    Qwen35Config (adapters.py:822-846 resolves a model name instead). ``kv_bits`` 8
+    keeps the KV cache in 8 bits (PagedKVCacheQ8)."""
     if isinstance(spec, (Qwen3Config, Qwen35Config)):
         cfg, name = spec, "random:custom"
     elif spec in ("random:qwen3-4b", "qwen3-4b"):
@@ -490,12 +491,12 @@ def load_target_model(spec: str | Qwen3Config | Qwen35Config = "random:qwen3-4b"
     cls = adapter_for_model_type(cfg.model_type)
     if isinstance(cfg, Qwen35Config):
         weights = Qwen35Weights.random(cfg, seed=seed, device=device, norm_jitter=norm_jitter, quant=quant)
-        model = Qwen35TreeModel(cfg, weights, max_past=max_past, layer_ids=layer_ids)
+        model = Qwen35TreeModel(cfg, weights, max_past=max_past, layer_ids=layer_ids, kv_bits=kv_bits)
     else:
         if quant == "q4":
             weights = Qwen3Weights.random_q4(cfg, seed=seed, device=device, norm_jitter=norm_jitter)
         else:
             weights = Qwen3Weights.random(cfg, seed=seed, device=device, norm_jitter=norm_jitter)
-        model = Qwen3TreeModel(cfg, weights, max_past=max_past, layer_ids=layer_ids)
+        model = Qwen3TreeModel(cfg, weights, max_past=max_past, layer_ids=layer_ids, kv_bits=kv_bits)
     return LoadedTargetModel(requested_model=name, resolved_model_path=None, model=model, tokenizer=None,
                              adapter=cls())

@@ -52,7 +52,7 @@ class DFlashGenerator:
                  draft_attention_mask: str = "auto", target_quant_bits: int | None = None,
                  target_quant_group_size: int = 64, draft_quant_bits: int | None = None,
                  draft_quant_group_size: int = 64, seed: int = 0, *, max_past: int = 4096,
-                 device: str = "cuda", tokenizer=None):
+                 device: str = "cuda", tokenizer=None, target_kv_bits: int = 16):
         torch.manual_seed(seed)
         if target_quant_bits not in (None, 4) or (target_quant_bits == 4 and target_quant_group_size != 64):
             raise NotImplementedError("target quantisation is 4-bit affine groups of 64 (or none)")
@@ -61,12 +61,13 @@ class DFlashGenerator:
         self.requested_target_model = target_model
         self.requested_draft_model = draft_model
         if isinstance(target_model, LoadedTargetModel):
-            if target_quant_bits is not None:
-                raise ValueError("target_quant_bits applies to targets built here, not to a loaded target")
+            if target_quant_bits is not None or target_kv_bits != 16:
+                raise ValueError("target_quant_bits and target_kv_bits apply to targets built here, not to a loaded "
+                                 "target")
             self.target = target_model
         else:
             self.target = load_target_model(target_model, seed=seed, max_past=max_past, device=device,
-                                            quant="q4" if target_quant_bits == 4 else "bf16")
+                                            quant="q4" if target_quant_bits == 4 else "bf16", kv_bits=target_kv_bits)
         if tokenizer is not None:
             self.target.tokenizer = tokenizer
         self.target_quantization = ({"group_size": 64, "bits": 4} if target_quant_bits == 4 else None)

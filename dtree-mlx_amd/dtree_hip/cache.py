@@ -309,14 +309,16 @@ class Qwen35Cache:
     commit writes (it reads the committed state and the accepted path).
     ``flip()`` makes the spare the committed state. A verify step that is not
     kept (``commit=False``) therefore leaves the state it started from
-    untouched and can be replayed as it is."""
+    untouched and can be replayed as it is. ``kv_bits`` 8 holds the attention
+    layers' keys and values in 8 bits."""
 
-    def __init__(self, cfg, capacity: int, device="cuda", page_order: torch.Tensor | None = None):
+    def __init__(self, cfg, capacity: int, device="cuda", page_order: torch.Tensor | None = None, kv_bits: int = 16):
         self.cfg = cfg
         self.attn_layers = cfg.attention_layers
         self.gdn_layers = cfg.linear_layers
-        self.kv = PagedKVCache(len(self.attn_layers), cfg.num_key_value_heads, cfg.head_dim, capacity,
-                               device=device, page_order=page_order)
+        self.kv = (PagedKVCacheQ8 if kv_bits == 8 else PagedKVCache)(
+            len(self.attn_layers), cfg.num_key_value_heads, cfg.head_dim, capacity, device=device,
+            page_order=page_order)
         dev = torch.device(device)
         nG = len(self.gdn_layers)
         self._windows = torch.zeros(2, nG, cfg.linear_conv_kernel_dim - 1, cfg.conv_dim, dtype=torch.float32,

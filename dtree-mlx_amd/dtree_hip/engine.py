@@ -23,7 +23,7 @@ import numpy as np
 import torch
 
 from . import _native as N
-from .cache import PagedKVCache
+from .cache import PagedKVCache, PagedKVCacheQ8
 from .config import Qwen3Config
 from .weights import W_TILED, W_TILED_F16, Q4Linear, Qwen3Weights, tile_weight, tile_weight_f16
 
@@ -124,8 +124,12 @@ class TreeEngineBase:
     # loads, reads a third fewer bytes.
     HI_ONLY = frozenset({"qkv"})
 
-    def __init__(self, cfg, weights, max_past: int, max_nodes: int = 32, layer_ids=(), split_k: dict | None = None):
+    def __init__(self, cfg, weights, max_past: int, max_nodes: int = 32, layer_ids=(), split_k: dict | None = None,
+                 kv_bits: int = 16):
         cfg.validate()
+        if kv_bits not in (8, 16):
+            raise ValueError("kv_bits is 16 (bf16 cache) or 8 (int8 rows with one fp32 scale each)")
+        self.kv_bits = kv_bits
         if not 1 <= max_nodes <= self.max_nodes_limit:
             raise NotImplementedError(f"trees of 1 .. {self.max_nodes_limit} nodes per verify step")
         self.cfg = cfg
@@ -340,6 +344,8 @@ class TreeEngineBase:
     def _prefill_attention(self, pf: dict, lw, kv: PagedKVCache, slot: int, P0: int, n: int, rows: int, st: int,
                            **geometry) -> None:
         """Causal attention of a segment's n rows (appending their K / V) in one call."""
+        if self.kv_bits == 8:
+            return self._prefill_attention_q8(pf, lw, kv, slot, P0, n, rows, st)
         c = self.cfg
         a = N.AttnArgs()
         a.qkv = pf["qkv"].data_ptr(); a.ld_qkv = pf["qkv"].shape[1]
@@ -398,8 +404,102 @@ class TreeEngineBase:
     def launch_attention_status(self, ws: torch.Tensor, st: int) -> None:
         """ORs the attention workspace's error word into the result's status
         slot (checked by read_result) and clears it."""
+        if self.kv_bits == 8:  # that attention waits for no other workgroup
+            return
         N.check(self.lib.dtree_attention_status(ws.data_ptr(), self.result.data_ptr() + 4 * self.STATUS_SLOT, st),
                 "attention status")
+
+    # ---- 8-bit KV cache (kv_bits = 8) --------------------------------------------
+    # The tree step and the prefill append their rows to the 8-bit cache and attend
+    # over it: dtree_kv_q8_append + dtree_attention_q8 in place of one
+    # dtree_tree_attention / dtree_causal_attention.
+    def _new_kv_cache(self, layers: int, capacity: int, page_order=None):
+        c = self.cfg
+        cls = PagedKVCacheQ8 if self.kv_bits == 8 else PagedKVCache
+        return cls(layers, c.num_key_value_heads, c.head_dim, capacity, device=self.dev, page_order=page_order)
+
+    def _q8_args(self, lw, qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, out: torch.Tensor,
+                 rows_padded: int) -> N.AttnQ8Args:
+        c = self.cfg
+        gated = hasattr(c, "rope_dims")  # Qwen3.5: [q | gate] per head, partial rotary
+        a = N.AttnQ8Args()
+        a.q = qkv.data_ptr(); a.q_type = N.T_F32; a.ld_q = qkv.shape[1]
+        a.q_stride = 2 * c.head_dim if gated else c.head_dim
+        a.q_norm = lw.q_norm.data_ptr(); a.eps = c.rms_norm_eps
+        a.rope_cos = cos.data_ptr(); a.rope_sin = sin.data_ptr()
+        a.rope_dims = c.rope_dims if gated else c.head_dim
+        a.out = out[0].data_ptr(); a.out_lo = self.lo_ptr(out); a.ld_out = c.q_dim; a.out_layout = self.w.layout
+        a.num_heads = c.num_attention_heads; a.scale = c.head_dim ** -0.5
+        a.gated = 1 if gated else 0; a.rows_padded = rows_padded
+        return a
+
+    def _q8_workspace(self, kv: PagedKVCacheQ8, lw) -> torch.Tensor:
+        """Room for the key ranges of every prefix length a tree step's grid is
+        sized for (allocated once, outside any graph capture)."""
+        ws = getattr(self, "_q8_ws", None)
+        if ws is None:
+            a = self._q8_args(lw, self.qkv, self.rope_cos, self.rope_sin, self.attn, self.MP)
+            need = 16
+            for past in {min(b, self.max_past) for b in (*self.ATTN_GRID_PAST, self.max_past)}:
+                r = kv.record(0, self.desc.data_ptr(), self.desc.data_ptr(), past, self.max_nodes, self.MP)
+                need = max(need, self.lib.dtree_attention_q8_workspace_bytes(C.byref(r), C.byref(a)))
+            ws = self._q8_ws = torch.empty(need, dtype=torch.uint8, device=self.dev)
+        return ws
+
+    def _attention_q8(self, lw, kv: PagedKVCacheQ8, rec: N.KvQ8, a: N.AttnQ8Args, qkv: torch.Tensor, ws: torch.Tensor,
+                      st: int) -> None:
+        """Append the rows' K / V, then attend (qkv rows are [q heads | k heads | v heads])."""
+        c = self.cfg
+        k = qkv.data_ptr() + 4 * c.num_attention_heads * a.q_stride
+        ld = qkv.shape[1]
+        N.check(self.lib.dtree_kv_q8_append(
+            C.byref(rec), k, k + 4 * c.num_key_value_heads * c.head_dim, N.T_F32, ld, ld, lw.k_norm.data_ptr(),
+            c.rms_norm_eps, a.rope_cos, a.rope_sin, a.rope_dims, st), "kv append")
+        a.workspace = ws.data_ptr(); a.workspace_bytes = ws.numel()
+        N.check(self.lib.dtree_attention_q8(C.byref(rec), C.byref(a), st), "8-bit attention")
+
+    def _tree_attention_q8(self, lw, kv: PagedKVCacheQ8, layer: int, st: int) -> None:
+        """The step descriptor's tree rows at [P, P + L): lengths and ancestors are
+        read from the device, so one captured graph serves every step."""
+        d = self.desc.data_ptr()
+        rec = kv.record(layer, d + N.StepDesc.past_length.offset, d + N.StepDesc.num_nodes.offset,
+                        self.attn_grid_past(self._step_past), self.max_nodes, self.MP)
+        a = self._q8_args(lw, self.qkv, self.rope_cos, self.rope_sin, self.attn, self.MP)
+        a.ancestors = d + N.StepDesc.ancestors.offset
+        self._attention_q8(lw, kv, rec, a, self.qkv, self._q8_workspace(kv, lw), st)
+
+    def _prefill_lengths_q8(self, pf: dict, P0: int, n: int) -> None:
+        """A prompt segment's past length and row count, on the device."""
+        if self.kv_bits == 8:
+            pf["q8_lengths"] = torch.tensor([P0, n], dtype=torch.int32, device=self.dev)
+
+    def _prefill_attention_q8(self, pf: dict, lw, kv: PagedKVCacheQ8, layer: int, P0: int, n: int, rows: int,
+                              st: int) -> None:
+        at = pf["q8_lengths"]
+        rec = kv.record(layer, at.data_ptr(), at.data_ptr() + 4, P0, n, rows)
+        a = self._q8_args(lw, pf["qkv"], pf["cos"], pf["sin"], pf["attn"], rows)
+        need = self.lib.dtree_attention_q8_workspace_bytes(C.byref(rec), C.byref(a))
+        ws = pf.get("q8_ws")
+        if ws is None or ws.numel() < need:
+            ws = pf["q8_ws"] = torch.empty(max(need, 16), dtype=torch.uint8, device=self.dev)
+        self._attention_q8(lw, kv, rec, a, pf["qkv"], ws, st)
+
+    def _launch_kv_compact(self, kv, desc: torch.Tensor, select_hidden: bool, st: int) -> None:
+        """dtree_compact, or its 8-bit form, over every layer of the cache."""
+        c = self.cfg
+        if not isinstance(kv, PagedKVCacheQ8 if self.kv_bits == 8 else PagedKVCache):
+            raise TypeError(f"an engine with kv_bits {self.kv_bits} got a {type(kv).__name__}")
+        hid = (self.hidden.data_ptr() if select_hidden else None, self.hidden.shape[1],
+               self.hidden_sel.data_ptr() if select_hidden else None, st)
+        if self.kv_bits == 8:
+            N.check(self.lib.dtree_kv_q8_compact(
+                desc.data_ptr(), kv.k_pages.data_ptr(), kv.v_pages.data_ptr(), kv.k_scales.data_ptr(),
+                kv.v_scales.data_ptr(), kv.layers, kv.n_pages, c.num_key_value_heads, c.head_dim,
+                kv.page_table.data_ptr(), kv.page_table.shape[1], *hid), "compact")
+            return
+        N.check(self.lib.dtree_compact(
+            desc.data_ptr(), kv.k_pages.data_ptr(), kv.v_pages.data_ptr(), kv.layer_stride, kv.layers,
+            c.num_key_value_heads, c.head_dim, kv.page_table.data_ptr(), *hid), "compact")
 
     def launch_walk(self, st: int, aux: bool = False) -> None:
         d = self.desc_aux if aux else self.desc
@@ -650,14 +750,14 @@ class Qwen3TreeEngine(TreeEngineBase):
         H, F = c.hidden_size, c.intermediate_size
         return {"qkv": (c.qkv_dim, H), "o": (H, c.q_dim), "gu": (2 * F, H), "down": (H, F)}
 
-    def new_cache(self, page_order=None) -> PagedKVCache:
-        c = self.cfg
-        return PagedKVCache(c.num_hidden_layers, c.num_key_value_heads, c.head_dim,
-                            self.max_past + self.max_nodes, device=self.dev, page_order=page_order)
+    def new_cache(self, page_order=None) -> PagedKVCache | PagedKVCacheQ8:
+        return self._new_kv_cache(self.cfg.num_hidden_layers, self.max_past + self.max_nodes, page_order)
 
     def _attention(self, li, cache: PagedKVCache, st, write_cache=True):
         c = self.cfg
         lw = self.w.layers[li]
+        if self.kv_bits == 8:
+            return self._tree_attention_q8(lw, cache, li, st)
         a = N.AttnArgs()
         a.qkv = self.qkv.data_ptr(); a.ld_qkv = self.qkv.shape[1]
         a.q_norm = lw.q_norm.data_ptr(); a.k_norm = lw.k_norm.data_ptr(); a.eps = c.rms_norm_eps
@@ -676,6 +776,8 @@ class Qwen3TreeEngine(TreeEngineBase):
         """embed + all layers; tree K/V rows land in the cache at [P, P+L)."""
         c = self.cfg
         H = c.hidden_size
+        if not isinstance(cache, PagedKVCacheQ8 if self.kv_bits == 8 else PagedKVCache):
+            raise TypeError(f"an engine with kv_bits {self.kv_bits} got a {type(cache).__name__}")
         if cache.capacity < self.max_past + self.max_nodes:
             raise ValueError("cache capacity is smaller than max_past + max_nodes")
         emb, emb_layout, emb_sb = self._embedding()
@@ -779,6 +881,7 @@ class Qwen3TreeEngine(TreeEngineBase):
                 self.w.layers[0].input_norm.data_ptr(), rows, pf["x"].data_ptr(), pf["xg"][0].data_ptr(),
                 self.lo_ptr(pf["xg"]), self.w.layout, pf["ss"].data_ptr(), st), "embed tokens")
             self._prefill_rope(pf, P0, rows, D, st)
+            self._prefill_lengths_q8(pf, P0, n)
             nL = c.num_hidden_layers
             for li in range(nL):
                 lw = self.w.layers[li]
@@ -804,11 +907,4 @@ class Qwen3TreeEngine(TreeEngineBase):
         return logits, hidden
 
     def launch_compact(self, cache: PagedKVCache, st: int, select_hidden: bool = True, aux: bool = False) -> None:
-        c = self.cfg
-        d = self.desc_aux if aux else self.desc
-        N.check(self.lib.dtree_compact(
-            d.data_ptr(), cache.k_pages.data_ptr(), cache.v_pages.data_ptr(), cache.layer_stride,
-            c.num_hidden_layers, c.num_key_value_heads, c.head_dim, cache.page_table.data_ptr(),
-            self.hidden.data_ptr() if select_hidden else None, self.hidden.shape[1],
-            self.hidden_sel.data_ptr() if select_hidden else None, st), "compact")
-
+        self._launch_kv_compact(cache, self.desc_aux if aux else self.desc, select_hidden, st)

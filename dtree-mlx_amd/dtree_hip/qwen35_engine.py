@@ -80,7 +80,8 @@ class Qwen35TreeEngine(TreeEngineBase):
                          accepted=accepted)
 
     def new_cache(self, page_order=None) -> Qwen35Cache:
-        return Qwen35Cache(self.cfg, self.max_past + self.max_nodes, device=self.dev, page_order=page_order)
+        return Qwen35Cache(self.cfg, self.max_past + self.max_nodes, device=self.dev, page_order=page_order,
+                           kv_bits=self.kv_bits)
 
     # ---- launches ----------------------------------------------------------------
     def gdn_args(self, li: int, cache: Qwen35Cache) -> N.GdnArgs:
@@ -109,6 +110,8 @@ class Qwen35TreeEngine(TreeEngineBase):
         ai = cache.slot[li]
         lw = self.w.layers[li]
         kv = cache.kv
+        if self.kv_bits == 8:
+            return self._tree_attention_q8(lw, kv, ai, st)
         a = N.AttnArgs()
         a.qkv = self.qkv.data_ptr(); a.ld_qkv = self.qkv.shape[1]
         a.q_norm = lw.q_norm.data_ptr(); a.k_norm = lw.k_norm.data_ptr(); a.eps = c.rms_norm_eps
@@ -173,14 +176,8 @@ class Qwen35TreeEngine(TreeEngineBase):
         """commit_qwen35_tree_path: KV compaction of the attention layers (+ the
         hidden-state select), then every GatedDeltaNet layer's window / state
         replayed along desc.accepted."""
-        c = self.cfg
         d = self.desc_aux if aux else self.desc
-        kv = cache.kv
-        N.check(self.lib.dtree_compact(
-            d.data_ptr(), kv.k_pages.data_ptr(), kv.v_pages.data_ptr(), kv.layer_stride, kv.layers,
-            c.num_key_value_heads, c.head_dim, kv.page_table.data_ptr(),
-            self.hidden.data_ptr() if select_hidden else None, self.hidden.shape[1],
-            self.hidden_sel.data_ptr() if select_hidden else None, st), "compact")
+        self._launch_kv_compact(cache.kv, d, select_hidden, st)
         self._commit_gdn(cache, st, d)
 
     def _commit_gdn(self, cache: Qwen35Cache, st: int, desc: torch.Tensor) -> None:
@@ -330,6 +327,7 @@ class Qwen35TreeEngine(TreeEngineBase):
                 self.w.layers[0].input_norm.data_ptr(), rows, pf["x"].data_ptr(), pf["xg"][0].data_ptr(),
                 self.lo_ptr(pf["xg"]), self.w.layout, pf["ss"].data_ptr(), st), "embed tokens")
             self._prefill_rope(pf, P0, rows, c.rope_dims, st)
+            self._prefill_lengths_q8(pf, P0, n)
             nL = c.num_hidden_layers
             for li in range(nL):
                 lw = self.w.layers[li]
