@@ -264,6 +264,7 @@ class PagedKVCacheQ8:
         idx = _block_index_q8(self.head_dim, which).to(pages.device).reshape(-1)
         rows = pages[table][:, :, idx].view(n, self.kv_heads, PAGE, self.head_dim).float()
         rows = rows * scales[table].unsqueeze(-1)
+        rows = torch.where(table.view(n, 1, 1, 1) >= 0, rows, 0.0)  # pages given away read as zeros
         return rows.permute(0, 2, 1, 3).reshape(n * PAGE, self.kv_heads, self.head_dim)[:T]
 
     def logical_keys(self, layer: int, length: int | None = None, seq: int = 0) -> torch.Tensor:
@@ -284,6 +285,8 @@ class PagedKVCacheQ8:
         dev = self.k_pages.device
         pos = torch.arange(start, start + T, device=dev)
         page = self.page_table[seq].long()[pos // PAGE]
+        if bool((page < 0).any()):
+            raise ValueError("a page of these positions was given away")
         slot = pos % PAGE
         head = torch.arange(self.kv_heads, device=dev)
         for pages, scales, rows, which in ((self.k_pages[layer], self.k_scales[layer], keys, "k"),

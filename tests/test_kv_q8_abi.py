@@ -171,3 +171,18 @@ def test_cache_class_on_the_cpu():
         c.record(2, None, None, 0, 1, 1)
     with pytest.raises(ValueError):
         c.record(0, torch.zeros(2), torch.zeros(2, dtype=torch.int32), 0, 1, 1)
+
+
+def test_cache_class_with_a_page_given_away():
+    """Its positions read as zeros and take no rows; the pool's other pages stay."""
+    c = PagedKVCacheQ8(1, 2, 64, 192, device="cpu")
+    rows = torch.randn(192, 2, 64, generator=torch.Generator().manual_seed(0))
+    c.write_logical(0, rows, -rows)
+    keys = c.logical_keys(0, 192)
+    c.page_table[0, 0] = -1
+    assert torch.equal(c.logical_keys(0, 192)[64:], keys[64:])
+    assert not c.logical_keys(0, 192)[:64].any() and not c.logical_values(0, 192)[:64].any()
+    before = c.k_pages.clone()
+    with pytest.raises(ValueError):
+        c.write_logical(0, rows[:1], rows[:1], start=63)
+    assert torch.equal(c.k_pages, before)
