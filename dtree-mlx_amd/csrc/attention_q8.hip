@@ -17,6 +17,13 @@
 // whatever the scales are. q is moved by a power of two per workgroup, into the
 // upper part of fp16's range, and taken back in ks.
 // A masked key's t is -inf, whatever its scales and bytes are (u = 0 exactly).
+//
+// Two kernels. Up to 32 pairs of a sequence and KV head (decoded tokens; 16 with
+// 256 dims) are bound by the pages' bytes or, for short prefixes, by latency: the
+// token kernel, pages straight to registers. More pairs are bound by issue: the
+// rows kernel, a page converted once for 128 or 256 pairs through LDS. Both split
+// the keys into ranges where sequences are too few to fill the card, and a third
+// joins them.
 #include <algorithm>
 #include <type_traits>
 

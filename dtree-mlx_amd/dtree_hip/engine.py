@@ -164,6 +164,8 @@ class TreeEngineBase:
         self.logits = None
         self.split_k = dict(split_k or {})
         self._alloc_layer_buffers()
+        if kv_bits == 8:
+            self._alloc_q8_workspace()
         shapes = self._gemm_shapes()
         ws = max(self.lib.dtree_gemm_workspace_bytes(MP, n, k, self.split_k.get(name, 0))
                  for name, (n, k) in shapes.items())
@@ -433,18 +435,27 @@ class TreeEngineBase:
         a.gated = 1 if gated else 0; a.rows_padded = rows_padded
         return a
 
-    def _q8_workspace(self, kv: PagedKVCacheQ8, lw) -> torch.Tensor:
+    def _alloc_q8_workspace(self) -> None:
         """Room for the key ranges of every prefix length a tree step's grid is
-        sized for (allocated once, outside any graph capture)."""
-        ws = getattr(self, "_q8_ws", None)
-        if ws is None:
-            a = self._q8_args(lw, self.qkv, self.rope_cos, self.rope_sin, self.attn, self.MP)
-            need = 16
-            for past in {min(b, self.max_past) for b in (*self.ATTN_GRID_PAST, self.max_past)}:
-                r = kv.record(0, self.desc.data_ptr(), self.desc.data_ptr(), past, self.max_nodes, self.MP)
-                need = max(need, self.lib.dtree_attention_q8_workspace_bytes(C.byref(r), C.byref(a)))
-            ws = self._q8_ws = torch.empty(need, dtype=torch.uint8, device=self.dev)
-        return ws
+        sized for (here, and not at the first step, which may be a graph capture)."""
+        c = self.cfg
+        r, a = N.KvQ8(), N.AttnQ8Args()
+        r.num_kv_heads = c.num_key_value_heads; r.head_dim = c.head_dim; r.num_seqs = 1
+        r.ld_page_table = (self.max_past + self.max_nodes + 63) // 64
+        r.max_rows = self.max_nodes; r.total_rows = self.MP
+        a.num_heads = c.num_attention_heads; a.rows_padded = self.MP
+        need = 16
+        for past in {self.attn_grid_past(b) for b in (*self.ATTN_GRID_PAST, self.max_past)}:
+            r.max_past_length = past
+            need = max(need, self.lib.dtree_attention_q8_workspace_bytes(C.byref(r), C.byref(a)))
+        self.q8_ws = torch.empty(need, dtype=torch.uint8, device=self.dev)
+
+    def _check_kv(self, kv) -> None:
+        """The layers' cache is of the engine's kind and holds one sequence."""
+        if not isinstance(kv, PagedKVCacheQ8 if self.kv_bits == 8 else PagedKVCache):
+            raise TypeError(f"an engine with kv_bits {self.kv_bits} got a {type(kv).__name__}")
+        if self.kv_bits == 8 and kv.num_seqs != 1:
+            raise ValueError("the engines verify one sequence: the cache must have num_seqs 1")
 
     def _attention_q8(self, lw, kv: PagedKVCacheQ8, rec: N.KvQ8, a: N.AttnQ8Args, qkv: torch.Tensor, ws: torch.Tensor,
                       st: int) -> None:
@@ -466,7 +477,7 @@ class TreeEngineBase:
                         self.attn_grid_past(self._step_past), self.max_nodes, self.MP)
         a = self._q8_args(lw, self.qkv, self.rope_cos, self.rope_sin, self.attn, self.MP)
         a.ancestors = d + N.StepDesc.ancestors.offset
-        self._attention_q8(lw, kv, rec, a, self.qkv, self._q8_workspace(kv, lw), st)
+        self._attention_q8(lw, kv, rec, a, self.qkv, self.q8_ws, st)
 
     def _prefill_lengths_q8(self, pf: dict, P0: int, n: int) -> None:
         """A prompt segment's past length and row count, on the device."""
@@ -487,8 +498,7 @@ class TreeEngineBase:
     def _launch_kv_compact(self, kv, desc: torch.Tensor, select_hidden: bool, st: int) -> None:
         """dtree_compact, or its 8-bit form, over every layer of the cache."""
         c = self.cfg
-        if not isinstance(kv, PagedKVCacheQ8 if self.kv_bits == 8 else PagedKVCache):
-            raise TypeError(f"an engine with kv_bits {self.kv_bits} got a {type(kv).__name__}")
+        self._check_kv(kv)
         hid = (self.hidden.data_ptr() if select_hidden else None, self.hidden.shape[1],
                self.hidden_sel.data_ptr() if select_hidden else None, st)
         if self.kv_bits == 8:
@@ -776,8 +786,7 @@ class Qwen3TreeEngine(TreeEngineBase):
         """embed + all layers; tree K/V rows land in the cache at [P, P+L)."""
         c = self.cfg
         H = c.hidden_size
-        if not isinstance(cache, PagedKVCacheQ8 if self.kv_bits == 8 else PagedKVCache):
-            raise TypeError(f"an engine with kv_bits {self.kv_bits} got a {type(cache).__name__}")
+        self._check_kv(cache)
         if cache.capacity < self.max_past + self.max_nodes:
             raise ValueError("cache capacity is smaller than max_past + max_nodes")
         emb, emb_layout, emb_sb = self._embedding()
@@ -864,6 +873,7 @@ class Qwen3TreeEngine(TreeEngineBase):
             raise ValueError("token id outside the vocabulary")
         if cache.offset + len(toks) > self.max_past:
             raise ValueError(f"prefill of {len(toks)} tokens beyond max_past {self.max_past}")
+        self._check_kv(cache)
         st = self.stream_handle()
         emb, emb_layout, emb_sb = self._embedding()
         slot = {li: i for i, li in enumerate(self.layer_ids)}

@@ -132,6 +132,7 @@ class Qwen35TreeEngine(TreeEngineBase):
         [P, P + L); GatedDeltaNet per-node inputs stay in the layer buffers."""
         c = self.cfg
         H = c.hidden_size
+        self._check_kv(cache.kv)
         if cache.capacity < self.max_past + self.max_nodes:
             raise ValueError("cache capacity is smaller than max_past + max_nodes")
         emb, emb_layout, emb_sb = self._embedding()
@@ -309,6 +310,7 @@ class Qwen35TreeEngine(TreeEngineBase):
             raise ValueError("token id outside the vocabulary")
         if cache.offset + len(toks) > self.max_past:
             raise ValueError(f"prefill of {len(toks)} tokens beyond max_past {self.max_past}")
+        self._check_kv(cache.kv)
         st = self.stream_handle()
         emb, emb_layout, emb_sb = self._embedding()
         slot = {li: i for i, li in enumerate(self.layer_ids)}

@@ -217,3 +217,42 @@ def test_caches_of_the_other_kind_are_refused(gpu_device):
             eng.launch_compact(cache, eng.stream_handle())
     with pytest.raises(ValueError):
         Qwen3TreeModel(cfg, w, max_past=100, kv_bits=4)
+
+
+@pytest.mark.parametrize("family", ["qwen3", "qwen35"])
+def test_prefill_and_steps_refuse_the_other_kind(gpu_device, family):
+    cfg, cls, wcls = ((tiny_qwen3(), Qwen3TreeModel, Qwen3Weights) if family == "qwen3" else
+                      (tiny_qwen35(), Qwen35TreeModel, Qwen35Weights))
+    w = wcls.random(cfg, seed=0, device=gpu_device)
+    engines = [cls(cfg, w, max_past=256, kv_bits=bits).engine for bits in (8, 16)]
+    for eng, other in (engines, engines[::-1]):
+        cache = other.new_cache()
+        with pytest.raises(TypeError):
+            eng.prefill_long(cache, list(range(1, 129)))
+        with pytest.raises(TypeError):
+            eng.forward_only(cache, [1], [0], [-1])
+
+
+def test_a_cache_of_several_sequences_is_refused(gpu_device):
+    cfg = tiny_qwen3()
+    eng = Qwen3TreeModel(cfg, Qwen3Weights.random(cfg, seed=0, device=gpu_device), max_past=100, kv_bits=8).engine
+    cache = PagedKVCacheQ8(cfg.num_hidden_layers, cfg.num_key_value_heads, cfg.head_dim, 256, num_seqs=2,
+                           device=gpu_device)
+    for call in (lambda: eng.forward_only(cache, [1], [0], [-1]), lambda: eng.prefill_long(cache, list(range(1, 129))),
+                 lambda: eng.launch_compact(cache, eng.stream_handle())):
+        with pytest.raises(ValueError):
+            call()
+
+
+def test_first_step_from_a_captured_graph(gpu_device):
+    """A graph captured before any eager step allocates nothing, and replays as the eager step."""
+    cfg = tiny_qwen3()
+    w = Qwen3Weights.random(cfg, seed=0, device=gpu_device)
+    got = []
+    for use_graph in (True, False):
+        eng = Qwen3TreeModel(cfg, w, max_past=100, kv_bits=8).engine
+        cache = eng.new_cache()
+        res = [eng.verify(cache, [5, 6, 7], [0, 1, 2], [-1, 0, 1], use_graph=use_graph, commit=False)
+               for _ in range(3)]
+        got.append([(list(r.accepted), r.bonus_token) for r in res])
+    assert got[0] == got[1]
