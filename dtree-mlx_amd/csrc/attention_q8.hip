@@ -35,7 +35,6 @@ namespace {
 constexpr float kFloor = -3.4e38f;      // m of a row that has seen no key
 constexpr float kMinVs = 0x1p-80f;      // value scales below count as this
 constexpr float kTop = 6.f, kSlack = 8.f;  // u <= 2^kTop after a rescale, <= 2^(kTop + kSlack) before the next
-constexpr int kWaves = 4;
 
 struct AttnQ8Params {
   DtreeKvQ8 kv;
@@ -336,7 +335,7 @@ __device__ __forceinline__ f32x4_t mfma16_f16(u32x4_t a, u32x4_t b, f32x4_t c) {
 }
 
 // A workgroup: all pairs of a sequence and KV head, up to 16 NC, over one key
-// range, its pages dealt to the four waves in turn. A wave loads its pages
+// range, its pages dealt to the W waves in turn. A wave loads its pages
 // straight into registers, the next one during the current one; the waves'
 // results meet in LDS.
 //
@@ -348,18 +347,18 @@ __device__ __forceinline__ f32x4_t mfma16_f16(u32x4_t a, u32x4_t b, f32x4_t c) {
 //   8 step + ..);
 // * V's lane (dim % 16, kq) reads its 16 keys of one dim as they lie, i = 2 step,
 //   2 step + 1, and P needs no exchange.
-template <int D, int NC>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void q8_token_kernel(AttnQ8Params p) {
+template <int D, int NC, int W>
+__global__ __launch_bounds__(64 * W, D == 256 ? 1 : 8 / W) void q8_token_kernel(AttnQ8Params p) {
   constexpr int NJ = D / 64, NK = 4 * NJ, ND = D / 16;  // K loads (block, 64 dims) and V loads (16 dims) per page
   constexpr int RS = D + 4;                             // a pair's row in `red`
   union Lds {
     uint16_t q[16 * NC * (D + 8)];
-    float red[kWaves * 16 * NC * RS];
+    float red[W * 16 * NC * RS];
   };
   __shared__ __attribute__((aligned(16))) Lds lds;
-  __shared__ __attribute__((aligned(16))) float scl[kWaves][192];
-  __shared__ float mls[kWaves][2][16 * NC];
-  __shared__ float wmax[kWaves];
+  __shared__ __attribute__((aligned(16))) float scl[W][192];
+  __shared__ float mls[W][2][16 * NC];
+  __shared__ float wmax[W];
   __shared__ uint32_t anc[16 * NC][DTREE_MASK_WORDS];
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, kq = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -367,7 +366,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void q8_token_kernel(AttnQ8P
   const int part = b0 % p.parts, s = b0 / p.parts;
   const Q8Seq q = q8_seq(p.kv, s);
   if (part == 0 && q.n < p.a.rows_padded) {  // rows past the sequence's
-    for (int e = tid; e < (p.a.rows_padded - q.n) * p.G * (D / 4); e += 256)
+    for (int e = tid; e < (p.a.rows_padded - q.n) * p.G * (D / 4); e += 64 * W)
       q8_store_zero(p, q.n + e / (D / 4) / p.G, g * p.G + e / (D / 4) % p.G, 4 * (e % (D / 4)));
   }
   if (q.n == 0) return;
@@ -384,7 +383,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void q8_token_kernel(AttnQ8P
   // have to come back, and with it every load before it, to be used.
   int ids = -1;
   auto load_ids = [&](int i) {
-    const int t = t0 + wave + kWaves * (i + lane);
+    const int t = t0 + wave + W * (i + lane);
     ids = t < t1 ? q8_page(p.kv, s, rg.page(t)) : -1;
   };
   auto page_of = [&](int i) {
@@ -408,11 +407,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void q8_token_kernel(AttnQ8P
 #pragma unroll
     for (int i = 0; i < ND; ++i) vb[i] = buf_ld(rv, voff + 1024 * (i >> 1) + 256 * (i & 1));
   };
-  const int steps = max(0, (t1 - t0 - wave + kWaves - 1) / kWaves);  // the wave's pages
+  const int steps = max(0, (t1 - t0 - wave + W - 1) / W);  // the wave's pages
   int cur = page_of(0);
   if constexpr (NC == 1) load_k(cur);
   q8_ancestors(p, q, 0, 16 * NC, pairs, anc);
-  const float inv = q8_queries<D, 16 * NC, kWaves>(p, q, g, 0, pairs, lds.q, wmax);
+  const float inv = q8_queries<D, 16 * NC, W>(p, q, g, 0, pairs, lds.q, wmax);
   if constexpr (NC == 2) load_k(cur);
   load_v(cur);  // (not earlier: the queries' registers)
   u32x4_t qf[NC][2 * NJ];
@@ -441,7 +440,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void q8_token_kernel(AttnQ8P
   float* sc = scl[wave];
   for (int i = 0; i < steps; ++i) {
     const int next = page_of(i + 1);
-    const int k0 = DTREE_PAGE * rg.page(t0 + wave + kWaves * i);
+    const int k0 = DTREE_PAGE * rg.page(t0 + wave + W * i);
     {
       float k, lv, iv;
       q8_scales(ksl, vsl, inv, k, lv, iv);
@@ -536,7 +535,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void q8_token_kernel(AttnQ8P
     __builtin_amdgcn_wave_barrier();
   }
 
-  // the four waves' results
+  // the waves' results
 #pragma unroll
   for (int n = 0; n < NC; ++n) {
     l[n] += __shfl_xor(l[n], 16);
@@ -553,7 +552,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void q8_token_kernel(AttnQ8P
     if (pr >= pairs) continue;
     float mt = kFloor;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) mt = fmaxf(mt, mls[w][0][pr]);
+    for (int w = 0; w < W; ++w) mt = fmaxf(mt, mls[w][0][pr]);
     const float fac = fast_exp2(m[n] - mt);
 #pragma unroll
     for (int d = 0; d < ND; ++d)
@@ -561,16 +560,16 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void q8_token_kernel(AttnQ8P
           f32x4_t{o[n][d][0] * fac, o[n][d][1] * fac, o[n][d][2] * fac, o[n][d][3] * fac};
   }
   lds_barrier();
-  for (int u = tid; u < pairs * (D / 4); u += 256) {
+  for (int u = tid; u < pairs * (D / 4); u += 64 * W) {
     const int pr = u / (D / 4), d = 4 * (u % (D / 4)), head = g * p.G + pr % p.G;
     const size_t row = (size_t)q.start + pr / p.G;
     const f32x4_t gate = q8_gate(p, row, head, d);
     float mt = kFloor, lt = 0.f;
     f32x4_t y = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) mt = fmaxf(mt, mls[w][0][pr]);
+    for (int w = 0; w < W; ++w) mt = fmaxf(mt, mls[w][0][pr]);
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
+    for (int w = 0; w < W; ++w) {
       lt += mls[w][1][pr] * fast_exp2(mls[w][0][pr] - mt);
       y += *reinterpret_cast<const f32x4_t*>(lds.red + (w * 16 * NC + pr) * RS + d);
     }
@@ -991,7 +990,7 @@ __global__ __launch_bounds__(256) void q8_join_kernel(AttnQ8Params p) {
 struct Plan {
   bool tokens;
   int nc;     // tokens: column blocks of 16 pairs
-  int waves;  // rows: waves of 32 pairs
+  int waves;  // of a workgroup
   int blocks, parts, per;
 };
 
@@ -1007,7 +1006,11 @@ size_t part_bytes(const DtreeKvQ8& kv, const DtreeAttnQ8Args& a) {
 // but not longer than kRagged where sequences differ (32 of up to 129: 31.4 us with
 // 16), and no more of them than kMost. Rows: as many workgroups as the CUs hold.
 constexpr int kOneRange = 24, kMinTokens = 8, kRagged = 16, kMost = 4096, kResident = 512;
-constexpr int kMinRows = 4;
+// A row block's few pages are one range (4 pages, 128 dims: 14.6 us, in two 15.3;
+// 256 dims, with twice the work a page: 3 pages in two 23.3, in one 29.8). More are
+// cut down to kMinRows (25 tree rows, 33 pages: 18.4 us, with 4 pages a range 20.2),
+// with many row blocks to twice that (128 of 10 pages: 20.8 us, cut finer 22.1).
+constexpr int kMinRows = 2, kOneRows = 4, kOneRows256 = 2, kManyRows = 64;
 // 8 waves share a page's conversion where they read many (64 pages: 171 us, 4 waves
 // 181); 4 start sooner and leave less of a CU idle at the end (20: 45 us, 8 waves 50).
 constexpr int kLongPages = 32;
@@ -1038,10 +1041,16 @@ Plan make_plan(const DtreeKvQ8& kv, const DtreeAttnQ8Args& a) {
     per = tiles <= kOneRange ? tiles : std::max(per, cut(tiles, std::max<int64_t>(1, kMost / units)));
   } else {
     const int64_t fill = D == 256 || pl.waves == 8 ? kResident / 2 : kResident;
-    per = std::max<int64_t>(kMinRows, cut(tiles, std::max<int64_t>(1, fill / units)));
+    const int64_t least = units > kManyRows ? 2 * kMinRows : kMinRows;
+    per = tiles <= (D == 256 ? kOneRows256 : kOneRows)
+              ? tiles
+              : std::max(least, cut(tiles, std::max<int64_t>(1, fill / units)));
   }
   pl.per = (int)per;
   pl.parts = (int)((tiles + pl.per - 1) / pl.per);
+  // Tokens that leave CUs to spare: 8 waves, fewer pages for each (128 workgroups of
+  // 20 pages: 11.7 us, 4 waves 12.3). With 256 dims the registers hold one a SIMD.
+  if (pl.tokens && D != 256 && pl.parts * units <= kResident / 2) pl.waves = 8;
   return pl;
 }
 
@@ -1060,8 +1069,16 @@ int launch_join(const AttnQ8Params& p, hipStream_t stream) {
 template <int D>
 int launch(const AttnQ8Params& p, const Plan& pl, unsigned grid, hipStream_t stream) {
   if (pl.tokens) {
-    if (pl.nc == 1) q8_token_kernel<D, 1><<<grid, 256, 0, stream>>>(p);
-    else if constexpr (D != 256) q8_token_kernel<D, 2><<<grid, 256, 0, stream>>>(p);
+    if constexpr (D == 256) {
+      q8_token_kernel<D, 1, 4><<<grid, 256, 0, stream>>>(p);
+    } else if (pl.waves == 8) {
+      if (pl.nc == 1) q8_token_kernel<D, 1, 8><<<grid, 512, 0, stream>>>(p);
+      else q8_token_kernel<D, 2, 8><<<grid, 512, 0, stream>>>(p);
+    } else if (pl.nc == 1) {
+      q8_token_kernel<D, 1, 4><<<grid, 256, 0, stream>>>(p);
+    } else {
+      q8_token_kernel<D, 2, 4><<<grid, 256, 0, stream>>>(p);
+    }
   } else if (pl.waves == 4) {
     q8_rows_kernel<D, 4><<<grid, 256, 0, stream>>>(p);
   } else if constexpr (D == 128) {
