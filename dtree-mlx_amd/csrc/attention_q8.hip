@@ -347,6 +347,11 @@ __device__ __forceinline__ f32x4_t mfma16_f16(u32x4_t a, u32x4_t b, f32x4_t c) {
 //   8 step + ..);
 // * V's lane (dim % 16, kq) reads its 16 keys of one dim as they lie, i = 2 step,
 //   2 step + 1, and P needs no exchange.
+//
+// Measured (8 KV heads of 128, 4 query heads each): one token over 65536 keys 28.0
+// us, 138 MB at 4.9 TB/s, as a copy; 32 tokens over up to 8193 keys 27.5 us, 100 MB;
+// one over 1001 keys 10 us, all latency: lengths, page ids, the first page with the
+// query rows, 3 pages a wave, the merge.
 template <int D, int NC, int W>
 __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 8 / W) void q8_token_kernel(AttnQ8Params p) {
   constexpr int NJ = D / 64, NK = 4 * NJ, ND = D / 16;  // K loads (block, 64 dims) and V loads (16 dims) per page
@@ -591,6 +596,10 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 8 / W) void q8_token_kernel(
 // that order: with each product before or behind all of its softmax, neither unit
 // was busy for half the time. Two waves a SIMD: one of 64 pairs, with half the LDS
 // reads, took 8 % longer, since a wave alone issues one instruction at a time.
+//
+// Measured: 4096 rows, 32 heads of 128 on 8: 172 us, 0.80 PFLOP/s (a large library
+// product 1.2), MFMA busy 41 %, VALU 54 %, LDS 43 % of the time; 1000 gated rows after
+// 8192 keys, 16 heads of 256, one wave a SIMD: 186 us without the join, 0.76 PFLOP/s.
 template <int D, int W>
 __global__ __launch_bounds__(64 * W, D <= 128 ? 8 / W : 1) void q8_rows_kernel(AttnQ8Params p) {
   constexpr int NB = D / 32, PB = DTREE_PAGE * D;  // bytes of a page's K (or V) as int8
@@ -907,7 +916,8 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 8 / W : 1) void q8_rows_kernel(A
   }
 }
 
-// Adds the ranges' partial results: D / 4 threads for a pair's dims, NG groups of
+// Adds the ranges' partial results (4 to 5 us for a few tokens, latency; 1000 rows
+// of 16 heads of 256 in two ranges 12 us, 41 MB): D / 4 threads for a pair's dims, NG groups of
 // them take its ranges in turn (many ranges of few pairs), and meet in LDS.
 template <int D, bool TOKENS, int NG>
 __global__ __launch_bounds__(256) void q8_join_kernel(AttnQ8Params p) {

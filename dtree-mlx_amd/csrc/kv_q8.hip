@@ -10,7 +10,12 @@
 // All three are bound by the bytes they move (a decode step's by the launch). A
 // workgroup owns half a page (32 positions, whole 16-byte pieces of K and of V) of
 // one kv head. The rows' side is read and written in runs of their dims, the
-// pages' side in runs of their pieces, and LDS, rows of bytes, lies between.
+// pages' side in runs of their pieces, and LDS, rows of bytes, lies between (without
+// it, V's bytes one by one, 4000 rows in and out took 43 us, now 23).
+// Measured, 8 heads of 128: 4000 fp32 rows in 14.4 us (58 MB moved, 4.0 TB/s; the
+// fp64 arithmetic takes 54 % of the issue) and back in 9.4 us (4.4 TB/s); 4 x 8192
+// rows of 256 dims to bf16 28.2 us (120 MB, 4.3 TB/s, of 4.8 that a copy reaches);
+// one row 6.0 us.
 #include <cmath>
 #include <type_traits>
 
@@ -319,7 +324,8 @@ __global__ __launch_bounds__(256) void q8_read_kernel(Q8ReadParams p) {
 constexpr int kHidBlocks = 16;  // workgroups of the hidden rows' select
 
 // The accepted rows of one (layer, kv head), K or V, through LDS: a row's place
-// may be another accepted row's source.
+// may be another accepted row's source. At most 128 rows: bound by latency, hence
+// a workgroup for each, and V's bytes one by one.
 __global__ __launch_bounds__(256) void q8_compact_kernel(const DtreeStepDesc* desc, int8_t* kp, int8_t* vp, float* ks,
                                                          float* vs, int layers, int num_pages, int Hkv, int D,
                                                          const int32_t* page_table, int table_pages,
