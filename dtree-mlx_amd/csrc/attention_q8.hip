@@ -401,9 +401,9 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 8 / W) void q8_token_kernel(
   auto load_k = [&](int page) {
     const auto rk = buf_rsrc(p.kv.k_pages + block(page) * (DTREE_PAGE * D), page < 0 ? 0 : DTREE_PAGE * D);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int j = 0; j < NJ; ++j)
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) kb[i * NJ + j] = buf_ld(rk, koff + 128 * i + 2048 * j);
+      for (int i = 0; i < 4; ++i) kb[i * NJ + j] = buf_ld(rk, koff + 128 * i + 2048 * j);
     ksl = page < 0 ? 0.f : p.kv.k_scales[block(page) * DTREE_PAGE + lane];
     vsl = page < 0 ? 0.f : p.kv.v_scales[block(page) * DTREE_PAGE + lane];
   };
@@ -419,15 +419,18 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 8 / W) void q8_token_kernel(
   const float inv = q8_queries<D, 16 * NC, W>(p, q, g, 0, pairs, lds.q, wmax);
   if constexpr (NC == 2) load_k(cur);
   load_v(cur);  // (not earlier: the queries' registers)
-  u32x4_t qf[NC][2 * NJ];
+  // The queries' fragments in registers; the second block's of 128 dims is read from
+  // LDS in every step, since a register spilled waits for all loads before its own.
+  constexpr int NQ = D == 128 ? 1 : NC;
+  auto q_frag = [&](int n, int i) {
+    return *reinterpret_cast<const u32x4_t*>(lds.q + (16 * n + c) * (D + 8) + 64 * (i >> 1) + 16 * kq + 8 * (i & 1));
+  };
+  u32x4_t qf[NQ][2 * NJ];
   int pos[NC];  // the columns' positions; -1: no pair
 #pragma unroll
   for (int n = 0; n < NC; ++n) {
 #pragma unroll
-    for (int j = 0; j < NJ; ++j)
-#pragma unroll
-      for (int k = 0; k < 2; ++k)
-        qf[n][2 * j + k] = *reinterpret_cast<const u32x4_t*>(lds.q + (16 * n + c) * (D + 8) + 64 * j + 16 * kq + 8 * k);
+    for (int i = 0; i < 2 * NJ && n < NQ; ++i) qf[n][i] = q_frag(n, i);
     pos[n] = 16 * n + c < pairs ? q.past + (16 * n + c) / p.G : -1;
   }
   f32x4_t o[NC][ND];
@@ -459,17 +462,23 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 8 / W) void q8_token_kernel(
 #pragma unroll
       for (int b = 0; b < 4; ++b) st[n][b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int b = 0; b < 4; ++b)
+    for (int j = 0; j < NJ; ++j) {
+      u32x4_t qj[NC][2];
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) {
+      for (int n = 0; n < NC; ++n)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) qj[n][k] = n < NQ ? qf[n < NQ ? n : 0][2 * j + k] : q_frag(n, 2 * j + k);
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
         u32x4_t a0, a1;
         q8_to_h16(kb[b * NJ + j], a0, a1);
 #pragma unroll
         for (int n = 0; n < NC; ++n) {
-          st[n][b] = mfma16_f16(a0, qf[n][2 * j], st[n][b]);
-          st[n][b] = mfma16_f16(a1, qf[n][2 * j + 1], st[n][b]);
+          st[n][b] = mfma16_f16(a0, qj[n][0], st[n][b]);
+          st[n][b] = mfma16_f16(a1, qj[n][1], st[n][b]);
         }
       }
+    }
     load_k(next);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
