@@ -353,7 +353,7 @@ __device__ __forceinline__ f32x4_t mfma16_f16(u32x4_t a, u32x4_t b, f32x4_t c) {
 // one over 1001 keys 10 us, all latency: lengths, page ids, the first page with the
 // query rows, 3 pages a wave, the merge.
 template <int D, int NC, int W>
-__global__ __launch_bounds__(64 * W, D == 256 ? 1 : 8 / W) void q8_token_kernel(AttnQ8Params p) {
+__global__ __launch_bounds__(64 * W, 8 / W) void q8_token_kernel(AttnQ8Params p) {
   constexpr int NJ = D / 64, NK = 4 * NJ, ND = D / 16;  // K loads (block, 64 dims) and V loads (16 dims) per page
   constexpr int RS = D + 4;                             // a pair's row in `red`
   union Lds {
@@ -419,13 +419,15 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 8 / W) void q8_token_kernel(
   const float inv = q8_queries<D, 16 * NC, W>(p, q, g, 0, pairs, lds.q, wmax);
   if constexpr (NC == 2) load_k(cur);
   load_v(cur);  // (not earlier: the queries' registers)
-  // The queries' fragments in registers; the second block's of 128 dims is read from
-  // LDS in every step, since a register spilled waits for all loads before its own.
-  constexpr int NQ = D == 128 ? 1 : NC;
+  // The queries' fragments in registers; of 128 dims the first block's alone, of 256
+  // dims none, the others read from LDS in every step: two waves a SIMD have room for
+  // no more (32 x 2 tokens over 8000 keys of 256 dims: 53.6 us, with one 62.7), and a
+  // register spilled and read back waits for all loads before its own.
+  constexpr int NQ = D == 256 ? 0 : D == 128 ? 1 : NC;
   auto q_frag = [&](int n, int i) {
     return *reinterpret_cast<const u32x4_t*>(lds.q + (16 * n + c) * (D + 8) + 64 * (i >> 1) + 16 * kq + 8 * (i & 1));
   };
-  u32x4_t qf[NQ][2 * NJ];
+  u32x4_t qf[NQ ? NQ : 1][2 * NJ];
   int pos[NC];  // the columns' positions; -1: no pair
 #pragma unroll
   for (int n = 0; n < NC; ++n) {
@@ -1068,7 +1070,7 @@ Plan make_plan(const DtreeKvQ8& kv, const DtreeAttnQ8Args& a) {
   pl.per = (int)per;
   pl.parts = (int)((tiles + pl.per - 1) / pl.per);
   // Tokens that leave CUs to spare: 8 waves, fewer pages for each (128 workgroups of
-  // 20 pages: 11.7 us, 4 waves 12.3). With 256 dims the registers hold one a SIMD.
+  // 20 pages: 11.7 us, 4 waves 12.3; with 256 dims no gain, 11.6 and 11.3 for 16 of 8).
   if (pl.tokens && D != 256 && pl.parts * units <= kResident / 2) pl.waves = 8;
   return pl;
 }
