@@ -1024,9 +1024,10 @@ size_t part_bytes(const DtreeKvQ8& kv, const DtreeAttnQ8Args& a) {
 // More are cut so that the ranges are as many as the CUs hold at once, two
 // workgroups each, if all sequences are as long as the longest (1 x 1025 pages:
 // 32.9 us with 16 pages a range, 36.8 with 8; 1 x 125: 13.0 with 8, 16.3 with 32),
-// but not longer than kRagged where sequences differ (32 of up to 129: 31.4 us with
-// 16), and no more of them than kMost. Rows: as many workgroups as the CUs hold.
-constexpr int kOneRange = 24, kMinTokens = 8, kRagged = 16, kMost = 4096, kResident = 512;
+// but not longer than kRagged where sequences differ, whose short ones leave their
+// ranges empty (32 of up to 129 pages: 30.8 us, with 16 a range 31.2, with 8 32.1; 64
+// of up to 32: 19.9, 23.5, 32.0), and no more of them than kMost. Rows: as many workgroups as the CUs hold.
+constexpr int kOneRange = 24, kMinTokens = 8, kRagged = 12, kMost = 4096, kResident = 512;
 // A row block's few pages are one range (4 pages, 128 dims: 14.6 us, in two 15.3;
 // 256 dims, with twice the work a page: 3 pages in two 23.3, in one 29.8). More are
 // cut down to kMinRows (25 tree rows, 33 pages: 18.4 us, with 4 pages a range 20.2),
@@ -1070,7 +1071,7 @@ Plan make_plan(const DtreeKvQ8& kv, const DtreeAttnQ8Args& a) {
   pl.per = (int)per;
   pl.parts = (int)((tiles + pl.per - 1) / pl.per);
   // Tokens that leave CUs to spare: 8 waves, fewer pages for each (128 workgroups of
-  // 20 pages: 11.7 us, 4 waves 12.3; with 256 dims no gain, 11.6 and 11.3 for 16 of 8).
+  // 20 pages: 11.7 us, 4 waves 12.3; with 256 dims no gain).
   if (pl.tokens && D != 256 && pl.parts * units <= kResident / 2) pl.waves = 8;
   return pl;
 }
