@@ -349,7 +349,7 @@ __device__ __forceinline__ f32x4_t mfma16_f16(u32x4_t a, u32x4_t b, f32x4_t c) {
 //   2 step + 1, and P needs no exchange.
 //
 // Measured (8 KV heads of 128, 4 query heads each): one token over 65536 keys 28.0
-// us, 138 MB at 4.9 TB/s, as a copy; 32 tokens over up to 8193 keys 27.5 us, 100 MB;
+// us, 138 MB at 4.9 TB/s, as a copy; 32 tokens over up to 8193 keys 26.9 us, 100 MB;
 // one over 1001 keys 10 us, all latency: lengths, page ids, the first page with the
 // query rows, 3 pages a wave, the merge.
 template <int D, int NC, int W>
@@ -608,7 +608,7 @@ __global__ __launch_bounds__(64 * W, 8 / W) void q8_token_kernel(AttnQ8Params p)
 // was busy for half the time. Two waves a SIMD: one of 64 pairs, with half the LDS
 // reads, took 8 % longer, since a wave alone issues one instruction at a time.
 //
-// Measured: 4096 rows, 32 heads of 128 on 8: 172 us, 0.80 PFLOP/s (a large library
+// Measured: 4096 rows, 32 heads of 128 on 8: 167 to 172 us, 0.8 PFLOP/s (a large library
 // product 1.2), MFMA busy 41 %, VALU 54 %, LDS 43 % of the time; 1000 gated rows after
 // 8192 keys, 16 heads of 256, one wave a SIMD: 186 us without the join, 0.76 PFLOP/s.
 template <int D, int W>

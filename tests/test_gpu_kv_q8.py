@@ -356,6 +356,22 @@ def test_attention_causal(gpu_device, heads, past, rows):
     assert torch.equal(one, b.attend(workspace=False)) and torch.equal(b.attend(), b.attend())  # bit for bit
 
 
+@pytest.mark.parametrize("heads", list(HEADS))
+@pytest.mark.parametrize("pairs", [1, 32])
+def test_attention_of_many_sequences(gpu_device, heads, pairs):
+    """More workgroups than CUs (fewer waves each): one row a sequence, and up to 32 pairs."""
+    hq, hkv = HEADS[heads][:2]
+    S, n = 256 // hkv + 5, max(1, pairs // (hq // hkv))
+    past = [(37 * s) % 150 for s in range(S)]
+    rows = [1 + s % n for s in range(S)]
+    b = Batch(gpu_device, heads, past, rows, seed=17)
+    b.append()
+    want, tol = b.reference()
+    check(b.attend(), want, tol, BF16)
+    want, tol = b.reference(sink=3, window=70)
+    check(b.attend(sink=3, window=70), want, tol, BF16, "window")
+
+
 @pytest.mark.parametrize("heads", ["128", "256g", "64"])
 @pytest.mark.parametrize("sink,window", [(0, 1), (1, 1), (0, 64), (4, 100), (64, 65), (70, 257), (0, 5000), (5000, 3)])
 @pytest.mark.parametrize("past,rows", [([900], [1]), ([900, 30, 64], [1, 1, 1]), ([0], [200]), ([450], [140]),
