@@ -101,7 +101,10 @@ __device__ __forceinline__ double rcp64(double a) {
 }
 
 // A row's bytes (this lane's two pieces) and scale. Not finite anywhere (or beyond
-// what an fp32 scale can stand for): scale NaN, bytes 0.
+// what an fp32 scale can stand for): scale NaN, bytes 0. x / scale as x times a
+// rounded reciprocal may fall beside a border that it lies on (73.5 / 49); one
+// correction by the remainder, which fp64 holds whole for rows of 24 bits, makes
+// every quotient that ends in 1 / 2 exact, so that the tie goes to even.
 template <int TPR>
 __device__ __forceinline__ void quantise(const double (&x)[8], uint32_t (&w)[2], float& scale) {
   constexpr double kMost = 4.3e40;  // fp32's largest times 127, less a little
@@ -116,14 +119,15 @@ __device__ __forceinline__ void quantise(const double (&x)[8], uint32_t (&w)[2],
   amax = over_row<TPR>(bad ? (double)INFINITY : amax, [](double a, double b) { return fmax(a, b); });
   const bool fine = amax <= kMost;
   scale = fine ? (float)(amax * (1.0 / 127.0)) : NAN;
-  const double inv = scale > 0.f ? rcp64((double)scale) : 0.;
+  const double by = (double)scale, inv = scale > 0.f ? rcp64(by) : 0.;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     w[i] = 0;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
+      const double t = x[4 * i + e] * inv, r = rint(fma(fma(-t, by, x[4 * i + e]), inv, t));
       // (clamped: a subnormal scale may have been rounded by more than 1 / 254)
-      const int q = fine ? (int)fmin(fmax(rint(x[4 * i + e] * inv), -127.), 127.) : 0;
+      const int q = fine ? min(max((int)r, -127), 127) : 0;
       w[i] |= (uint32_t)(q & 0xff) << (8 * e);
     }
   }

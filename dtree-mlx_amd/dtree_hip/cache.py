@@ -173,8 +173,8 @@ def quantise_q8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     amax = x.abs().amax(-1)
     fine = torch.isfinite(x).all(-1)
     scale = torch.where(fine, amax / 127, torch.nan).float()
-    inv = torch.where(scale > 0, 1.0 / scale.double(), 0.0)
-    q = torch.where(fine[..., None], x, 0.0) * inv[..., None]
+    by = torch.where(scale > 0, scale.double(), torch.inf)[..., None]
+    q = torch.where(fine[..., None], x, 0.0) / by
     return torch.round(q).clamp_(-127, 127).to(torch.int8), scale
 
 

@@ -1,0 +1,33 @@
+"""Rules of the 8-bit cache that ordinary random rows do not meet, on the host.
+CPU only."""
+import torch
+
+from dtree_hip.cache import quantise_q8
+
+
+def tie_rows(dim, scales, seed=0):
+    """Rows whose scale is exactly s (max |x| = 127 s) and whose other elements
+    lie halfway between two integers: ([rows, dim] fp32, [rows, dim] integers)."""
+    g = torch.Generator().manual_seed(seed)
+    k = torch.randint(-126, 126, (len(scales), dim), generator=g)  # x / s = k + 1 / 2
+    s = torch.tensor(scales, dtype=torch.float64)[:, None]
+    x = (2 * k + 1).double() * (s / 2)
+    q = torch.where(k % 2 == 0, k, k + 1)  # to even
+    x[:, 5], q[:, 5] = 127 * s[:, 0], 127
+    assert torch.equal(x.float().double(), x)  # 24 bits hold them all
+    return x.float(), q
+
+
+SCALES = [49, 3, 7, 11, 13, 41, 107, 257, 1021, 8191, 32771, 65535, 49 * 2.0 ** -30, 41 * 2.0 ** 60, 0.75, 1.0, 64.0]
+
+
+def test_ties_go_to_even_whatever_the_scale():
+    x, want = tie_rows(128, SCALES)
+    q, scale = quantise_q8(x)
+    assert torch.equal(scale.double(), torch.tensor(SCALES, dtype=torch.float64))
+    assert torch.equal(q.long(), want)
+
+
+def test_ties_of_one_row_worked_by_hand():
+    q, scale = quantise_q8(torch.tensor([6223.0, 73.5, 171.5, -122.5]))
+    assert float(scale) == 49.0 and q.tolist() == [127, 2, 4, -2]  # 1.5, 3.5, -2.5
