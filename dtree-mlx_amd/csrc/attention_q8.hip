@@ -15,7 +15,8 @@
 // further factor before its rounding to fp16, and the running maximum m keeps
 // the largest weight times value scale of the row inside fp16's normal range
 // whatever the scales are. q is moved by a power of two per workgroup, into the
-// upper part of fp16's range, and taken back in ks.
+// upper part of fp16's range, and taken back in ks; pairs of a workgroup too far
+// apart for that by one of their own each, taken back in raw.
 // A masked key's t is -inf, whatever its scales and bytes are (u = 0 exactly).
 //
 // Two kernels. Up to 32 pairs of a sequence and KV head (decoded tokens; 16 with
@@ -34,6 +35,10 @@ namespace {
 
 constexpr float kFloor = -3.4e38f;      // m of a row that has seen no key
 constexpr float kMinVs = 0x1p-80f;      // value scales below count as this
+// Pairs without an RMSNorm whose largest values differ by more than this have an
+// exponent each: fp16 has 2^27 from a workgroup's largest value down to its
+// smallest normal one, so a pair keeps its 11 bits down to 2^-14 of its own largest.
+constexpr float kFarApart = 0x1p12f;
 constexpr float kTop = 6.f, kSlack = 8.f;  // u <= 2^kTop after a rescale, <= 2^(kTop + kSlack) before the next
 
 struct AttnQ8Params {
@@ -120,12 +125,15 @@ __device__ __forceinline__ float q8_max_lanes(float a) {
 // in log2 units), in fp16 at qs[pair][D + 8] (past `pairs` anything, their
 // results unread), moved by one power of two for the workgroup, whose inverse is
 // returned: from a bound on the values, sqrt(2 D) max |w| behind an RMSNorm, else
-// sqrt(2) times the largest finite one. W waves; the barriers wait for LDS alone.
+// sqrt(2) times the largest finite one. `wide` (one value for the workgroup): the
+// pairs' sizes are further apart than kFarApart, each is moved by a power of its
+// own, whose inverse lies behind its values in qs, and 1 is returned. W waves;
+// the barriers wait for LDS alone.
 // No load is in a branch, so that a batch's loads go out together: lanes without a
 // rotation read a table's first entries, calls without one the row.
 template <int D, int PAIRS, int W, bool BF>
 __device__ __forceinline__ float q8_queries_of(const AttnQ8Params& p, const Q8Seq& q, int g, int pair0, int pairs,
-                                               uint16_t* qs, float* wmax) {
+                                               uint16_t* qs, float (*wmax)[W], bool& wide) {
   constexpr int TPR = D / 8, NT = 64 * W, PPR = NT / TPR, kFlight = 8;  // PPR pairs a round
   constexpr int NR = (PAIRS + PPR - 1) / PPR, BR = NR < kFlight ? NR : kFlight;  // rounds; rounds in flight
   constexpr int SZ = BF ? 2 : 4;
@@ -166,6 +174,18 @@ __device__ __forceinline__ float q8_queries_of(const AttnQ8Params& p, const Q8Se
   const bool norm = p.a.q_norm != nullptr;
   f32x4_t w0 = {p.scale_log2, p.scale_log2, p.scale_log2, p.scale_log2}, w1 = w0;
   float f, inv, bound = 0.f;
+  wide = false;
+  // the largest finite value of a lane's pieces (what is not finite stays in its row)
+  auto largest = [](f32x4_t a, f32x4_t b) {
+    float t = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      t = fabsf(a[e]) < INFINITY ? fmaxf(t, fabsf(a[e])) : t;
+      t = fabsf(b[e]) < INFINITY ? fmaxf(t, fabsf(b[e])) : t;
+    }
+    return t;
+  };
+  const float unit = p.scale_log2 * 1.4142136f;
   if (norm) {
     u32x2_t a, b;  // (tables and weights at any address of their type)
     __builtin_memcpy(&a, p.a.q_norm + pc.at[0], 8);
@@ -179,33 +199,40 @@ __device__ __forceinline__ float q8_queries_of(const AttnQ8Params& p, const Q8Se
     }
     bound = q8_max_lanes<TPR>(bound) * sqrtf(2.f * D);
   } else {
+    float least = -INFINITY;  // less the smallest pair's largest value (a pair of zeros has no size)
 #pragma unroll 1
     for (int k = 0; k < rounds; ++k) {
       u32x4_t x0, x1;
       size_t row;
       const char* base;
       load(x0, x1, row, base);
-      const f32x4_t a = value(x0), b = value(x1);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        bound = fabsf(a[e]) < INFINITY ? fmaxf(bound, fabsf(a[e])) : bound;  // (what is not finite stays in its row)
-        bound = fabsf(b[e]) < INFINITY ? fmaxf(bound, fabsf(b[e])) : bound;
-      }
+      const float top = q8_max_lanes<TPR>(largest(value(x0), value(x1)));
+      bound = fmaxf(bound, top);
+      least = top > 0.f ? fmaxf(least, -top) : least;
     }
     r = r0;
     hd = h0;
     bound = max_halves(q8_max_lanes<32>(bound));
-    if ((tid & 63) == 0) wmax[tid >> 6] = bound;
+    least = max_halves(q8_max_lanes<32>(least));
+    if ((tid & 63) == 0) {
+      wmax[0][tid >> 6] = bound;
+      wmax[1][tid >> 6] = least;
+    }
     lds_barrier();
 #pragma unroll
-    for (int k = 0; k < W; ++k) bound = fmaxf(bound, wmax[k]);
-    bound *= p.scale_log2 * 1.4142136f;
+    for (int k = 0; k < W; ++k) {
+      bound = fmaxf(bound, wmax[0][k]);
+      least = fmaxf(least, wmax[1][k]);
+    }
+    wide = __builtin_amdgcn_readfirstlane(bound > -least * kFarApart);
+    bound *= unit;
   }
   q8_exponent(bound, f, inv);
 #pragma unroll 1
   for (int k0 = 0; k0 < rounds; k0 += BR) {
     u32x4_t x[BR][2];
     f32x4_t cs[BR], sn[BR];
+    float fk[BR];
 #pragma unroll
     for (int k = 0; k < BR; ++k) {
       size_t row;
@@ -216,6 +243,16 @@ __device__ __forceinline__ float q8_queries_of(const AttnQ8Params& p, const Q8Se
       const char* ts = half ? reinterpret_cast<const char*>(p.a.rope_sin) + at : base;
       __builtin_memcpy(&cs[k], tc, 16);
       __builtin_memcpy(&sn[k], ts, 16);
+      fk[k] = f;
+    }
+    if (wide) {
+#pragma unroll
+      for (int k = 0; k < BR; ++k) {
+        const int pl = tid / TPR + (k0 + k) * PPR;
+        float back;
+        q8_exponent(q8_max_lanes<TPR>(largest(value(x[k][0]), value(x[k][1]))) * unit, fk[k], back);
+        if (j == 0 && (PAIRS % PPR == 0 || pl < PAIRS)) *reinterpret_cast<float*>(qs + pl * (D + 8) + D) = back;
+      }
     }
 #pragma unroll
     for (int k = 0; k < BR; ++k) {
@@ -228,7 +265,7 @@ __device__ __forceinline__ float q8_queries_of(const AttnQ8Params& p, const Q8Se
       ss += dpp<0x141>(ss);
       if constexpr (TPR >= 16) ss += dpp<0x140>(ss);
       if constexpr (TPR >= 32) ss += swz_xor16(ss);
-      const float rs = norm ? f * __builtin_amdgcn_rsqf(ss * (1.0f / D) + p.a.eps) : f;  // (1 ulp; fp16 follows)
+      const float rs = norm ? f * __builtin_amdgcn_rsqf(ss * (1.0f / D) + p.a.eps) : fk[k];  // (1 ulp; fp16 follows)
       f32x4_t y, z;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -245,13 +282,13 @@ __device__ __forceinline__ float q8_queries_of(const AttnQ8Params& p, const Q8Se
     }
   }
   lds_barrier();
-  return inv;
+  return wide ? 1.f : inv;
 }
 template <int D, int PAIRS, int W>
 __device__ __forceinline__ float q8_queries(const AttnQ8Params& p, const Q8Seq& q, int g, int pair0, int pairs,
-                                            uint16_t* qs, float* wmax) {
-  return p.a.q_type == DTREE_T_BF16 ? q8_queries_of<D, PAIRS, W, true>(p, q, g, pair0, pairs, qs, wmax)
-                                    : q8_queries_of<D, PAIRS, W, false>(p, q, g, pair0, pairs, qs, wmax);
+                                            uint16_t* qs, float (*wmax)[W], bool& wide) {
+  return p.a.q_type == DTREE_T_BF16 ? q8_queries_of<D, PAIRS, W, true>(p, q, g, pair0, pairs, qs, wmax, wide)
+                                    : q8_queries_of<D, PAIRS, W, false>(p, q, g, pair0, pairs, qs, wmax, wide);
 }
 
 // (ks, log2 vs, 1 / vs) of a key. A NaN reaches a row that sees the key through
@@ -363,7 +400,7 @@ __global__ __launch_bounds__(64 * W, 8 / W) void q8_token_kernel(AttnQ8Params p)
   __shared__ __attribute__((aligned(16))) Lds lds;
   __shared__ __attribute__((aligned(16))) float scl[W][192];
   __shared__ float mls[W][2][16 * NC];
-  __shared__ float wmax[W];
+  __shared__ float wmax[2][W];
   __shared__ uint32_t anc[16 * NC][DTREE_MASK_WORDS];
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, kq = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -416,7 +453,8 @@ __global__ __launch_bounds__(64 * W, 8 / W) void q8_token_kernel(AttnQ8Params p)
   int cur = page_of(0);
   if constexpr (NC == 1) load_k(cur);
   q8_ancestors(p, q, 0, 16 * NC, pairs, anc);
-  const float inv = q8_queries<D, 16 * NC, W>(p, q, g, 0, pairs, lds.q, wmax);
+  bool wide;
+  const float inv = q8_queries<D, 16 * NC, W>(p, q, g, 0, pairs, lds.q, wmax, wide);
   if constexpr (NC == 2) load_k(cur);
   load_v(cur);  // (not earlier: the queries' registers)
   // The queries' fragments in registers; of 128 dims the first block's alone, of 256
@@ -429,11 +467,13 @@ __global__ __launch_bounds__(64 * W, 8 / W) void q8_token_kernel(AttnQ8Params p)
   };
   u32x4_t qf[NQ ? NQ : 1][2 * NJ];
   int pos[NC];  // the columns' positions; -1: no pair
+  float own[NC];  // what takes a column's own power of two back (wide)
 #pragma unroll
   for (int n = 0; n < NC; ++n) {
 #pragma unroll
     for (int i = 0; i < 2 * NJ && n < NQ; ++i) qf[n][i] = q_frag(n, i);
     pos[n] = 16 * n + c < pairs ? q.past + (16 * n + c) / p.G : -1;
+    own[n] = wide ? *reinterpret_cast<const float*>(lds.q + (16 * n + c) * (D + 8) + D) : 1.f;
   }
   f32x4_t o[NC][ND];
 #pragma unroll
@@ -498,7 +538,7 @@ __global__ __launch_bounds__(64 * W, 8 / W) void q8_token_kernel(AttnQ8Params p)
           const f32x4_t ks = *reinterpret_cast<const f32x4_t*>(sc + kkey + 8 * b);
           const f32x4_t lv = *reinterpret_cast<const f32x4_t*>(sc + 64 + kkey + 8 * b);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) st[n][b][e] = fmaf(st[n][b][e], ks[e], lv[e]);
+          for (int e = 0; e < 4; ++e) st[n][b][e] = fmaf(st[n][b][e] * own[n], ks[e], lv[e]);
         }
         if (masked) {
           const uint32_t sees = q8_sees(p, q, pos[n], k0 + (kkey & 32), anc[16 * n + c]) >> (kkey & 31);
@@ -630,7 +670,7 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 8 / W : 1) void q8_rows_kernel(A
   };
   __shared__ __attribute__((aligned(16))) Lds lds;
   __shared__ __attribute__((aligned(16))) float scl[NBUF][192];
-  __shared__ float wmax[W];
+  __shared__ float wmax[2][W];
   __shared__ uint32_t anc[WP][DTREE_MASK_WORDS];
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -683,7 +723,8 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 8 / W : 1) void q8_rows_kernel(A
   };
   bool here = load(0);
   q8_ancestors(p, q, pair0, WP, pairs, anc);
-  const float inv = q8_queries<D, WP, W>(p, q, g, pair0, pairs, lds.q, wmax);
+  bool wide;
+  const float inv = q8_queries<D, WP, W>(p, q, g, pair0, pairs, lds.q, wmax, wide);
   u32x4_t qf[NF];
   const int pos = wpair + c < pairs ? q.past + (wpair + c) / p.G : -1;  // -1: the lane has no pair
 #pragma unroll
@@ -692,6 +733,8 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 8 / W : 1) void q8_rows_kernel(A
     // (an MFMA reads its B operand from either file: not the one the softmax needs)
     if constexpr (D == 256) asm("" : "+a"(qf[i]));
   }
+  // what takes the lane's own power of two back (wide)
+  const float own = wide ? *reinterpret_cast<const float*>(lds.q + (32 * wave + c) * (D + 8) + D) : 1.f;
   lds_barrier();
   auto stage_scales = [&](int buf) {
     if (tid < DTREE_PAGE) {
@@ -819,6 +862,10 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 8 / W : 1) void q8_rows_kernel(A
       for (int r = k * 8 / NF; r < (k + 1) * 8 / NF; ++r) weight(cur, r);
     }
     asm volatile("" : "+v"(ph[0]), "+v"(l));  // taken here, not sunk to their use
+    if (wide) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) next[r] *= own;
+    }
   };
   auto hidden = [&](int k0) {  // does a page hold keys that some row may not see
     return p.a.ancestors ? k0 + DTREE_PAGE > q.past

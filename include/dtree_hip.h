@@ -654,9 +654,11 @@ int dtree_kv_q8_compact(const DtreeStepDesc* desc, int8_t* k_pages, int8_t* v_pa
  * rows_padded - 1 of out become zero.
  *
  * The products run on fp16 MFMA: q and the softmax weights are rounded to fp16
- * (11 bits, with exponents moved so that they keep them), the cached integers
- * are exact in it; sums and statistics are fp32. Value scales below 2^-80 count
- * as 2^-80.
+ * (11 bits; their exponents are moved so that a (row, head)'s query keeps them
+ * down to 2^-14 of its largest element, whatever the other rows hold; behind a
+ * q_norm down to 2^-27 of sqrt(2 head_dim) max |q_norm|), the cached integers are
+ * exact in it; sums and statistics are fp32. Value scales below 2^-80 count as
+ * 2^-80.
  * workspace: dtree_attention_q8_workspace_bytes (16-byte aligned, any contents)
  * holds partial results of key ranges; calls that share one must not overlap.
  * With less room, or none, fewer ranges are used.
