@@ -495,8 +495,8 @@ class TreeEngineBase:
             ws = pf["q8_ws"] = torch.empty(max(need, 16), dtype=torch.uint8, device=self.dev)
         self._attention_q8(lw, kv, rec, a, pf["qkv"], ws, st)
 
-    def _launch_kv_compact(self, kv, desc: torch.Tensor, select_hidden: bool, st: int) -> None:
-        """dtree_compact, or its 8-bit form, over every layer of the cache."""
+    def _launch_kv_compact(self, kv, layers: int, desc: torch.Tensor, select_hidden: bool, st: int) -> None:
+        """dtree_compact, or its 8-bit form, over the model's layers of the cache."""
         c = self.cfg
         self._check_kv(kv)
         hid = (self.hidden.data_ptr() if select_hidden else None, self.hidden.shape[1],
@@ -504,11 +504,11 @@ class TreeEngineBase:
         if self.kv_bits == 8:
             N.check(self.lib.dtree_kv_q8_compact(
                 desc.data_ptr(), kv.k_pages.data_ptr(), kv.v_pages.data_ptr(), kv.k_scales.data_ptr(),
-                kv.v_scales.data_ptr(), kv.layers, kv.n_pages, c.num_key_value_heads, c.head_dim,
+                kv.v_scales.data_ptr(), layers, kv.n_pages, c.num_key_value_heads, c.head_dim,
                 kv.page_table.data_ptr(), kv.page_table.shape[1], *hid), "compact")
             return
         N.check(self.lib.dtree_compact(
-            desc.data_ptr(), kv.k_pages.data_ptr(), kv.v_pages.data_ptr(), kv.layer_stride, kv.layers,
+            desc.data_ptr(), kv.k_pages.data_ptr(), kv.v_pages.data_ptr(), kv.layer_stride, layers,
             c.num_key_value_heads, c.head_dim, kv.page_table.data_ptr(), *hid), "compact")
 
     def launch_walk(self, st: int, aux: bool = False) -> None:
@@ -917,4 +917,4 @@ class Qwen3TreeEngine(TreeEngineBase):
         return logits, hidden
 
     def launch_compact(self, cache: PagedKVCache, st: int, select_hidden: bool = True, aux: bool = False) -> None:
-        self._launch_kv_compact(cache, self.desc_aux if aux else self.desc, select_hidden, st)
+        self._launch_kv_compact(cache, self.cfg.num_hidden_layers, self.desc_aux if aux else self.desc, select_hidden, st)

@@ -178,7 +178,7 @@ class Qwen35TreeEngine(TreeEngineBase):
         hidden-state select), then every GatedDeltaNet layer's window / state
         replayed along desc.accepted."""
         d = self.desc_aux if aux else self.desc
-        self._launch_kv_compact(cache.kv, d, select_hidden, st)
+        self._launch_kv_compact(cache.kv, cache.kv.layers, d, select_hidden, st)
         self._commit_gdn(cache, st, d)
 
     def _commit_gdn(self, cache: Qwen35Cache, st: int, desc: torch.Tensor) -> None:
