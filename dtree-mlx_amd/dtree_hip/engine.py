@@ -451,8 +451,9 @@ class TreeEngineBase:
         self.q8_ws = torch.empty(need, dtype=torch.uint8, device=self.dev)
 
     def _check_kv(self, kv) -> None:
-        """The layers' cache is of the engine's kind and holds one sequence."""
-        if not isinstance(kv, PagedKVCacheQ8 if self.kv_bits == 8 else PagedKVCache):
+        """The layers' cache is of the engine's kind and holds one sequence. (A bf16
+        engine reads fields alone: any class that has them will do.)"""
+        if isinstance(kv, PagedKVCacheQ8) != (self.kv_bits == 8):
             raise TypeError(f"an engine with kv_bits {self.kv_bits} got a {type(kv).__name__}")
         if self.kv_bits == 8 and kv.num_seqs != 1:
             raise ValueError("the engines verify one sequence: the cache must have num_seqs 1")

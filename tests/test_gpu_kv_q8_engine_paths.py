@@ -16,6 +16,38 @@ def _engine(dev, family, kv_bits, **kw):
     return model(cfg, weights.random(cfg, seed=0, device=dev, norm_jitter=0.1), kv_bits=kv_bits, **kw).engine
 
 
+class OwnCache:
+    """A caller's own cache: what the bf16 engines read of one, and no more."""
+    k_ptr, v_ptr, layer_stride = PagedKVCache.k_ptr, PagedKVCache.v_ptr, PagedKVCache.layer_stride
+
+    def __init__(self, c, fields):
+        for f in ("k_pages", "v_pages", "page_table", "n_pages", "kv_heads", "head_dim", "capacity", "offset", *fields):
+            setattr(self, f, getattr(c, f))
+
+
+@pytest.mark.parametrize("family", ["qwen3", "qwen35"])
+@pytest.mark.parametrize("use_graph", [False, True])
+def test_a_bf16_engine_takes_a_cache_of_another_class(gpu_device, family, use_graph):
+    """Prefill, step and compaction on it give what they give on PagedKVCache."""
+    got = []
+    for own in (False, True):
+        eng = _engine(gpu_device, family, 16, max_past=300)
+        cache = eng.new_cache()
+        if own and family == "qwen3":
+            cache = OwnCache(cache, ())
+        elif own:
+            cache.kv = OwnCache(cache.kv, ("layers",))
+        eng.prefill_long(cache, random_prefix(150, eng.cfg.vocab_size, seed=3))
+        P = cache.offset
+        res = [eng.verify(cache, [5, 6, 7, 8], [P, P + 1, P + 1, P + 2], [-1, 0, 0, 2], use_graph=use_graph)
+               for _ in range(2)]
+        eng.launch_compact(cache, eng.stream_handle())
+        kv = cache if family == "qwen3" else cache.kv
+        got.append(([(r.accepted, r.bonus_token, r.posterior) for r in res], cache.offset, kv.k_pages, kv.v_pages))
+    assert got[0][:2] == got[1][:2]
+    assert torch.equal(got[0][2], got[1][2]) and torch.equal(got[0][3], got[1][3])
+
+
 def test_a_step_moves_its_own_layers_rows_alone(gpu_device):
     """A cache with more layers than the model: compaction leaves the others as they are."""
     eng = _engine(gpu_device, "qwen3", 16, max_past=100)
