@@ -316,6 +316,8 @@ class Qwen35Cache:
     layers' keys and values in 8 bits."""
 
     def __init__(self, cfg, capacity: int, device="cuda", page_order: torch.Tensor | None = None, kv_bits: int = 16):
+        if kv_bits not in (8, 16):
+            raise ValueError("kv_bits is 16 (bf16 cache) or 8 (int8 rows with one fp32 scale each)")
         self.cfg = cfg
         self.attn_layers = cfg.attention_layers
         self.gdn_layers = cfg.linear_layers

@@ -1,8 +1,10 @@
 """Rules of the 8-bit cache that ordinary random rows do not meet, on the host.
 CPU only."""
+import pytest
 import torch
 
-from dtree_hip.cache import quantise_q8
+from dtree_hip import tiny_qwen35
+from dtree_hip.cache import PagedKVCache, PagedKVCacheQ8, Qwen35Cache, quantise_q8
 
 
 def tie_rows(dim, scales, seed=0):
@@ -31,3 +33,14 @@ def test_ties_go_to_even_whatever_the_scale():
 def test_ties_of_one_row_worked_by_hand():
     q, scale = quantise_q8(torch.tensor([6223.0, 73.5, 171.5, -122.5]))
     assert float(scale) == 49.0 and q.tolist() == [127, 2, 4, -2]  # 1.5, 3.5, -2.5
+
+
+@pytest.mark.parametrize("bits", [0, 4, 32, None, "8"])
+def test_hybrid_cache_refuses_other_widths(bits):
+    with pytest.raises(ValueError):
+        Qwen35Cache(tiny_qwen35(), 64, device="cpu", kv_bits=bits)
+
+
+def test_hybrid_cache_of_either_width():
+    assert type(Qwen35Cache(tiny_qwen35(), 64, device="cpu").kv) is PagedKVCache
+    assert type(Qwen35Cache(tiny_qwen35(), 64, device="cpu", kv_bits=8).kv) is PagedKVCacheQ8
