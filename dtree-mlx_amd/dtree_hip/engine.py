@@ -470,9 +470,11 @@ class TreeEngineBase:
         a.workspace = ws.data_ptr(); a.workspace_bytes = ws.numel()
         N.check(self.lib.dtree_attention_q8(C.byref(rec), C.byref(a), st), "8-bit attention")
 
-    def _tree_attention_q8(self, lw, kv: PagedKVCacheQ8, layer: int, st: int) -> None:
+    def _tree_attention_q8(self, lw, kv: PagedKVCacheQ8, layer: int, st: int, write_cache: bool = True) -> None:
         """The step descriptor's tree rows at [P, P + L): lengths and ancestors are
         read from the device, so one captured graph serves every step."""
+        if not write_cache:
+            raise NotImplementedError("the 8-bit attention reads a step's own rows from the cache: they are written")
         d = self.desc.data_ptr()
         rec = kv.record(layer, d + N.StepDesc.past_length.offset, d + N.StepDesc.num_nodes.offset,
                         self.attn_grid_past(self._step_past), self.max_nodes, self.MP)
@@ -768,7 +770,7 @@ class Qwen3TreeEngine(TreeEngineBase):
         c = self.cfg
         lw = self.w.layers[li]
         if self.kv_bits == 8:
-            return self._tree_attention_q8(lw, cache, li, st)
+            return self._tree_attention_q8(lw, cache, li, st, write_cache)
         a = N.AttnArgs()
         a.qkv = self.qkv.data_ptr(); a.ld_qkv = self.qkv.shape[1]
         a.q_norm = lw.q_norm.data_ptr(); a.k_norm = lw.k_norm.data_ptr(); a.eps = c.rms_norm_eps

@@ -111,7 +111,7 @@ class Qwen35TreeEngine(TreeEngineBase):
         lw = self.w.layers[li]
         kv = cache.kv
         if self.kv_bits == 8:
-            return self._tree_attention_q8(lw, kv, ai, st)
+            return self._tree_attention_q8(lw, kv, ai, st, write_cache)
         a = N.AttnArgs()
         a.qkv = self.qkv.data_ptr(); a.ld_qkv = self.qkv.shape[1]
         a.q_norm = lw.q_norm.data_ptr(); a.k_norm = lw.k_norm.data_ptr(); a.eps = c.rms_norm_eps

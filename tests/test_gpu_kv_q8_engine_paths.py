@@ -61,3 +61,17 @@ def test_a_step_moves_its_own_layers_rows_alone(gpu_device):
     eng.launch_compact(cache, eng.stream_handle(), select_hidden=False)
     torch.cuda.synchronize()
     assert torch.equal(cache.k_pages[-1], k) and torch.equal(cache.v_pages[-1], v)
+
+
+@pytest.mark.parametrize("family", ["qwen3", "qwen35"])
+def test_attention_without_a_cache_write_is_refused_in_8_bits(gpu_device, family):
+    """The 8-bit attention reads a step's own rows from the cache."""
+    eng = _engine(gpu_device, family, 8, max_past=100)
+    cache = eng.new_cache()
+    kv = cache if family == "qwen3" else cache.kv
+    li = eng.cfg.num_hidden_layers - 1
+    eng.set_step([5, 6], [0, 1], [-1, 0], 0)
+    with pytest.raises(NotImplementedError):
+        eng._attention(li, cache, eng.stream_handle(), write_cache=False)
+    torch.cuda.synchronize()
+    assert not kv.k_pages.any() and not kv.k_scales.any()
