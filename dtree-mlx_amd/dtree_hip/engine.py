@@ -403,7 +403,15 @@ class TreeEngineBase:
 
     STATUS_SLOT = 3 + 2 * N.MAX_NODES
 
-    def launch_attention_status(self, ws: torch.Tensor, st: int) -> None:
+    def _tree_attention_workspace(self) -> torch.Tensor | None:
+        """dtree_tree_attention's, which an engine on the 8-bit cache does not call."""
+        if self.kv_bits == 8:
+            return None
+        c = self.cfg
+        need = self.lib.dtree_attention_workspace_bytes(c.num_attention_heads, c.head_dim, self.max_past, self.MP)
+        return torch.zeros(need, dtype=torch.uint8, device=self.dev)
+
+    def launch_attention_status(self, ws: torch.Tensor | None, st: int) -> None:
         """ORs the attention workspace's error word into the result's status
         slot (checked by read_result) and clears it."""
         if self.kv_bits == 8:  # that attention waits for no other workgroup
@@ -750,8 +758,7 @@ class Qwen3TreeEngine(TreeEngineBase):
         self.act = torch.zeros(2, MP, c.intermediate_size, dtype=self.act_dtype, device=dev)
         self.rope_cos = torch.zeros(MP, c.head_dim // 2, dtype=f32, device=dev)
         self.rope_sin = torch.zeros(MP, c.head_dim // 2, dtype=f32, device=dev)
-        aws = self.lib.dtree_attention_workspace_bytes(c.num_attention_heads, c.head_dim, self.max_past, self.MP)
-        self.attn_ws = torch.zeros(aws, dtype=torch.uint8, device=dev)
+        self.attn_ws = self._tree_attention_workspace()
         # Prefix length the attention grid is sized for (launch_forward sets it
         # from the step's P); the cache's page table must cover it (the
         # kernels read page entries before P is known).
@@ -852,9 +859,10 @@ class Qwen3TreeEngine(TreeEngineBase):
                   act=torch.zeros(2, rows, F, dtype=self.act_dtype, device=dev),
                   hidden=torch.zeros(rows, nh * H, dtype=bf16, device=dev),
                   cos=torch.zeros(rows, D // 2, dtype=f32, device=dev),
-                  sin=torch.zeros(rows, D // 2, dtype=f32, device=dev),
-                  attn_ws=torch.empty(self.lib.dtree_causal_attention_workspace_bytes(c.head_dim), dtype=torch.uint8,
-                                      device=dev))
+                  sin=torch.zeros(rows, D // 2, dtype=f32, device=dev))
+        if self.kv_bits != 8:
+            pf["attn_ws"] = torch.empty(self.lib.dtree_causal_attention_workspace_bytes(c.head_dim), dtype=torch.uint8,
+                                        device=dev)
         self._pf = pf
         return pf
 

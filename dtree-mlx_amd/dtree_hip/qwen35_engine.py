@@ -60,8 +60,7 @@ class Qwen35TreeEngine(TreeEngineBase):
         self.act = torch.zeros(2, MP, c.intermediate_size, dtype=self.act_dtype, device=dev)
         self.rope_cos = torch.zeros(MP, c.rope_dims // 2, dtype=f32, device=dev)
         self.rope_sin = torch.zeros(MP, c.rope_dims // 2, dtype=f32, device=dev)
-        aws = self.lib.dtree_attention_workspace_bytes(c.num_attention_heads, c.head_dim, self.max_past, self.MP)
-        self.attn_ws = torch.zeros(aws, dtype=torch.uint8, device=dev)
+        self.attn_ws = self._tree_attention_workspace()
 
     def _gemm_shapes(self):
         c = self.cfg
@@ -263,9 +262,10 @@ class Qwen35TreeEngine(TreeEngineBase):
                   act=torch.zeros(2, rows, F, dtype=self.act_dtype, device=dev),
                   hidden=torch.zeros(rows, nh * H, dtype=bf16, device=dev),
                   cos=torch.zeros(rows, c.rope_dims // 2, dtype=f32, device=dev),
-                  sin=torch.zeros(rows, c.rope_dims // 2, dtype=f32, device=dev),
-                  attn_ws=torch.empty(self.lib.dtree_causal_attention_workspace_bytes(c.head_dim), dtype=torch.uint8,
-                                      device=dev))
+                  sin=torch.zeros(rows, c.rope_dims // 2, dtype=f32, device=dev))
+        if self.kv_bits != 8:
+            pf["attn_ws"] = torch.empty(self.lib.dtree_causal_attention_workspace_bytes(c.head_dim), dtype=torch.uint8,
+                                        device=dev)
         self._pf = pf
         return pf
 

@@ -75,3 +75,14 @@ def test_attention_without_a_cache_write_is_refused_in_8_bits(gpu_device, family
         eng._attention(li, cache, eng.stream_handle(), write_cache=False)
     torch.cuda.synchronize()
     assert not kv.k_pages.any() and not kv.k_scales.any()
+
+
+@pytest.mark.parametrize("family", ["qwen3", "qwen35"])
+def test_an_8_bit_engine_holds_no_bf16_attention_workspace(gpu_device, family):
+    eng = _engine(gpu_device, family, 8, max_past=300)
+    assert eng.attn_ws is None
+    cache = eng.new_cache()
+    eng.prefill_long(cache, random_prefix(140, eng.cfg.vocab_size, seed=6))
+    assert "attn_ws" not in eng._pf
+    eng.verify(cache, [5, 6], [140, 141], [-1, 0])
+    assert _engine(gpu_device, family, 16, max_past=300).attn_ws.numel() > 0
