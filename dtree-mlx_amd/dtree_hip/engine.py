@@ -466,8 +466,8 @@ class TreeEngineBase:
         if self.kv_bits == 8 and kv.num_seqs != 1:
             raise ValueError("the engines verify one sequence: the cache must have num_seqs 1")
 
-    def _attention_q8(self, lw, kv: PagedKVCacheQ8, rec: N.KvQ8, a: N.AttnQ8Args, qkv: torch.Tensor, ws: torch.Tensor,
-                      st: int) -> None:
+    def _attention_q8(self, lw, kv: PagedKVCacheQ8, rec: N.KvQ8, a: N.AttnQ8Args, qkv: torch.Tensor,
+                      ws: torch.Tensor | None, st: int) -> None:
         """Append the rows' K / V, then attend (qkv rows are [q heads | k heads | v heads])."""
         c = self.cfg
         k = qkv.data_ptr() + 4 * c.num_attention_heads * a.q_stride
@@ -475,7 +475,8 @@ class TreeEngineBase:
         N.check(self.lib.dtree_kv_q8_append(
             C.byref(rec), k, k + 4 * c.num_key_value_heads * c.head_dim, N.T_F32, ld, ld, lw.k_norm.data_ptr(),
             c.rms_norm_eps, a.rope_cos, a.rope_sin, a.rope_dims, st), "kv append")
-        a.workspace = ws.data_ptr(); a.workspace_bytes = ws.numel()
+        if ws is not None:
+            a.workspace = ws.data_ptr(); a.workspace_bytes = ws.numel()
         N.check(self.lib.dtree_attention_q8(C.byref(rec), C.byref(a), st), "8-bit attention")
 
     def _tree_attention_q8(self, lw, kv: PagedKVCacheQ8, layer: int, st: int, write_cache: bool = True) -> None:
@@ -490,6 +491,30 @@ class TreeEngineBase:
         a.ancestors = d + N.StepDesc.ancestors.offset
         self._attention_q8(lw, kv, rec, a, self.qkv, self.q8_ws, st)
 
+    def _prefill_workspace_q8(self, kv: PagedKVCacheQ8, past: int, tokens: int, seg: int) -> None:
+        """Room for the key ranges of all of a prompt's segments, before its first
+        row is written (a longer prefix may want more of it). Where the device has
+        none, the attention runs in one range, which is slower and needs none."""
+        if self.kv_bits != 8:
+            return
+        a = N.AttnQ8Args()
+        a.num_heads = self.cfg.num_attention_heads
+        need = 0
+        for s0 in range(0, tokens, seg):
+            n = min(seg, tokens - s0)
+            a.rows_padded = 128 * ((n + 127) // 128)
+            rec = kv.record(0, None, None, past + s0, n, a.rows_padded)
+            need = max(need, self.lib.dtree_attention_q8_workspace_bytes(C.byref(rec), C.byref(a)))
+        pf = self._pf
+        ws = pf.get("q8_ws")
+        if need > (0 if ws is None else ws.numel()):
+            ws = pf["q8_ws"] = None  # release the smaller one first
+            try:
+                ws = torch.empty(need, dtype=torch.uint8, device=self.dev)
+            except torch.cuda.OutOfMemoryError:
+                pass
+        pf["q8_ws"] = ws
+
     def _prefill_lengths_q8(self, pf: dict, P0: int, n: int) -> None:
         """A prompt segment's past length and row count, on the device."""
         if self.kv_bits == 8:
@@ -500,11 +525,7 @@ class TreeEngineBase:
         at = pf["q8_lengths"]
         rec = kv.record(layer, at.data_ptr(), at.data_ptr() + 4, P0, n, rows)
         a = self._q8_args(lw, pf["qkv"], pf["cos"], pf["sin"], pf["attn"], rows)
-        need = self.lib.dtree_attention_q8_workspace_bytes(C.byref(rec), C.byref(a))
-        ws = pf.get("q8_ws")
-        if ws is None or ws.numel() < need:
-            ws = pf["q8_ws"] = torch.empty(max(need, 16), dtype=torch.uint8, device=self.dev)
-        self._attention_q8(lw, kv, rec, a, pf["qkv"], ws, st)
+        self._attention_q8(lw, kv, rec, a, pf["qkv"], pf["q8_ws"], st)
 
     def _launch_kv_compact(self, kv, layers: int, desc: torch.Tensor, select_hidden: bool, st: int) -> None:
         """dtree_compact, or its 8-bit form, over the model's layers of the cache."""
@@ -890,6 +911,7 @@ class Qwen3TreeEngine(TreeEngineBase):
         slot = {li: i for i, li in enumerate(self.layer_ids)}
         hid_parts = []
         seg = self._prefill_segment(len(toks))
+        self._prefill_workspace_q8(cache, cache.offset, len(toks), seg)
         for s0 in range(0, len(toks), seg):
             part = toks[s0:s0 + seg]
             n = len(part)

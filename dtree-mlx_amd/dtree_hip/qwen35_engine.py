@@ -317,6 +317,7 @@ class Qwen35TreeEngine(TreeEngineBase):
         hid_parts = []
         seg = self._prefill_segment(len(toks))
         kv = cache.kv
+        self._prefill_workspace_q8(kv, cache.offset, len(toks), seg)
         for s0 in range(0, len(toks), seg):
             part = toks[s0:s0 + seg]
             n = len(part)

@@ -8,6 +8,7 @@ from dtree_hip.cache import PagedKVCache
 from dtree_hip.synthetic import random_prefix
 
 pytestmark = pytest.mark.gpu
+TOL = 2e-2  # of the row maximum, as the engines' other tests grant
 
 
 def _engine(dev, family, kv_bits, **kw):
@@ -75,6 +76,59 @@ def test_attention_without_a_cache_write_is_refused_in_8_bits(gpu_device, family
         eng._attention(li, cache, eng.stream_handle(), write_cache=False)
     torch.cuda.synchronize()
     assert not kv.k_pages.any() and not kv.k_scales.any()
+
+
+@pytest.mark.parametrize("family", ["qwen3", "qwen35"])
+def test_a_prompt_allocates_its_8_bit_workspace_before_its_first_row(gpu_device, monkeypatch, family):
+    """Segments over a growing prefix want more of it: had before the first of them."""
+    eng = _engine(gpu_device, family, 8, max_past=1400)
+    eng.PREFILL_SEGMENT = 128
+    toks = random_prefix(1300, eng.cfg.vocab_size, seed=5)
+    empty, attention, inside = torch.empty, eng._prefill_attention_q8, [False]
+
+    def guarded(*a, **kw):
+        if inside[0]:
+            raise torch.cuda.OutOfMemoryError("no room")
+        return empty(*a, **kw)
+
+    def layer(*a, **kw):
+        inside[0] = True
+        try:
+            return attention(*a, **kw)
+        finally:
+            inside[0] = False
+
+    monkeypatch.setattr(torch, "empty", guarded)
+    monkeypatch.setattr(eng, "_prefill_attention_q8", layer)
+    cache = eng.new_cache()
+    eng.prefill_long(cache, toks)
+    torch.cuda.synchronize()
+    assert cache.offset == 1300 and eng._pf["q8_ws"].numel() > 16
+
+
+@pytest.mark.parametrize("family", ["qwen3", "qwen35"])
+def test_a_prompt_runs_without_room_for_its_8_bit_workspace(gpu_device, monkeypatch, family):
+    """Fewer key ranges, the same answer."""
+    logits = []
+    for full in (False, True):
+        eng = _engine(gpu_device, family, 8, max_past=1400)
+        toks = random_prefix(1300, eng.cfg.vocab_size, seed=5)
+        cache = eng.new_cache()
+        eng.prefill_long(cache, toks[:1100])
+        eng._pf = None
+        empty = torch.empty
+
+        def short(*a, **kw):
+            if kw.get("dtype") == torch.uint8:
+                raise torch.cuda.OutOfMemoryError("no room")
+            return empty(*a, **kw)
+
+        with monkeypatch.context() as m:
+            if full:
+                m.setattr(torch, "empty", short)
+            logits.append(eng.prefill_long(cache, toks[1100:])[0][0, 0].clone())
+        assert cache.offset == 1300 and (eng._pf["q8_ws"] is None) == full
+    assert float((logits[0] - logits[1]).abs().max()) <= TOL * float(logits[0].abs().max())
 
 
 @pytest.mark.parametrize("family", ["qwen3", "qwen35"])
