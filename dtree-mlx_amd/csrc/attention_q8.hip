@@ -1230,8 +1230,9 @@ extern "C" int dtree_attention_q8(const DtreeKvQ8* kv, const DtreeAttnQ8Args* a,
   if (p.h16) p.a.out_lo = nullptr;
   p.plain = !tiled && !p.a.out_lo && !a->gated && ((uintptr_t)a->out & 15) == 0 && a->ld_out % 8 == 0;
   const int64_t grid = (int64_t)kv->num_seqs * pl.blocks * pl.parts * kv->num_kv_heads;
-  DTREE_REQUIRE(grid < (int64_t)1 << 31 && (int64_t)kv->max_rows * a->num_heads < (int64_t)1 << 31 &&
-                    (pl.parts == 1 || kv->num_seqs <= 65535),
+  // (a launch counts its work items in 32 bits; the join has 256 for up to one (row, head))
+  DTREE_REQUIRE(64 * pl.waves * grid < (int64_t)1 << 32 && (int64_t)kv->max_rows * a->num_heads < (int64_t)1 << 31 &&
+                    (pl.parts == 1 || (kv->num_seqs <= 65535 && kv->max_rows * (int64_t)a->num_heads < 1 << 24)),
                 "attention_q8: num_seqs * max_rows too large for one launch");
   if (D == 64) return launch<64>(p, pl, (unsigned)grid, stream);
   if (D == 128) return launch<128>(p, pl, (unsigned)grid, stream);

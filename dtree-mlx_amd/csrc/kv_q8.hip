@@ -429,7 +429,7 @@ static int row_buffer_check(const DtreeKvQ8* kv, const void* p, int ld, int type
 
 static int grid_of(const DtreeKvQ8* kv, const std::string& what, unsigned* grid) {
   const int64_t n = (int64_t)kv->num_seqs * span_halves(*kv) * kv->num_kv_heads;
-  DTREE_REQUIRE(n < (int64_t)1 << 31, what + ": num_seqs * max_rows too large for one launch");
+  DTREE_REQUIRE(256 * n < (int64_t)1 << 32, what + ": num_seqs * max_rows too large for one launch");  // work items
   *grid = (unsigned)n;
   return DTREE_OK;
 }

@@ -596,7 +596,8 @@ int dtree_gdn_layer_chain(const DtreeGdnArgs* args, int32_t num_tokens, hipStrea
  * masked, it reads as zeros), so pages that a window has passed can be given
  * away (-1). Sequences may share pages
  * that no call writes. Rows of the buffers that belong to no sequence are
- * neither read nor written.
+ * neither read nor written. A batch whose launch would have 2^32 work items or
+ * more (2^24 workgroups of 256: half pages by kv heads here) is refused.
  */
 #define DTREE_T_F32 0   /* element types of row buffers */
 #define DTREE_T_BF16 1

@@ -1,10 +1,15 @@
-"""Rules of the 8-bit cache that ordinary random rows do not meet, on the host.
-CPU only."""
+"""The 8-bit cache's rounding rule and the bounds its records are held to, on
+the host. CPU only."""
+import ctypes as C
+
 import pytest
 import torch
 
+from dtree_hip import _native as N
 from dtree_hip import tiny_qwen35
 from dtree_hip.cache import PagedKVCache, PagedKVCacheQ8, Qwen35Cache, quantise_q8
+
+from test_kv_q8_abi import attn, cache, refused
 
 
 def tie_rows(dim, scales, seed=0):
@@ -44,3 +49,18 @@ def test_hybrid_cache_refuses_other_widths(bits):
 def test_hybrid_cache_of_either_width():
     assert type(Qwen35Cache(tiny_qwen35(), 64, device="cpu").kv) is PagedKVCache
     assert type(Qwen35Cache(tiny_qwen35(), 64, device="cpu", kv_bits=8).kv) is PagedKVCacheQ8
+
+
+# Work items of a launch are counted in 32 bits: 2^24 workgroups of 256 threads are one too many.
+WIDE = dict(num_kv_heads=256, num_seqs=65536, max_rows=1, total_rows=65536, max_past_length=0, ld_page_table=1)
+
+
+def test_launches_of_2_to_the_32_threads_are_refused():
+    lib = N.lib()
+    r = cache(**WIDE)
+    width = 256 * 128
+    refused(lib.dtree_kv_q8_append(C.byref(r), 4096, 4096, N.T_F32, width, width, None, 0.0, None, None, 0, None),
+            "too large")
+    refused(lib.dtree_kv_q8_read(C.byref(r), 4096, 4096, N.T_F32, width, width, None), "too large")
+    a = attn(num_heads=256, ld_q=width, ld_out=width)
+    refused(lib.dtree_attention_q8(C.byref(r), C.byref(a), None), "too large")
