@@ -21,7 +21,8 @@
 //
 // Two kernels. Up to 32 pairs of a sequence and KV head (decoded tokens; 16 with
 // 256 dims) are bound by the pages' bytes or, for short prefixes, by latency: the
-// token kernel, pages straight to registers. More pairs are bound by issue: the
+// token kernel, pages straight to registers. More pairs are bound by the matrix and
+// vector units together (neither alone is busy for more than 56 % of the time): the
 // rows kernel, a page converted once for 128 or 256 pairs through LDS. Both split
 // the keys into ranges where sequences are too few to fill the card, and a third
 // joins them.
@@ -385,10 +386,11 @@ __device__ __forceinline__ f32x4_t mfma16_f16(u32x4_t a, u32x4_t b, f32x4_t c) {
 // * V's lane (dim % 16, kq) reads its 16 keys of one dim as they lie, i = 2 step,
 //   2 step + 1, and P needs no exchange.
 //
-// Measured (8 KV heads of 128, 4 query heads each): one token over 65536 keys 28.0
-// us, 138 MB at 4.9 TB/s, as a copy; 32 tokens over up to 8193 keys 26.9 us, 100 MB;
-// one over 1001 keys 10 us, all latency: lengths, page ids, the first page with the
-// query rows, 3 pages a wave, the merge.
+// Measured (8 KV heads of 128, 4 query heads each): one token over 65536 keys 27.7
+// us, 138 MB at 5.0 TB/s, as a copy; 32 tokens over up to 8193 keys 27.1 us, 100 MB
+// at 3.7 TB/s (half of them hold under 200 keys, a few long ones' ranges are what is
+// left at the end); one over 1001 keys 10 us, all latency: lengths, page ids, the
+// first page with the query rows, 3 pages a wave, the merge.
 template <int D, int NC, int W>
 __global__ __launch_bounds__(64 * W, 8 / W) void q8_token_kernel(AttnQ8Params p) {
   constexpr int NJ = D / 64, NK = 4 * NJ, ND = D / 16;  // K loads (block, 64 dims) and V loads (16 dims) per page
@@ -648,8 +650,9 @@ __global__ __launch_bounds__(64 * W, 8 / W) void q8_token_kernel(AttnQ8Params p)
 // was busy for half the time. Two waves a SIMD: one of 64 pairs, with half the LDS
 // reads, took 8 % longer, since a wave alone issues one instruction at a time.
 //
-// Measured: 4096 rows, 32 heads of 128 on 8: 167 to 172 us, 0.8 PFLOP/s (a large library
-// product 1.2), MFMA busy 41 %, VALU 54 %, LDS 43 % of the time; 1000 gated rows after
+// Measured: 4096 rows, 32 heads of 128 on 8: 165 to 173 us, 0.8 PFLOP/s (a large library
+// product 1.2), MFMA busy 42 %, VALU 56 %, LDS 44 % of the time, waves waiting 31 %:
+// no unit is full, and what the waits are for was not found. 1000 gated rows after
 // 8192 keys, 16 heads of 256, one wave a SIMD: 186 us without the join, 0.76 PFLOP/s.
 template <int D, int W>
 __global__ __launch_bounds__(64 * W, D <= 128 ? 8 / W : 1) void q8_rows_kernel(AttnQ8Params p) {
@@ -974,9 +977,10 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 8 / W : 1) void q8_rows_kernel(A
   }
 }
 
-// Adds the ranges' partial results (4 to 5 us for a few tokens, latency; 1000 rows
-// of 16 heads of 256 in two ranges 12 us, 41 MB): D / 4 threads for a pair's dims, NG groups of
-// them take its ranges in turn (many ranges of few pairs), and meet in LDS.
+// Adds the ranges' partial results (4 to 5 us for a few tokens, latency; 1000 gated
+// rows of 16 heads of 256 in two ranges 12.5 us, 58 MB at 4.6 TB/s: 33 of partials and
+// 16 of gate logits in, 8 out): D / 4 threads for a pair's dims, NG groups of them
+// take its ranges in turn (many ranges of few pairs), and meet in LDS.
 template <int D, bool TOKENS, int NG>
 __global__ __launch_bounds__(256) void q8_join_kernel(AttnQ8Params p) {
   constexpr int TPP = D / 4, PPB = 256 / TPP / NG;  // pairs of a workgroup
@@ -1071,9 +1075,12 @@ size_t part_bytes(const DtreeKvQ8& kv, const DtreeAttnQ8Args& a) {
 // More are cut so that the ranges are as many as the CUs hold at once, two
 // workgroups each, if all sequences are as long as the longest (1 x 1025 pages:
 // 32.9 us with 16 pages a range, 36.8 with 8; 1 x 125: 13.0 with 8, 16.3 with 32),
-// but not longer than kRagged where sequences differ, whose short ones leave their
-// ranges empty (32 of up to 129 pages: 30.8 us, with 16 a range 31.2, with 8 32.1; 64
-// of up to 32: 19.9, 23.5, 32.0), and no more of them than kMost. Rows: as many workgroups as the CUs hold.
+// but not longer than kRagged in a batch, where sequences may differ (the host knows
+// bounds alone) and short ones leave their ranges empty (32 of up to 129 pages: 30.8
+// us, with 16 a range 31.2, with 8 32.1; 64 of up to 32: 19.9, 23.5, 32.0), and no
+// more of them than kMost. Rows: as many workgroups as the CUs hold, each sequence
+// counted with max_rows rows: a single token beside a chunk has the chunk's ranges
+// (one over 65536 keys beside 1000 rows: 1.8 ms, the two in calls of their own 92 us).
 constexpr int kOneRange = 24, kMinTokens = 8, kRagged = 12, kMost = 4096, kResident = 512;
 // A row block's few pages are one range (4 pages, 128 dims: 14.6 us, in two 15.3;
 // 256 dims, with twice the work a page: 3 pages in two 23.3, in one 29.8). More are

@@ -3,19 +3,21 @@
 // (adapters.py:635-668).
 //
 // A row is quantised as scale = fp32(max |x| / 127), q = nearest integer of
-// x / scale. Everything before the rounding to q is fp64: x stays within 1e-15
-// of its value, so q is the nearest integer but for borders met by less than
-// that, and two programs that follow the definition store the same bytes.
+// x / scale, ties to even. Everything before the rounding to q is fp64: V rows and
+// K rows without norm and rotation give the definition's bytes exactly, others x
+// within 1e-15 of its value, so that q differs only at borders met by less.
 //
-// All three are bound by the bytes they move (a decode step's by the launch). A
+// Long runs are bound by the bytes they move, a single row by latency. A
 // workgroup owns half a page (32 positions, whole 16-byte pieces of K and of V) of
 // one kv head. The rows' side is read and written in runs of their dims, the
 // pages' side in runs of their pieces, and LDS, rows of bytes, lies between (without
 // it, V's bytes one by one, 4000 rows in and out took 43 us, now 23).
-// Measured, 8 heads of 128: 4000 fp32 rows in 14.4 us (58 MB moved, 4.0 TB/s; the
-// fp64 arithmetic takes 54 % of the issue) and back in 9.4 us (4.4 TB/s); 4 x 8192
-// rows of 256 dims to bf16 28.2 us (120 MB, 4.3 TB/s, of 4.8 that a copy reaches);
-// one row 6.0 us.
+// Measured, 8 heads of 128: 4000 fp32 rows in 13.4 to 15 us (58 MB moved; waves wait
+// 61 % of the time, the fp64 arithmetic takes 54 % of the issue), bf16 rows 12.4, and
+// back in 9.3 us (4.4 TB/s); 4 x 8192 rows of 256 dims to bf16 28.1 us (120 MB, 4.3
+// TB/s, of 4.8 that a copy reaches). Of the 49 MB that the append reads 35 are
+// needed: with 8 heads each is on an XCD of its own, and each reads the rows'
+// rotations. One row: append 6.0 us, read 3.2, the fp64 chain's latency between them.
 #include <cmath>
 #include <type_traits>
 
@@ -329,7 +331,8 @@ constexpr int kHidBlocks = 16;  // workgroups of the hidden rows' select
 
 // The accepted rows of one (layer, kv head), K or V, through LDS: a row's place
 // may be another accepted row's source. At most 128 rows: bound by latency, hence
-// a workgroup for each, and V's bytes one by one.
+// a workgroup for each, and V's bytes one by one (5 rows of 36 layers of 8 heads of
+// 128: 7.5 us).
 __global__ __launch_bounds__(256) void q8_compact_kernel(const DtreeStepDesc* desc, int8_t* kp, int8_t* vp, float* ks,
                                                          float* vs, int layers, int num_pages, int Hkv, int D,
                                                          const int32_t* page_table, int table_pages,

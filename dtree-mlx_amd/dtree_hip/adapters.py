@@ -479,7 +479,8 @@ def load_target_model(spec: str | Qwen3Config | Qwen35Config = "random:qwen3-4b"
     """Random-init target (no checkpoint download: weights ~ N(0, 0.02), seeded).
     ``spec`` is "random:qwen3-4b", "random:qwen35-4b" or a Qwen3Config /
     Qwen35Config (adapters.py:822-846 resolves a model name instead). ``kv_bits`` 8
-    keeps the KV cache in 8 bits (PagedKVCacheQ8)."""
+    keeps the KV cache in 8 bits (PagedKVCacheQ8); its attention rounds queries and
+    softmax weights to fp16, where the bf16 cache's holds both as split pairs."""
     if isinstance(spec, (Qwen3Config, Qwen35Config)):
         cfg, name = spec, "random:custom"
     elif spec in ("random:qwen3-4b", "qwen3-4b"):

@@ -313,7 +313,8 @@ class Qwen35Cache:
     ``flip()`` makes the spare the committed state. A verify step that is not
     kept (``commit=False``) therefore leaves the state it started from
     untouched and can be replayed as it is. ``kv_bits`` 8 holds the attention
-    layers' keys and values in 8 bits."""
+    layers' keys and values in 8 bits, and their attention rounds queries and
+    softmax weights to fp16."""
 
     def __init__(self, cfg, capacity: int, device="cuda", page_order: torch.Tensor | None = None, kv_bits: int = 16):
         if kv_bits not in (8, 16):

@@ -422,7 +422,8 @@ class TreeEngineBase:
     # ---- 8-bit KV cache (kv_bits = 8) --------------------------------------------
     # The tree step and the prefill append their rows to the 8-bit cache and attend
     # over it: dtree_kv_q8_append + dtree_attention_q8 in place of one
-    # dtree_tree_attention / dtree_causal_attention.
+    # dtree_tree_attention / dtree_causal_attention. Queries and softmax weights are
+    # rounded to fp16 there (split bf16 pairs here).
     def _new_kv_cache(self, layers: int, capacity: int, page_order=None):
         c = self.cfg
         cls = PagedKVCacheQ8 if self.kv_bits == 8 else PagedKVCache
