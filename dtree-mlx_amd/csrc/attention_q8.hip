@@ -16,7 +16,8 @@
 // the largest weight times value scale of the row inside fp16's normal range
 // whatever the scales are. q is moved by a power of two per workgroup, into the
 // upper part of fp16's range, and taken back in ks; pairs of a workgroup too far
-// apart for that by one of their own each, taken back in raw.
+// apart for that by one of their own each, taken back in the pair's ks (raw alone
+// is larger than the logit, by up to 127 / max |k|).
 // A masked key's t is -inf, whatever its scales and bytes are (u = 0 exactly).
 //
 // Two kernels. Up to 32 pairs of a sequence and KV head (decoded tokens; 16 with
@@ -540,7 +541,7 @@ __global__ __launch_bounds__(64 * W, 8 / W) void q8_token_kernel(AttnQ8Params p)
           const f32x4_t ks = *reinterpret_cast<const f32x4_t*>(sc + kkey + 8 * b);
           const f32x4_t lv = *reinterpret_cast<const f32x4_t*>(sc + 64 + kkey + 8 * b);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) st[n][b][e] = fmaf(st[n][b][e] * own[n], ks[e], lv[e]);
+          for (int e = 0; e < 4; ++e) st[n][b][e] = fmaf(st[n][b][e], ks[e] * own[n], lv[e]);
         }
         if (masked) {
           const uint32_t sees = q8_sees(p, q, pos[n], k0 + (kkey & 32), anc[16 * n + c]) >> (kkey & 31);
@@ -867,7 +868,7 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 8 / W : 1) void q8_rows_kernel(A
     asm volatile("" : "+v"(ph[0]), "+v"(l));  // taken here, not sunk to their use
     if (wide) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) next[r] *= own;
+      for (int i = 0; i < 4; ++i) ks[i] *= own;
     }
   };
   auto hidden = [&](int k0) {  // does a page hold keys that some row may not see

@@ -51,3 +51,39 @@ def test_a_query_far_larger_than_its_neighbours(gpu_device, heads, past, rows, w
         b.qkv[5, 0] = float("inf")
     want, tol = b.reference()
     check(b.attend(pair=True, workspace=workspace), want, tol, PAIR)
+
+
+@pytest.mark.parametrize("heads", ["128", "256g", "64"])
+@pytest.mark.parametrize("rows", [1, 60])
+def test_a_query_near_the_end_of_fp32(gpu_device, heads, rows):
+    """Its logits are finite, its products with the cached integers are not: those are
+    larger by 127 / max |k|. Beside ordinary queries, and all of them so."""
+    for all_of_them in (False, True):
+        b = Batch(gpu_device, heads, [300], [rows], seed=42, norm=False)
+        b.append()
+        for h in range(b.hq if all_of_them else 1):
+            at = ((h + 1) % b.hq) * (2 * b.d if b.gated else b.d)
+            b.qkv[(slice(None) if all_of_them else rows // 2), at:at + b.d] *= 2e37
+        want, tol = b.reference()
+        check(b.attend(pair=True), want, tol, PAIR, all_of_them)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_rows_whose_scale_is_subnormal(gpu_device, d):
+    """Multiples of fp32's smallest number, ties among them."""
+    dev, unit = gpu_device, 2.0 ** -149
+    scales = [2 * unit, 6 * unit, 98 * unit, 65534 * unit]
+    x, q = tie_rows(d, scales, seed=9)
+    rows = torch.cat([x, x], 1).to(dev).contiguous()
+    c = PagedKVCacheQ8(1, 1, d, len(scales), device=dev)
+    past, count = i32([0], dev), i32([len(scales)], dev)
+    rec = c.record(0, past, count, 0, len(scales), len(scales))
+    N.check(N.lib().dtree_kv_q8_append(C.byref(rec), rows.data_ptr(), rows.data_ptr() + 4 * d, N.T_F32, 2 * d, 2 * d, None,
+                                       0.0, None, None, 0, stream()), "append")
+    at = [_block_index_q8(d, which)[:len(scales)].to(dev) for which in "kv"]
+    for pages, s, i in ((c.k_pages, c.k_scales, at[0]), (c.v_pages, c.v_scales, at[1])):
+        assert torch.equal(s[0, 0, 0, :len(scales)].cpu().double(), torch.tensor(scales, dtype=torch.float64))
+        assert torch.equal(pages[0, 0, 0][i].cpu().long(), q)
+    k = torch.zeros(len(scales), d, device=dev)
+    N.check(N.lib().dtree_kv_q8_read(C.byref(rec), k.data_ptr(), None, N.T_F32, d, 0, stream()), "read")
+    assert torch.equal(k.cpu().double(), q.double() * torch.tensor(scales, dtype=torch.float64)[:, None])
