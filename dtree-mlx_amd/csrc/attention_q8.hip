@@ -230,32 +230,53 @@ __device__ __forceinline__ float q8_queries_of(const AttnQ8Params& p, const Q8Se
     bound *= unit;
   }
   q8_exponent(bound, f, inv);
+  auto load_all = [&](u32x4_t (&x)[2], f32x4_t& cs, f32x4_t& sn) {
+    size_t row;
+    const char* base;
+    load(x[0], x[1], row, base);
+    const size_t at = 4 * (row * half + (pc.turns ? 4 * j : 0));
+    const char* tc = half ? reinterpret_cast<const char*>(p.a.rope_cos) + at : base;
+    const char* ts = half ? reinterpret_cast<const char*>(p.a.rope_sin) + at : base;
+    __builtin_memcpy(&cs, tc, 16);
+    __builtin_memcpy(&sn, ts, 16);
+  };
+  // The pair of round k, rotated, times rs, to LDS.
+  auto put = [&](int k, f32x4_t x0, f32x4_t x1, f32x4_t cs, f32x4_t sn, float rs) {
+    f32x4_t y, z;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float a = x0[e] * w0[e], b = x1[e] * w1[e];
+      // (a select, not sn = 0, which would carry an infinity to another dim)
+      y[e] = (pc.turns ? a * cs[e] - b * sn[e] : a) * rs;
+      z[e] = (pc.turns ? a * sn[e] + b * cs[e] : b) * rs;
+    }
+    const int pl = tid / TPR + k * PPR;
+    if (PAIRS % PPR == 0 || pl < PAIRS) {
+      *reinterpret_cast<u32x2_t*>(qs + pl * (D + 8) + pc.at[0]) = u32x2_t{pack_h2(y[0], y[1]), pack_h2(y[2], y[3])};
+      *reinterpret_cast<u32x2_t*>(qs + pl * (D + 8) + pc.at[1]) = u32x2_t{pack_h2(z[0], z[1]), pack_h2(z[2], z[3])};
+    }
+  };
+  if (wide) {  // (rare: one round at a time, little code)
+#pragma unroll 1
+    for (int k = 0; k < rounds; ++k) {
+      u32x4_t x[2];
+      f32x4_t cs, sn;
+      load_all(x, cs, sn);
+      const f32x4_t x0 = value(x[0]), x1 = value(x[1]);
+      q8_exponent(q8_max_lanes<TPR>(largest(x0, x1)) * unit, f, inv);
+      put(k, x0, x1, cs, sn, f);
+      const int pl = tid / TPR + k * PPR;
+      if (j == 0 && (PAIRS % PPR == 0 || pl < PAIRS)) *reinterpret_cast<float*>(qs + pl * (D + 8) + D) = inv;
+    }
+    lds_barrier();
+    return 1.f;
+  }
 #pragma unroll 1
   for (int k0 = 0; k0 < rounds; k0 += BR) {
     u32x4_t x[BR][2];
     f32x4_t cs[BR], sn[BR];
-    float fk[BR];
 #pragma unroll
-    for (int k = 0; k < BR; ++k) {
-      size_t row;
-      const char* base;
-      load(x[k][0], x[k][1], row, base);
-      const size_t at = 4 * (row * half + (pc.turns ? 4 * j : 0));
-      const char* tc = half ? reinterpret_cast<const char*>(p.a.rope_cos) + at : base;
-      const char* ts = half ? reinterpret_cast<const char*>(p.a.rope_sin) + at : base;
-      __builtin_memcpy(&cs[k], tc, 16);
-      __builtin_memcpy(&sn[k], ts, 16);
-      fk[k] = f;
-    }
-    if (wide) {
-#pragma unroll
-      for (int k = 0; k < BR; ++k) {
-        const int pl = tid / TPR + (k0 + k) * PPR;
-        float back;
-        q8_exponent(q8_max_lanes<TPR>(largest(value(x[k][0]), value(x[k][1]))) * unit, fk[k], back);
-        if (j == 0 && (PAIRS % PPR == 0 || pl < PAIRS)) *reinterpret_cast<float*>(qs + pl * (D + 8) + D) = back;
-      }
-    }
+    for (int k = 0; k < BR; ++k) load_all(x[k], cs[k], sn[k]);
 #pragma unroll
     for (int k = 0; k < BR; ++k) {
       const f32x4_t x0 = value(x[k][0]), x1 = value(x[k][1]);
@@ -267,24 +288,12 @@ __device__ __forceinline__ float q8_queries_of(const AttnQ8Params& p, const Q8Se
       ss += dpp<0x141>(ss);
       if constexpr (TPR >= 16) ss += dpp<0x140>(ss);
       if constexpr (TPR >= 32) ss += swz_xor16(ss);
-      const float rs = norm ? f * __builtin_amdgcn_rsqf(ss * (1.0f / D) + p.a.eps) : fk[k];  // (1 ulp; fp16 follows)
-      f32x4_t y, z;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float a = x0[e] * w0[e], b = x1[e] * w1[e];
-        // (a select, not sn = 0, which would carry an infinity to another dim)
-        y[e] = (pc.turns ? a * cs[k][e] - b * sn[k][e] : a) * rs;
-        z[e] = (pc.turns ? a * sn[k][e] + b * cs[k][e] : b) * rs;
-      }
-      const int pl = tid / TPR + (k0 + k) * PPR;
-      if (PAIRS % PPR == 0 || pl < PAIRS) {
-        *reinterpret_cast<u32x2_t*>(qs + pl * (D + 8) + pc.at[0]) = u32x2_t{pack_h2(y[0], y[1]), pack_h2(y[2], y[3])};
-        *reinterpret_cast<u32x2_t*>(qs + pl * (D + 8) + pc.at[1]) = u32x2_t{pack_h2(z[0], z[1]), pack_h2(z[2], z[3])};
-      }
+      const float rs = norm ? f * __builtin_amdgcn_rsqf(ss * (1.0f / D) + p.a.eps) : f;  // (1 ulp; fp16 follows)
+      put(k0 + k, x0, x1, cs[k], sn[k], rs);
     }
   }
   lds_barrier();
-  return wide ? 1.f : inv;
+  return inv;
 }
 template <int D, int PAIRS, int W>
 __device__ __forceinline__ float q8_queries(const AttnQ8Params& p, const Q8Seq& q, int g, int pair0, int pairs,
