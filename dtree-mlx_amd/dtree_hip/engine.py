@@ -526,7 +526,7 @@ class TreeEngineBase:
         at = pf["q8_lengths"]
         rec = kv.record(layer, at.data_ptr(), at.data_ptr() + 4, P0, n, rows)
         a = self._q8_args(lw, pf["qkv"], pf["cos"], pf["sin"], pf["attn"], rows)
-        self._attention_q8(lw, kv, rec, a, pf["qkv"], pf["q8_ws"], st)
+        self._attention_q8(lw, kv, rec, a, pf["qkv"], pf.get("q8_ws"), st)  # (buffers made anew hold none)
 
     def _launch_kv_compact(self, kv, layers: int, desc: torch.Tensor, select_hidden: bool, st: int) -> None:
         """dtree_compact, or its 8-bit form, over the model's layers of the cache."""

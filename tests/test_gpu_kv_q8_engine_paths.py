@@ -140,3 +140,17 @@ def test_an_8_bit_engine_holds_no_bf16_attention_workspace(gpu_device, family):
     assert "attn_ws" not in eng._pf
     eng.verify(cache, [5, 6], [140, 141], [-1, 0])
     assert _engine(gpu_device, family, 16, max_past=300).attn_ws.numel() > 0
+
+
+@pytest.mark.parametrize("family", ["qwen3", "qwen35"])
+@pytest.mark.parametrize("kv_bits", [8, 16])
+def test_a_prompt_in_segments_of_any_length(gpu_device, family, kv_bits):
+    """Buffers that grow between a prompt's segments: the same logits."""
+    logits = []
+    for segment in (1024, 200):
+        eng = _engine(gpu_device, family, kv_bits, max_past=700)
+        eng.PREFILL_SEGMENT = segment
+        cache = eng.new_cache()
+        logits.append(eng.prefill_long(cache, random_prefix(600, eng.cfg.vocab_size, seed=8))[0][0, 0].clone())
+        assert cache.offset == 600
+    assert float((logits[0] - logits[1]).abs().max()) <= TOL * float(logits[0].abs().max())
