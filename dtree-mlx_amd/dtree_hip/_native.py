@@ -16,7 +16,7 @@ LIB_PATH = Path(__file__).resolve().parent / "libdtree_hip.so"
 MAX_NODES = 128
 MASK_WORDS = 4
 PAGE = 64
-ABI_VERSION = 8
+ABI_VERSION = 9
 
 E_OK, E_ARG, E_HIP, E_TREE, E_WORKSPACE = 0, -1, -2, -3, -4
 
@@ -135,6 +135,35 @@ class AttnQ8Args(C.Structure):
     ]
 
 
+class BeamArgs(C.Structure):
+    _fields_ = [
+        ("logits", C.c_void_p), ("type", C.c_int32), ("ld_logits", C.c_int32),
+        ("vocab", C.c_int32), ("groups", C.c_int32), ("beams", C.c_int32), ("num_select", C.c_int32),
+        ("scores", C.c_void_p), ("lengths", C.c_void_p), ("finished", C.c_void_p),
+        ("eos_token", C.c_int32), ("pad_token", C.c_int32), ("length_penalty", C.c_float),
+        ("scores_out", C.c_void_p), ("tokens_out", C.c_void_p), ("parents_out", C.c_void_p),
+        ("lengths_out", C.c_void_p), ("finished_out", C.c_void_p), ("sources_out", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
+class PagesFork(C.Structure):
+    _fields_ = [
+        ("refs", C.c_void_p), ("num_pages", C.c_int32), ("num_seqs", C.c_int32), ("ld_tables", C.c_int32),
+        ("tables", C.c_void_p), ("tables_out", C.c_void_p), ("lengths", C.c_void_p), ("lengths_out", C.c_void_p),
+        ("parents", C.c_void_p), ("advance", C.c_int32), ("rows", C.c_int32), ("absent", C.c_int32),
+        ("copies", C.c_void_p), ("status", C.c_void_p),
+    ]
+
+
+class PagesCopy(C.Structure):
+    _fields_ = [
+        ("copies", C.c_void_p), ("max_copies", C.c_int32),
+        ("num_pages", C.c_int32), ("num_heads", C.c_int32), ("layers", C.c_int32),
+        ("pools", C.c_void_p * 4), ("block_bytes", C.c_int32 * 4),
+    ]
+
+
 _vp, _i32, _f32, _sz = C.c_void_p, C.c_int32, C.c_float, C.c_size_t
 
 # name -> (restype, argtypes)
@@ -200,6 +229,14 @@ SIGNATURES = {
                                       _vp]),
     "dtree_attention_q8_workspace_bytes": (_sz, [C.POINTER(KvQ8), C.POINTER(AttnQ8Args)]),
     "dtree_attention_q8": (C.c_int, [C.POINTER(KvQ8), C.POINTER(AttnQ8Args), _vp]),
+    "dtree_beam_args_bytes": (_sz, []),
+    "dtree_beam_select_workspace_bytes": (_sz, [C.POINTER(BeamArgs)]),
+    "dtree_beam_select": (C.c_int, [C.POINTER(BeamArgs), _vp]),
+    "dtree_pages_fork_bytes": (_sz, []),
+    "dtree_pages_fork": (C.c_int, [C.POINTER(PagesFork), _vp]),
+    "dtree_pages_copy_bytes": (_sz, []),
+    "dtree_pages_copy": (C.c_int, [C.POINTER(PagesCopy), _vp]),
+    "dtree_gdn_layer_batch": (C.c_int, [C.POINTER(GdnArgs), _vp, _i32, _vp]),
     "dtree_graph_begin": (C.c_int, [_vp]),
     "dtree_graph_end": (C.c_int, [_vp, C.POINTER(C.c_void_p)]),
     "dtree_graph_launch": (C.c_int, [_vp, _vp]),
@@ -227,7 +264,9 @@ def lib() -> C.CDLL:
         raise DtreeError("libdtree_hip.so ABI version mismatch; rebuild it")
     for fn, struct in (("dtree_step_desc_bytes", StepDesc), ("dtree_gemm_args_bytes", GemmArgs),
                        ("dtree_attn_args_bytes", AttnArgs), ("dtree_gdn_args_bytes", GdnArgs),
-                       ("dtree_kv_q8_bytes", KvQ8), ("dtree_attn_q8_args_bytes", AttnQ8Args)):
+                       ("dtree_kv_q8_bytes", KvQ8), ("dtree_attn_q8_args_bytes", AttnQ8Args),
+                       ("dtree_beam_args_bytes", BeamArgs), ("dtree_pages_fork_bytes", PagesFork),
+                       ("dtree_pages_copy_bytes", PagesCopy)):
         if getattr(h, fn)() != C.sizeof(struct):
             raise DtreeError(f"{struct.__name__} layout mismatch between Python and the library")
     _LIB = h

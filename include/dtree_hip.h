@@ -20,7 +20,7 @@
 extern "C" {
 #endif
 
-#define DTREE_ABI_VERSION 8
+#define DTREE_ABI_VERSION 9
 
 #define DTREE_OK 0
 #define DTREE_E_ARG (-1)      /* bad shape / pointer / enum */
@@ -683,6 +683,124 @@ size_t dtree_kv_q8_bytes(void);         /* sizeof, for bindings */
 size_t dtree_attn_q8_args_bytes(void);
 size_t dtree_attention_q8_workspace_bytes(const DtreeKvQ8* kv, const DtreeAttnQ8Args* args);
 int dtree_attention_q8(const DtreeKvQ8* kv, const DtreeAttnQ8Args* args, hipStream_t stream);
+
+/*
+ * Beam search's selection (the several-hypotheses counterpart of
+ * dtree_lmhead_argmax and dtree_accept_walk): of each of `groups` groups the best
+ * num_select continuations over its `beams` beams and the vocabulary. Row
+ * r = group * beams + beam of logits is that beam's; in it NaN counts as -inf and
+ * +inf as fp32's largest number, so forbidden tokens are -inf, and a row without
+ * any other has no continuation. With lse = log sum exp of the row, token t
+ * continues a beam with the sum scores[r] + (x_t - lse) and length lengths[r] + 1;
+ * a finished beam has one continuation, pad_token with its own score and length
+ * (its logits are not read); a beam with the score -inf (or NaN) has none. The best
+ * are those of the largest sum / max(length, 1)^length_penalty, ties to the lower
+ * beam, then the lower token; sums and comparisons are fp64, lse is within about
+ * 1e-7.
+ *
+ * Outputs, [groups][num_select], best first: the sum (fp32), the token, the parent
+ * (its row r), and optionally its length, whether it is finished (its beam was, or
+ * the token is eos_token) and its source (the parent, or -1 if finished: what
+ * dtree_pages_fork and dtree_gdn_layer_batch take, so that a finished hypothesis
+ * gives its pages up). Where fewer continuations exist the rest are -inf, -1, -1,
+ * 0, 0, -1. scores_out, lengths_out and finished_out may be the inputs' arrays if
+ * num_select == beams, and must not overlap them otherwise.
+ * Limits: beams and num_select up to 64, vocab up to 2^20.
+ * workspace: dtree_beam_select_workspace_bytes (16-byte aligned, any contents; 0
+ * for arguments that are refused); calls that share one must not overlap.
+ */
+typedef struct DtreeBeamArgs {
+  const void* logits; int32_t type, ld_logits;  /* DTREE_T_F32 or DTREE_T_BF16; ld_logits >= vocab, any */
+  int32_t vocab, groups, beams, num_select;
+  const float* scores;      /* [groups][beams], NULL: 0 */
+  const int32_t* lengths;   /* the same, NULL: 0 */
+  const int32_t* finished;  /* the same, NULL: none */
+  int32_t eos_token;        /* -1: none */
+  int32_t pad_token;
+  float length_penalty;     /* 0: none; in [-16, 16] */
+  float* scores_out; int32_t* tokens_out; int32_t* parents_out;
+  int32_t* lengths_out; int32_t* finished_out; int32_t* sources_out;  /* optional */
+  void* workspace; size_t workspace_bytes;
+} DtreeBeamArgs;
+
+size_t dtree_beam_args_bytes(void);
+size_t dtree_beam_select_workspace_bytes(const DtreeBeamArgs* args);
+int dtree_beam_select(const DtreeBeamArgs* args, hipStream_t stream);
+
+/*
+ * Forked sequences over one pool of cache pages (DTREE_PAGE positions each; of any
+ * of the paged caches: only page numbers are dealt with here). tables
+ * [num_seqs][ld_tables] hold the physical pages of a sequence's positions, lengths
+ * its positions, refs[page] the number of sequences that hold the page (0: free; a
+ * caller that keeps pages for itself counts too). A page stands at most once in a
+ * table.
+ *
+ * Sequence i of the result continues sequence parents[i] (any other value than a
+ * sequence: an empty one; parents NULL: itself) at the length L = lengths[parent] +
+ * advance, in [0, 64 ld_tables]. It holds the parent's pages of positions 0 .. L - 1
+ * (pages behind are given back) and pages for `rows` more positions, and no others:
+ * the rest of its table is `absent` (-1, or a page that the caller keeps for this,
+ * which is then never taken, counted or copied; the bf16 caches' kernels read table
+ * entries behind a sequence's end). Where rows > 0 and position L falls into a page
+ * that others hold as well, the sequence takes a page of its own for it, in
+ * ascending order of sequences, so that the last holder keeps the page. Pages are
+ * taken in ascending order, by ascending sequence, the copy's before the new ones.
+ * Entries of tables outside [0, num_pages) count as absent.
+ *
+ * copies (optional) [num_seqs][3]: the page copies to make (dtree_pages_copy), by
+ * ascending sequence: source, destination, positions in use (L % 64); the rest -1.
+ * status (optional) [2]: the number of pages that were not to be had (none free, or
+ * the table full) is added to the first word, and their entries are absent; the
+ * second becomes the number of copies. refs change in place. tables_out may be
+ * tables without parents, else they must not overlap; lengths_out may be lengths.
+ * Up to 1024 sequences.
+ */
+typedef struct DtreePagesFork {
+  int32_t* refs; int32_t num_pages;
+  int32_t num_seqs, ld_tables;
+  const int32_t* tables; int32_t* tables_out;
+  const int32_t* lengths; int32_t* lengths_out;
+  const int32_t* parents;
+  int32_t advance, rows, absent;
+  int32_t* copies; int32_t* status;
+} DtreePagesFork;
+
+size_t dtree_pages_fork_bytes(void);
+int dtree_pages_fork(const DtreePagesFork* args, hipStream_t stream);
+
+/*
+ * The page copies of a list [max_copies][3] of (source, destination, positions in
+ * use), which ends at its first negative source; entries with a page outside
+ * [0, num_pages) or no positions are passed over. pools[i] (up to 4, NULL: none) is
+ * [layers][num_pages][num_heads][block_bytes[i]], 16-byte aligned, block_bytes[i] a
+ * multiple of 32: K and V pages and, in the 8-bit cache, their scales. Up to 32
+ * positions in use copy the first half of each block, which holds positions 0 .. 31
+ * in every page order here; the other half of the destination stays as it was.
+ * Destinations are distinct, and no source is a destination.
+ */
+typedef struct DtreePagesCopy {
+  const int32_t* copies; int32_t max_copies;
+  int32_t num_pages, num_heads, layers;
+  void* pools[4]; int32_t block_bytes[4];
+} DtreePagesCopy;
+
+size_t dtree_pages_copy_bytes(void);
+int dtree_pages_copy(const DtreePagesCopy* args, hipStream_t stream);
+
+/*
+ * One token of each of num_seqs sequences through a GatedDeltaNet layer's core
+ * (custom_qwen35_model.py:823-878; the arithmetic of dtree_gdn_layer_prep,
+ * _recurrence and _gated_norm for a root alone, and its commit): row b of proj and
+ * out is sequence b's token. Its window and state before the token are those of
+ * sequence sources[b] (NULL: b; anything outside [0, num_seqs): a sequence that
+ * begins, zeros), so a beam search's reordering of states is part of the step.
+ * window, window_out: [num_seqs][conv_keep][C], state, state_out:
+ * [num_seqs][Hv][Dv][Dk], the new ones in buffers of their own. Rows num_seqs ..
+ * rows_padded - 1 of out become zero; desc, q, k, v, g, beta and y are not used.
+ * proj, conv_w, windows and states 16-byte aligned, ld_proj a multiple of 4.
+ * Compiled for Dk = Dv = 128.
+ */
+int dtree_gdn_layer_batch(const DtreeGdnArgs* args, const int32_t* sources, int32_t num_seqs, hipStream_t stream);
 
 /* Convert a row-major [n][k] bf16 matrix to DTREE_W_TILED (n % 32 == 0,
  * k % 64 == 0; src and dst must not overlap). */
