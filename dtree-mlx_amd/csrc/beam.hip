@@ -35,7 +35,6 @@ constexpr int kMaxSelect = 64;
 constexpr int kMaxVocab = 1 << 20;
 constexpr int kPickThreads = 512, kPickWaves = kPickThreads / 64;
 constexpr int kKeep = 2 * kMaxSelect;  // survivors of a level
-constexpr int kInReg = 8;              // a level's items of a thread that stay in registers
 constexpr float kBig = 3.40282347e38f;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -53,17 +52,21 @@ __device__ __forceinline__ float clean(float x) { return x > -INFINITY ? fminf(x
 __device__ __forceinline__ bool beam_over(const DtreeBeamArgs& a, int row) { return a.finished && a.finished[row]; }
 __device__ __forceinline__ float beam_score(const DtreeBeamArgs& a, int row) { return a.scores ? a.scores[row] : 0.f; }
 
+// f over the wave's 64 lanes, in each of them: within rows of 16, then the four rows.
+template <class F>
+__device__ __forceinline__ float wave_all(float v, F f) {
+  v = f(v, dpp<0xB1>(v));
+  v = f(v, dpp<0x4E>(v));
+  v = f(v, dpp<0x141>(v));
+  v = f(v, dpp<0x140>(v));
+  auto row = [&](int lane) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane)); };
+  return f(f(row(0), row(16)), f(row(32), row(48)));
+}
 __device__ __forceinline__ float wave_max(float v) {
-  v = fmaxf(v, dpp<0xB1>(v));
-  v = fmaxf(v, dpp<0x4E>(v));
-  v = fmaxf(v, dpp<0x141>(v));
-  v = fmaxf(v, dpp<0x140>(v));
-  v = fmaxf(v, swz_xor16(v));
-  return fmaxf(v, __shfl_xor(v, 32));
+  return wave_all(v, [](float a, float b) { return fmaxf(a, b); });
 }
 __device__ __forceinline__ float wave_sum(float v) {
-  v = row_sum32(v);
-  return v + __shfl_xor(v, 32);
+  return wave_all(v, [](float a, float b) { return a + b; });
 }
 
 template <bool BF>
@@ -72,6 +75,9 @@ __device__ __forceinline__ float logit(const DtreeBeamArgs& a, int row, int t) {
   if constexpr (BF) return clean(bf2f(static_cast<const uint16_t*>(a.logits)[at]));
   else return clean(static_cast<const float*>(a.logits)[at]);
 }
+
+// (rows at any address of their type)
+typedef u32x4_t u32x4_any_t __attribute__((aligned(2)));
 
 template <bool BF>
 __global__ __launch_bounds__(256) void beam_scan_kernel(BeamParams p) {
@@ -89,7 +95,7 @@ __global__ __launch_bounds__(256) void beam_scan_kernel(BeamParams p) {
     const int at = (i * 256 + tid) * E;
     if (at + E <= left) {
       u32x4_t w;
-      __builtin_memcpy(&w, src + (size_t)at * (BF ? 2 : 4), 16);  // (rows at any address of their type)
+      w = __builtin_nontemporal_load(reinterpret_cast<const u32x4_any_t*>(src + (size_t)at * (BF ? 2 : 4)));
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         if constexpr (BF) x[i][e] = __uint_as_float((e & 1) ? (w[e >> 1] & 0xffff0000u) : (w[e >> 1] << 16));
@@ -146,6 +152,66 @@ __device__ __forceinline__ uint64_t order_of(double v) {
   const uint64_t b = __builtin_bit_cast(uint64_t, v + 0.0);
   return (b >> 63) ? ~b : b | 0x8000000000000000ull;
 }
+__device__ __forceinline__ double rank_of(uint64_t key) {
+  return __builtin_bit_cast(double, (key >> 63) ? key & 0x7fffffffffffffffull : ~key);
+}
+
+template <int CTRL>
+__device__ __forceinline__ uint64_t dpp64(uint64_t v) {
+  return (uint64_t)(uint32_t)dpp_i<CTRL>((int)(uint32_t)(v >> 32)) << 32 | (uint32_t)dpp_i<CTRL>((int)(uint32_t)v);
+}
+template <int CTRL>
+__device__ __forceinline__ double dpp_f64(double v) {
+  return __builtin_bit_cast(double, dpp64<CTRL>(__builtin_bit_cast(uint64_t, v)));
+}
+__device__ __forceinline__ uint64_t lane64(uint64_t v, int lane) {
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), lane) << 32 |
+         (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
+}
+template <class F>
+__device__ __forceinline__ uint64_t wave_all64(uint64_t v, F f) {
+  v = f(v, dpp64<0xB1>(v));
+  v = f(v, dpp64<0x4E>(v));
+  v = f(v, dpp64<0x141>(v));
+  v = f(v, dpp64<0x140>(v));
+  return f(f(lane64(v, 0), lane64(v, 16)), f(lane64(v, 32), lane64(v, 48)));
+}
+
+// Lists of the quick way. A level of it keeps more than it must; where ties or a
+// crowd of near ranks overflow one, the group goes the sure way.
+constexpr int kSlack = 32;                  // more than the selected ones that a threshold may leave
+constexpr int kUnits1 = kMaxSelect + kSlack;  // units kept
+constexpr int kSegs1 = 512, kBest1 = 256;   // segments, logits
+constexpr int kStaged = 4096;               // (beam, chunk) pairs and units it takes, in LDS
+
+__device__ __forceinline__ uint32_t order_of(float v) {
+  const uint32_t b = __float_as_uint(v + 0.f);
+  return (b >> 31) ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float from_order(uint32_t o) {
+  return __uint_as_float((o >> 31) ? o & 0x7fffffffu : ~o);
+}
+
+// ln s for s >= 1/2, within 1e-9 (the sums are good to 1e-7): s = 2^e m, m in [0.7,
+// 1.4], ln m = 2 atanh((m - 1) / (m + 1)). Little code: the kernel's own instructions
+// are part of its latency.
+__device__ __forceinline__ double ln_of(double s) {
+  const uint64_t bits = __builtin_bit_cast(uint64_t, s);
+  const uint64_t shift = (bits & 0x000fffffffffffffull) > 0x0006a09e667f3bcdull ? 1 : 0;
+  const int e = (int)(bits >> 52) - 1023 + (int)shift;
+  const double m = __builtin_bit_cast(double, (bits & 0x000fffffffffffffull) | (1023 - shift) << 52);
+  const double d = m + 1.;
+  double r = __builtin_amdgcn_rcp(d);
+  r = fma(r, fma(-d, r, 1.), r);
+  const double t = (m - 1.) * r, u = t * t;
+  double y = 1. / 11;
+  y = fma(y, u, 1. / 9);
+  y = fma(y, u, 1. / 7);
+  y = fma(y, u, 1. / 5);
+  y = fma(y, u, 1. / 3);
+  y = fma(y, u, 1.);
+  return fma((double)e, 0.69314718055994531, 2. * t * y);
+}
 
 struct Item {
   uint64_t key;
@@ -153,24 +219,29 @@ struct Item {
 };
 
 struct PickLds {
-  double score[kMaxBeams], lse[kMaxBeams], weight[kMaxBeams];  // lse: less the maximum
-  int live[kMaxBeams];  // 1: summed over its vocabulary, 2: finished
-  float m[kMaxBeams];
+  double score[kMaxBeams], lse[kMaxBeams];        // lse: less the maximum
+  double weight[kMaxBeams], back[kMaxBeams];      // length^-penalty, length^penalty
+  float m[kMaxBeams], least[kMaxBeams];                        // least: the logits that reach the threshold
+  int kind[kMaxBeams], length[kMaxBeams];                      // kind 1: summed over its vocabulary, 2: finished
   int count[2][kPickWaves];
   uint64_t lo[kPickWaves], hi[kPickWaves];
-  int n;
+  int n, n2, n3;
   uint32_t list[2][kKeep];
-  uint64_t key[kKeep];
-  double total[kKeep];
+  uint32_t units[kUnits1], segs[kSegs1];  // beam << 16 | first segment, segment of the row
+  struct {
+    uint64_t key;
+    uint32_t id;
+    float x;
+  } cand[kBest1];
+  float top[kStaged];  // the chunks' maxima, of live beams
+  __attribute__((aligned(16))) float unit[kStaged];
 };
 
-// How many of the workgroup's threads' counts there are, in every thread.
+// The sum over the waves of a count that is uniform in each. Two buffers, so that one
+// barrier a call is enough.
 __device__ __forceinline__ int block_count(PickLds& l, int& turn, int c) {
-  // (sums over lanes; two buffers, so that one barrier a call is enough)
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) c += __shfl_xor(c, o);
   if ((threadIdx.x & 63) == 0) l.count[turn][threadIdx.x >> 6] = c;
-  __syncthreads();
+  lds_barrier();
   int n = 0;
 #pragma unroll
   for (int w = 0; w < kPickWaves; ++w) n += l.count[turn][w];
@@ -178,34 +249,37 @@ __device__ __forceinline__ int block_count(PickLds& l, int& turn, int c) {
   return n;
 }
 
+// A place in a list for each lane of `take`.
+__device__ __forceinline__ int place(int* n, bool take) {
+  const uint64_t mask = __ballot(take);
+  if (!mask) return 0;
+  int at = 0;
+  if ((threadIdx.x & 63) == 0) at = atomicAdd(n, (int)__popcll(mask));
+  return __builtin_amdgcn_readfirstlane(at) + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+}
+
 // Keeps n >= want of a level's N items, at most 2 want, that hold the best `want`
-// (all, if there are fewer): put(item) for each, in any order. `from`: a key that
-// `want` items are known to reach (1: nothing is known); returns one for the next level.
+// (all, if there are fewer): put(n, item) for each, in any order. `from`: a key that
+// `want` items are known to reach (1: nothing is known); returns one for the next
+// level. Bisection on the key, then, where keys tie, on the position: it ends whatever
+// the items are.
 template <class Get, class Put>
 __device__ __forceinline__ uint64_t level(PickLds& l, int& turn, int N, int want, uint64_t from, Get get, Put put) {
   const int tid = threadIdx.x;
   const int most = 2 * want;
-  Item mine[kInReg];
-#pragma unroll
-  for (int r = 0; r < kInReg; ++r) {
-    const int i = tid + r * kPickThreads;
-    mine[r] = i < N ? get(i) : Item{0, 0};
-  }
   auto each = [&](auto f) {
-#pragma unroll
-    for (int r = 0; r < kInReg; ++r) f(mine[r]);
-    for (int i = tid + kInReg * kPickThreads; i < N; i += kPickThreads) f(get(i));
+    for (int i0 = 0; i0 < N; i0 += kPickThreads) f(i0 + tid < N ? get(i0 + tid) : Item{0, 0});
   };
   auto count = [&](auto pred) {
     int c = 0;
-    each([&](const Item& it) { c += it.key && pred(it) ? 1 : 0; });
+    each([&](const Item& it) { c += __popcll(__ballot(it.key && pred(it))); });
     return block_count(l, turn, c);
   };
   uint64_t key = from;
   uint32_t id = ~0u;
   int n = count([&](const Item& it) { return it.key >= key; });
   if (n > most) {
-    // bisection: more than `most` reach lo, fewer than `want` reach hi
+    // more than `most` reach lo, fewer than `want` reach hi
     uint64_t lo = ~0ull, hi = 0;
     each([&](const Item& it) {
       if (it.key >= key && it.key) {
@@ -213,12 +287,8 @@ __device__ __forceinline__ uint64_t level(PickLds& l, int& turn, int N, int want
         hi = it.key > hi ? it.key : hi;
       }
     });
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) {
-      const uint64_t a = __shfl_xor(lo, o), b = __shfl_xor(hi, o);
-      lo = a < lo ? a : lo;
-      hi = b > hi ? b : hi;
-    }
+    lo = wave_all64(lo, [](uint64_t a, uint64_t b) { return a < b ? a : b; });
+    hi = wave_all64(hi, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
     if ((tid & 63) == 0) {
       l.lo[tid >> 6] = lo;
       l.hi[tid >> 6] = hi;
@@ -229,7 +299,7 @@ __device__ __forceinline__ uint64_t level(PickLds& l, int& turn, int N, int want
       lo = l.lo[w] < lo ? l.lo[w] : lo;
       hi = l.hi[w] > hi ? l.hi[w] : hi;
     }
-    hi += 1;  // (below the largest key's end: no rank is NaN)
+    hi += 1;  // (no rank is NaN: there is room)
     bool done = false;
     int above = 0;  // items that reach hi
     while (hi - lo > 1 && !done) {
@@ -254,7 +324,9 @@ __device__ __forceinline__ uint64_t level(PickLds& l, int& turn, int N, int want
   if (tid == 0) l.n = 0;
   __syncthreads();
   each([&](const Item& it) {
-    if (it.key && (it.key > key || (it.key == key && it.id <= id))) put(atomicAdd(&l.n, 1), it);
+    const bool take = it.key && (it.key > key || (it.key == key && it.id <= id));
+    const int at = place(&l.n, take);
+    if (take) put(at, it);
   });
   __syncthreads();
   return key;
@@ -265,94 +337,293 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(BeamParams p) {
   __shared__ PickLds l;
   const DtreeBeamArgs& a = p.a;
   const int g = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int K = a.beams, M = a.num_select, NC = p.chunks, row0 = g * K;
-  // the beams' sums: log sum exp over the chunks
-  for (int b = wave; b < K; b += kPickWaves) {
-    const float2* part = p.part + (size_t)(row0 + b) * NC;
-    const bool over = beam_over(a, row0 + b);
-    const bool live = !over && beam_score(a, row0 + b) > -INFINITY;
-    float m = -INFINITY;
-    double s = 0.;
-    if (live) {
-      for (int c = lane; c < NC; c += 64) m = fmaxf(m, part[c].x);
-      m = wave_max(m);
-      const float base = fmaxf(m, -kBig);
-      for (int c = lane; c < NC; c += 64) s += (double)(part[c].y * fast_exp2((part[c].x - base) * kLog2e));
+  const int K = a.beams, M = a.num_select, NC = p.chunks, row0 = g * K, V = a.vocab;
+  const int N1 = K * NC;
+  const float2* part = p.part + (size_t)row0 * NC;
+  const bool staged = N1 <= kStaged;
+  if (wave == kPickWaves - 1) {  // the beams' words
+    const int row = row0 + min(lane, K - 1);
+    const float score = beam_score(a, row);
+    const bool over = beam_over(a, row);
+    const int length = (a.lengths ? a.lengths[row] : 0) + (over ? 0 : 1);
+    double w = 1., back = 1.;
+    if (a.length_penalty != 0.f) {
+      back = exp((double)a.length_penalty * log((double)max(length, 1)));
+      w = 1. / back;
+    }
+    if (lane < K) {
+      l.kind[lane] = over ? 2 : score > -INFINITY ? 1 : 0;
+      l.score[lane] = score == score ? (double)score : -(double)INFINITY;
+      l.length[lane] = length;
+      l.weight[lane] = w;
+      l.back[lane] = back;
+    }
+    if (lane == 0) l.n = l.n2 = l.n3 = 0;
+  } else {  // their log sum exp over the chunks, 16 lanes each
+    for (int b = 4 * wave + (lane >> 4); b < K; b += 4 * (kPickWaves - 1)) {
+      const bool live = !beam_over(a, row0 + b) && beam_score(a, row0 + b) > -INFINITY;
+      float m = -INFINITY;
+      constexpr int kHeld = 3;  // pairs of a lane that stay in registers
+      float2 held[kHeld];
 #pragma unroll
-      for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o);
+      for (int r = 0; r < kHeld; ++r) {
+        const int c = (lane & 15) + 16 * r;
+        held[r] = c < NC ? part[b * NC + c] : make_float2(-INFINITY, 0.f);
+      }
+      // (a finished beam's are whatever the workspace holds)
+      auto each = [&](auto f) {
+#pragma unroll
+        for (int r = 0; r < kHeld; ++r)
+          if ((lane & 15) + 16 * r < NC) f((lane & 15) + 16 * r, held[r]);
+#pragma unroll 1
+        for (int c = (lane & 15) + 16 * kHeld; c < NC; c += 16) f(c, part[b * NC + c]);
+      };
+      each([&](int c, float2 v) {
+        const float x = live ? v.x : -INFINITY;
+        if (staged) l.top[b * NC + c] = x;
+        m = fmaxf(m, x);
+      });
+      m = fmaxf(m, dpp<0xB1>(m));
+      m = fmaxf(m, dpp<0x4E>(m));
+      m = fmaxf(m, dpp<0x141>(m));
+      m = fmaxf(m, dpp<0x140>(m));
+      const float base = fmaxf(m, -kBig);
+      double s = 0.;
+      each([&](int, float2 v) { s += (double)(v.y * fast_exp2((v.x - base) * kLog2e)); });
+      s += dpp_f64<0xB1>(s);
+      s += dpp_f64<0x4E>(s);
+      s += dpp_f64<0x141>(s);
+      s += dpp_f64<0x140>(s);
+      if ((lane & 15) == 0) {
+        l.m[b] = m;  // (-inf: a row without a token to choose, which no rank below stands for)
+        l.lse[b] = m > -INFINITY ? ln_of(s) : 0.;
+      }
     }
-    if (lane == 0) {
-      l.live[b] = over ? 2 : live && m > -INFINITY ? 1 : 0;
-      l.m[b] = m;
-      l.lse[b] = s;
-    }
-  }
-  __syncthreads();
-  if (tid < K) {
-    const float score = beam_score(a, row0 + tid);
-    const int kind = l.live[tid];
-    const int len = max((a.lengths ? a.lengths[row0 + tid] : 0) + (kind == 2 ? 0 : 1), 1);
-    l.score[tid] = score == score ? (double)score : -(double)INFINITY;
-    l.lse[tid] = kind == 1 ? log(l.lse[tid]) : 0.;
-    l.weight[tid] = a.length_penalty != 0.f ? pow((double)len, -(double)a.length_penalty) : 1.;
   }
   __syncthreads();
   int turn = 0;
   auto total = [&](int b, float x) { return l.score[b] + (((double)x - (double)l.m[b]) - l.lse[b]); };
-  auto item = [&](int b, float x, uint32_t id) {
-    return Item{x > -INFINITY && l.live[b] == 1 ? order_of(total(b, x) * l.weight[b]) : 0ull, id};
+  auto key_of = [&](int b, float x) {
+    return l.kind[b] == 1 && x > -INFINITY ? order_of(total(b, x) * l.weight[b]) : 0ull;
   };
-  uint64_t from = 1;
-  from = level(l, turn, K * NC, M, from,
-               [&](int i) {
-                 const int b = i / NC;
-                 return l.live[b] == 1 ? item(b, p.part[(size_t)row0 * NC + i].x, (uint32_t)i) : Item{0, 0};
-               },
-               [&](int n, const Item& it) { l.list[0][n] = it.id; });
-  const int nc = l.n;
-  from = level(l, turn, nc * kSegs, M, from,
-               [&](int i) {
-                 const uint32_t c = l.list[0][i / kSegs];
-                 const uint32_t id = c * kSegs + i % kSegs;
-                 return item(c / NC, p.seg[(size_t)row0 * NC * kSegs + id], id);
-               },
-               [&](int n, const Item& it) { l.list[1][n] = it.id; });
-  const int ns = l.n;
-  level(l, turn, ns * kSeg + K, M, from,
-        [&](int i) {
-          if (i >= ns * kSeg) {
-            const int b = i - ns * kSeg;
-            return Item{l.live[b] == 2 ? order_of(l.score[b] * l.weight[b]) : 0ull, (uint32_t)(b * a.vocab + a.pad_token)};
+  // the nearest fp32: in the same order, ranks below its range at its end
+  auto rank32 = [&](int b, float x) { return fmaxf((float)(total(b, x) * l.weight[b]), -kBig); };
+  auto ended = [&](int b) { return l.kind[b] == 2 ? order_of(l.score[b] * l.weight[b]) : 0ull; };
+
+  int n = -1;  // the candidates left, in l.cand; -1: none yet
+  if (staged) {
+    // The quick way. Units by their maxima: chunks, or, where there are few, parts of
+    // them, so that the threshold is one among many.
+    int shift = 7;  // segments of a unit: 1 << shift, at least four
+    if (N1 < 8 * M)
+      while (shift > 2 && (N1 << (8 - shift)) <= kStaged / 4) --shift;
+    const int NU = N1 << (7 - shift), ends = (NU + 255) & ~255;  // (padded with -inf)
+    const float inv = 1.f / NC;
+    // (i / NC for i < 4096: the half is far above the product's error)
+    auto beam_of = [&](int u) { return (int)(((u >> (7 - shift)) + 0.5f) * inv); };
+    const f32x4_t* seg4 = reinterpret_cast<const f32x4_t*>(p.seg + (size_t)row0 * NC * kSegs);
+#pragma unroll 1
+    for (int i = tid; i < ends; i += kPickThreads) {
+      const int b = min(beam_of(i), K - 1);
+      float x = -INFINITY;
+      if (i < NU && l.kind[b] == 1) {
+        if (shift == 7) {
+          x = l.top[i];
+        } else {
+          const f32x4_t* v = seg4 + ((size_t)i << (shift - 2));
+#pragma unroll 4
+          for (int j = 0; j < 1 << (shift - 2); ++j) x = fmaxf(fmaxf(fmaxf(x, v[j][0]), fmaxf(v[j][1], v[j][2])), v[j][3]);
+        }
+      }
+      l.unit[i] = x > -INFINITY ? rank32(b, x) : -INFINITY;
+    }
+    __syncthreads();
+    // A threshold that M to M + kSlack of them reach, if there is one: below the best
+    // rank by growing steps, then between two; eight thresholds at a time, one a wave.
+    const f32x4_t* unit4 = reinterpret_cast<const f32x4_t*>(l.unit);
+    float best = -INFINITY;
+    if (lane < K && l.kind[lane] == 1 && l.m[lane] > -INFINITY) best = rank32(lane, l.m[lane]);
+    best = wave_max(best);
+    const uint32_t all32 = order_of(-kBig);
+    uint32_t lo = all32, hi = order_of(best) + 1;  // more than M + kSlack reach lo, fewer than M hi
+    float t = -kBig;
+    bool ok = false;
+    for (int round = 0; !ok && (round == 0 || hi - lo > 1); ++round) {
+      const int w = lane & (kPickWaves - 1);  // the probe of lane w, from the highest down
+      uint32_t at;
+      if (round == 0) at = w == kPickWaves - 1 ? all32 : order_of(fmaxf(best - ldexpf((float)l.weight[0], w - 1), -kBig));
+      else at = hi - max((uint32_t)((uint64_t)(hi - lo) * (w + 1) / (kPickWaves + 1)), min((uint32_t)w + 1, hi - lo));
+      const float mine = from_order((uint32_t)__builtin_amdgcn_readlane((int)at, wave));
+      int c = 0;
+#pragma unroll 1
+      for (int i = lane; i < ends / 4; i += 64) {
+        const f32x4_t v = unit4[i];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c += (int)__popcll(__ballot(v[e] >= mine));
+      }
+      if (lane == 0) l.count[turn][wave] = c;
+      lds_barrier();
+      const int n = l.count[turn][w];
+      turn ^= 1;
+      if (round == 0 && __builtin_amdgcn_readlane(n, kPickWaves - 1) <= M) {  // all there are
+        ok = true;
+        break;
+      }
+      const int first = __ffsll((unsigned long long)(__ballot(n >= M) & ((1 << kPickWaves) - 1))) - 1;
+      if (first >= 0) {
+        const uint32_t reached = (uint32_t)__builtin_amdgcn_readlane((int)at, first);
+        if (__builtin_amdgcn_readlane(n, first) <= M + kSlack && !(round == 0 && first == kPickWaves - 1)) {
+          ok = true;
+          t = from_order(reached);
+          break;
+        }
+        lo = max(lo, reached);
+      }
+      if (first) hi = min(hi, (uint32_t)__builtin_amdgcn_readlane((int)at, first > 0 ? first - 1 : kPickWaves - 1));
+    }
+    if (ok) {
+#pragma unroll 1
+      for (int i = tid; i - lane < NU; i += kPickThreads) {
+        const bool take = l.unit[i] >= t;
+        const int at = place(&l.n, take);
+        if (take) {
+          const int b = beam_of(i);
+          l.units[at] = (uint32_t)(b << 16 | ((i << shift) - b * NC * kSegs));
+        }
+      }
+      // The least logit of a beam that reaches the number below t (and so every rank that
+      // rounds to t), or one just below.
+      const double low_rank = t > -kBig ? (double)from_order(order_of(t) - 1) : -INFINITY;
+      if (wave == kPickWaves - 1 && lane < K) {
+        float least = INFINITY;
+        if (l.kind[lane] == 1) {
+          const double by = low_rank * l.back[lane], m = (double)l.m[lane];
+          const double x = ((by - l.score[lane]) + l.lse[lane]) + m;
+          const double low = x - 1e-13 * (fabs(by) + fabs(l.score[lane]) + l.lse[lane] + fabs(m));
+          least = low > -(double)kBig ? (float)low : -kBig;
+          if ((double)least > low && least > -kBig) least = from_order(order_of(least) - 1);
+        }
+        l.least[lane] = least;
+      }
+      __syncthreads();
+      // their segments, four a lane
+      const int all = l.n << (shift - 2);
+      constexpr int kAhead = 4;
+      for (int i0 = tid; i0 - tid < all; i0 += kAhead * kPickThreads) {
+        f32x4_t x[kAhead];
+        uint32_t e[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+          const int i = min(i0 + u * kPickThreads, all - 1);
+          e[u] = l.units[i >> (shift - 2)] + 4 * (i & ((1 << (shift - 2)) - 1));
+          x[u] = seg4[(e[u] >> 16) * (NC * kSegs / 4) + (e[u] & 0xffff) / 4];
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+          const float least = i0 + u * kPickThreads < all ? l.least[e[u] >> 16] : INFINITY;
+          const int c = (x[u][0] >= least) + (x[u][1] >= least) + (x[u][2] >= least) + (x[u][3] >= least);
+          if (c) {
+            int at = atomicAdd(&l.n2, c);
+            for (int k = 0; k < 4; ++k)
+              if (x[u][k] >= least) {
+                if (at < kSegs1) l.segs[at] = e[u] + k;
+                ++at;
+              }
           }
-          const uint32_t s = l.list[1][i / kSeg];
-          const int b = s / (NC * kSegs), t = (s % (NC * kSegs)) * kSeg + i % kSeg;
-          return t < a.vocab ? item(b, logit<BF>(a, row0 + b, t), (uint32_t)(b * a.vocab + t)) : Item{0, 0};
-        },
-        [&](int n, const Item& it) {
-          l.key[n] = it.key;
-          l.list[0][n] = it.id;
-        });
-  const int n = l.n;
-  // (inputs that the outputs may replace are read before this barrier)
-  int rank = 0, b = 0, t = 0, len = 0, over = 0;
-  if (tid < n) {
-    const uint64_t key = l.key[tid];
-    const uint32_t id = l.list[0][tid];
-    for (int i = 0; i < n; ++i) rank += l.key[i] > key || (l.key[i] == key && l.list[0][i] < id);
-    b = id / a.vocab;
-    t = id % a.vocab;
-    over = l.live[b] == 2;
-    len = (a.lengths ? a.lengths[row0 + b] : 0) + (over ? 0 : 1);
+        }
+      }
+      __syncthreads();
+      // their logits: half a wave per segment
+      const int ns = min(l.n2, kSegs1);
+      const bool fits = l.n2 <= kSegs1;
+      if (wave == kPickWaves - 1) {  // and the beams that have ended
+        const uint64_t key = lane < K ? ended(lane) : 0;
+        const bool take = key && rank_of(key) >= low_rank;
+        const int at = take ? atomicAdd(&l.n3, 1) : 0;
+        if (take && at < kBest1) {
+          l.cand[at].id = (uint32_t)(lane * V + a.pad_token);
+          l.cand[at].key = key;
+        }
+      }
+      for (int j0 = 2 * wave; j0 < ns && fits; j0 += 2 * kAhead * kPickWaves) {
+        float x[kAhead];
+        uint32_t e[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+          const int j = j0 + 2 * u * kPickWaves + (lane >> 5);
+          e[u] = l.segs[min(j, ns - 1)];
+          const int at = (e[u] & 0xffff) * kSeg + (lane & 31);
+          x[u] = j < ns && at < V ? logit<BF>(a, row0 + (e[u] >> 16), at) : -INFINITY;
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+          const int b = e[u] >> 16;
+          if (x[u] >= l.least[b]) {
+            const int at = atomicAdd(&l.n3, 1);
+            if (at < kBest1) {
+              l.cand[at].id = (uint32_t)(b * V) + (e[u] & 0xffff) * kSeg + (lane & 31);
+              l.cand[at].x = x[u];
+              l.cand[at].key = key_of(b, x[u]);
+            }
+          }
+        }
+      }
+      __syncthreads();
+      if (fits && l.n3 <= kBest1) n = l.n3;
+    }
   }
-  __syncthreads();
+  if (n < 0) {
+    // The sure way, level by level.
+    uint64_t from = 1;
+    auto item = [&](int b, float x, uint32_t id) { return Item{key_of(b, x), id}; };
+    from = level(l, turn, N1, M, from, [&](int i) { return item(i / NC, part[i].x, (uint32_t)i); },
+                 [&](int at, const Item& it) { l.list[0][at] = it.id; });
+    const int nc = l.n;
+    from = level(l, turn, nc * kSegs, M, from,
+                 [&](int i) {
+                   const uint32_t c = l.list[0][i / kSegs];
+                   const uint32_t id = c * kSegs + i % kSegs;
+                   return item(c / NC, p.seg[(size_t)row0 * NC * kSegs + id], id);
+                 },
+                 [&](int at, const Item& it) { l.list[1][at] = it.id; });
+    const int ns = l.n;
+    level(l, turn, ns * kSeg + K, M, from,
+          [&](int i) {
+            if (i >= ns * kSeg) return Item{ended(i - ns * kSeg), (uint32_t)((i - ns * kSeg) * V + a.pad_token)};
+            const uint32_t s = l.list[1][i / kSeg];
+            const int b = s / (NC * kSegs), t = (s % (NC * kSegs)) * kSeg + i % kSeg;
+            return t < V ? item(b, logit<BF>(a, row0 + b, t), (uint32_t)(b * V + t)) : Item{0, 0};
+          },
+          [&](int at, const Item& it) {
+            l.cand[at].key = it.key;
+            l.cand[at].id = it.id;
+            const int b = it.id / V;
+            l.cand[at].x = l.kind[b] == 1 ? logit<BF>(a, row0 + b, it.id % V) : 0.f;
+          });
+    n = l.n;
+  }
+  // Ranked by counting, eight threads a candidate (as many as there are for them all).
+  const int q = n <= kPickThreads / 8 ? 8 : n <= kPickThreads / 4 ? 4 : 2;
+  const int i = tid / q;
+  int rank = 0;
+  if (i < n) {
+    const uint64_t key = l.cand[i].key;
+    const uint32_t id = l.cand[i].id;
+#pragma unroll 4
+    for (int j = tid % q; j < n; j += q) rank += l.cand[j].key > key || (l.cand[j].key == key && l.cand[j].id < id);
+  }
+  rank += dpp_i<0xB1>(rank);
+  if (q >= 4) rank += dpp_i<0x4E>(rank);
+  if (q == 8) rank += dpp_i<0x141>(rank);
+  // (what the outputs may replace has been read)
   const size_t o = (size_t)g * M;
-  if (tid < n && rank < M) {
-    const double s = over ? l.score[b] : total(b, logit<BF>(a, row0 + b, t));
-    const int end = over || t == a.eos_token;
-    a.scores_out[o + rank] = (float)s;
+  if (i < n && rank < M && tid % q == 0) {
+    const uint32_t id = l.cand[i].id;
+    const int b = id / V, t = id % V, over = l.kind[b] == 2, end = over || t == a.eos_token;
+    a.scores_out[o + rank] = (float)(over ? l.score[b] : total(b, l.cand[i].x));
     a.tokens_out[o + rank] = t;
     a.parents_out[o + rank] = row0 + b;
-    if (a.lengths_out) a.lengths_out[o + rank] = len;
+    if (a.lengths_out) a.lengths_out[o + rank] = l.length[b];
     if (a.finished_out) a.finished_out[o + rank] = end;
     if (a.sources_out) a.sources_out[o + rank] = end ? -1 : row0 + b;
   }
