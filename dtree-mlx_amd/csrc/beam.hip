@@ -76,6 +76,14 @@ __device__ __forceinline__ float logit(const DtreeBeamArgs& a, int row, int t) {
   else return clean(static_cast<const float*>(a.logits)[at]);
 }
 
+// v_med3_f32 itself: the compiler's median of a constant infinity is a minimum, which
+// gives the number for a NaN.
+__device__ __forceinline__ float median(float x, float low, float high) {
+  float y;
+  asm("v_med3_f32 %0, %1, %2, %3" : "=v"(y) : "v"(x), "s"(low), "v"(high));
+  return y;
+}
+
 // (rows at any address of their type)
 typedef u32x4_t u32x4_any_t __attribute__((aligned(2)));
 
@@ -87,6 +95,11 @@ __global__ __launch_bounds__(256) void beam_scan_kernel(BeamParams p) {
   const int row = blockIdx.x / p.chunks, chunk = blockIdx.x % p.chunks;
   if (beam_over(p.a, row) || !(beam_score(p.a, row) > -INFINITY)) return;
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  // The median of x, -inf and the largest number is x, cut to them, or, of a NaN, the
+  // least of the two others: -inf. With the mode's IEEE bit (9) cleared that holds for
+  // signalling NaNs too, which it otherwise hands on as quiet ones.
+  __builtin_amdgcn_s_setreg(1 | 9 << 6, 0);
+  const float low = -INFINITY, big = kBig;
   const int left = p.a.vocab - chunk * kChunk;
   float x[NL][E];
   const char* src = static_cast<const char*>(p.a.logits) + ((size_t)row * p.a.ld_logits + chunk * kChunk) * (BF ? 2 : 4);
@@ -118,7 +131,7 @@ __global__ __launch_bounds__(256) void beam_scan_kernel(BeamParams p) {
     float m = -INFINITY;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      x[i][e] = clean(x[i][e]);
+      x[i][e] = median(x[i][e], low, big);
       m = fmaxf(m, x[i][e]);
     }
     m = fmaxf(m, dpp<0xB1>(m));
@@ -136,10 +149,21 @@ __global__ __launch_bounds__(256) void beam_scan_kernel(BeamParams p) {
   mx = fmaxf(fmaxf(wm[0], wm[1]), fmaxf(wm[2], wm[3]));
   const float base = fmaxf(mx, -kBig);
   float sum = 0.f;
+  if (fabsf(base) < 1e30f) {
+    // one operation an exponent: x log2 e - c, c = base log2 e rounded, whose rounding
+    // is a factor of the whole sum
+    const float c = base * kLog2e;
 #pragma unroll
-  for (int i = 0; i < NL; ++i)
+    for (int i = 0; i < NL; ++i)
 #pragma unroll
-    for (int e = 0; e < E; ++e) sum += fast_exp2((x[i][e] - base) * kLog2e);
+      for (int e = 0; e < E; ++e) sum += fast_exp2(fmaf(x[i][e], kLog2e, -c));
+    sum *= fast_exp2(-fmaf(base, kLog2e, -c));
+  } else {
+#pragma unroll
+    for (int i = 0; i < NL; ++i)
+#pragma unroll
+      for (int e = 0; e < E; ++e) sum += fast_exp2((x[i][e] - base) * kLog2e);
+  }
   sum = wave_sum(sum);
   if (lane == 0) ws[wave] = sum;
   __syncthreads();
@@ -416,7 +440,7 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(BeamParams p) {
     // them, so that the threshold is one among many.
     int shift = 7;  // segments of a unit: 1 << shift, at least four
     if (N1 < 8 * M)
-      while (shift > 2 && (N1 << (8 - shift)) <= kStaged / 4) --shift;
+      while (shift > 2 && (N1 << (8 - shift)) <= kPickThreads) --shift;  // (a unit a thread)
     const int NU = N1 << (7 - shift), ends = (NU + 255) & ~255;  // (padded with -inf)
     const float inv = 1.f / NC;
     // (i / NC for i < 4096: the half is far above the product's error)

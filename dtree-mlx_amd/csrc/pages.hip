@@ -7,15 +7,17 @@
 // alone: the counts change by integer atomics, whose order does not matter, and the
 // pages taken are the lowest free ones, by ascending sequence.
 //
-// share  A workgroup per (sequence, 1024 table entries): the entry of its parent into
-//        its new table, and its old table's pages' counts by (children - 1), or down by
-//        one past its length. Sequences with one child touch no count.
+// share  The entry of a sequence's parent into its new table, and its old table's pages'
+//        counts by (children - 1), or down by one past its length. Sequences with one
+//        child touch no count. A workgroup per (sequence, 1024 entries).
 // take   One workgroup, a thread per sequence: which page must be copied (held by others
 //        and about to be written), how many are needed, a prefix sum over the
-//        sequences; then one pass over the counts in page order, in which the free page
-//        of rank r goes to the sequence whose range holds r (a search of the sums in LDS).
+//        sequences. The free pages come from one pass over the counts in page order,
+//        whose loads go out first; they are listed in LDS, and the page of rank r goes
+//        to the sequence whose range holds r (a search of the sums).
+//        Small forks (kOneLaunch entries) are shared by this workgroup too.
 // copy   Persistent workgroups over (copy, layer, head): the half pages in use of every
-//        pool. Bound by the bytes, the tables' two launches by latency.
+//        pool. Bound by the bytes, the tables by latency.
 #include "common.h"
 
 namespace dtree {
@@ -24,8 +26,10 @@ namespace {
 constexpr int kMaxSeqs = 1024;
 constexpr int kShare = 1024;          // table entries of a share workgroup
 constexpr int kTake = 1024, kTakeWaves = kTake / 64;
-constexpr int kScan = 16 * 4;         // counts a thread looks at in one round
-constexpr int kRound = kTake * kScan;
+constexpr int kOneLaunch = 8192;      // table entries that the take workgroup shares by itself
+constexpr int kRun = 32;              // neighbouring counts of a thread in one round
+constexpr int kRound = kTake * kRun;
+constexpr int kList = 4096;           // free pages listed at a time
 constexpr int kHalfPage = DTREE_PAGE / 2;
 
 __device__ __forceinline__ int fork_parent(const DtreePagesFork& a, int i) {
@@ -38,6 +42,21 @@ __device__ __forceinline__ int fork_length(const DtreePagesFork& a, int p) {
 }
 __device__ __forceinline__ bool is_page(const DtreePagesFork& a, int page) {
   return page >= 0 && page < a.num_pages && page != a.absent;
+}
+
+// Entry e of sequence s: the new table's, and the old one's page's count. (SCOPE: an
+// agent's atomics are done behind the XCDs' caches, a lone workgroup's in its own.)
+template <int SCOPE>
+__device__ __forceinline__ void share_entry(const DtreePagesFork& a, int s, int e, int par, int take, int have, int children) {
+  const int mine = a.tables[(size_t)s * a.ld_tables + e];
+  int out = a.absent;
+  if (e < take) {
+    const int page = par == s ? mine : a.tables[(size_t)par * a.ld_tables + e];
+    if (is_page(a, page)) out = page;
+  }
+  a.tables_out[(size_t)s * a.ld_tables + e] = out;
+  const int by = e < have ? children - 1 : -1;
+  if (by && is_page(a, mine)) __hip_atomic_fetch_add(a.refs + mine, by, __ATOMIC_RELAXED, SCOPE);
 }
 
 __global__ __launch_bounds__(256) void pages_share_kernel(DtreePagesFork a) {
@@ -57,163 +76,171 @@ __global__ __launch_bounds__(256) void pages_share_kernel(DtreePagesFork a) {
   const int have = (fork_length(a, s) + DTREE_PAGE - 1) / DTREE_PAGE;
   const int take = par >= 0 ? (fork_length(a, par) + DTREE_PAGE - 1) / DTREE_PAGE : 0;
   const int end = min(a.ld_tables, (int)(blockIdx.y + 1) * kShare);
-  for (int e = blockIdx.y * kShare + tid; e < end; e += 256) {
-    const int mine = a.tables[(size_t)s * a.ld_tables + e];
-    int out = a.absent;
-    if (e < take) {
-      const int page = par == s ? mine : a.tables[(size_t)par * a.ld_tables + e];
-      if (is_page(a, page)) out = page;
-    }
-    a.tables_out[(size_t)s * a.ld_tables + e] = out;
-    const int by = e < have ? children - 1 : -1;
-    if (by && is_page(a, mine)) atomicAdd(a.refs + mine, by);
-  }
+  for (int e = blockIdx.y * kShare + tid; e < end; e += 256)
+    share_entry<__HIP_MEMORY_SCOPE_AGENT>(a, s, e, par, take, have, children);
 }
 
-// Exclusive prefix sum over the workgroup's threads; `all`: the total.
+// Inclusive prefix sum over a wave: within rows of 16, then from row to row.
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);   // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1, 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2, 3
+  return v;
+}
+// Exclusive prefix sum over the workgroup's threads; `all`: the total. `waves`: a
+// buffer that no call shares with the one before it.
 __device__ __forceinline__ int block_scan(int v, int* waves, int& all) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int inc = v;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int u = __shfl_up(inc, o);
-    if (lane >= o) inc += u;
-  }
-  __syncthreads();  // (the last call's sums are read)
-  if (lane == 63) waves[wave] = inc;
+  const int wave = threadIdx.x >> 6, inc = wave_scan(v);
+  if ((threadIdx.x & 63) == 63) waves[wave] = inc;
   __syncthreads();
-  int before = 0, sum = 0;
-#pragma unroll
-  for (int w = 0; w < kTakeWaves; ++w) {
-    before += w < wave ? waves[w] : 0;
-    sum += waves[w];
-  }
-  all = sum;
-  return before + inc - v;
+  const int w = wave_scan((threadIdx.x & 63) < kTakeWaves ? waves[threadIdx.x & 63] : 0);
+  all = __builtin_amdgcn_readlane(w, kTakeWaves - 1);
+  return inc - v + (wave ? __builtin_amdgcn_readlane(w, wave - 1) : 0);
 }
 
+// The free pages among the kRun counts from `first` on, a bit each.
+__device__ __forceinline__ uint32_t free_pages(const DtreePagesFork& a, int64_t first) {
+  int c[kRun];
+  if (first + kRun <= a.num_pages) {
+    __builtin_memcpy(c, a.refs + first, sizeof(c));
+  } else {
+#pragma unroll
+    for (int e = 0; e < kRun; ++e) c[e] = a.refs[min(first + e, (int64_t)a.num_pages - 1)];
+#pragma unroll
+    for (int e = 0; e < kRun; ++e) c[e] |= first + e >= a.num_pages;
+  }
+  uint32_t mask = 0;
+#pragma unroll
+  for (int e = 0; e < kRun; ++e) mask |= c[e] == 0 ? 1u << e : 0u;
+  const int64_t keep = a.absent - first;
+  return keep >= 0 && keep < kRun ? mask & ~(1u << keep) : mask;
+}
+
+template <bool ONE>
 __global__ __launch_bounds__(kTake) void pages_take_kernel(DtreePagesFork a) {
-  __shared__ int waves[kTakeWaves];
-  __shared__ int writes[kMaxSeqs];       // the shared page that a sequence is about to write, -1
-  __shared__ int start[kMaxSeqs + 1];    // pages wanted before a sequence's
+  __shared__ int waves[2][kTakeWaves];
+  __shared__ __attribute__((aligned(16))) int writes[kMaxSeqs];  // the shared page that a sequence is about to write, -1
+  __shared__ int start[kMaxSeqs];        // pages wanted before a sequence's
   __shared__ int first[kMaxSeqs];        // its table entry of the first page past its length; copies: complemented
-  __shared__ int shared_any;
-  const int i = threadIdx.x, n = a.num_seqs;
+  __shared__ int list[kList];            // free pages, ascending
+  __shared__ int kids[ONE ? kMaxSeqs : 1], from[ONE ? kMaxSeqs : 1], size[ONE ? kMaxSeqs : 1];
+  __shared__ int past, fewer;
+  const int i = threadIdx.x, n = a.num_seqs, wave = i >> 6;
   const bool in = i < n;
+  const int64_t mine = (int64_t)i * kRun;
+  // (no count becomes or stops being 0 before the pages are taken: a copied page has
+  // another holder)
+  uint32_t mask = 0;
+  if constexpr (!ONE) mask = mine < a.num_pages ? free_pages(a, mine) : 0;
   const int par = in ? fork_parent(a, i) : -1;
   const int L = par >= 0 ? fork_length(a, par) : 0;
+  if (i == 0) past = fewer = 0;
+  if constexpr (ONE) {
+    const int own = in ? fork_length(a, i) : 0;
+    kids[i] = a.parents ? 0 : 1;
+    from[i] = par;
+    size[i] = own;
+    __syncthreads();
+    if (a.parents && par >= 0) atomicAdd(&kids[par], 1);
+    __syncthreads();
+    const int all = n * a.ld_tables;
+    const float inv = 1.f / a.ld_tables;
+    for (int j = i; j < all; j += kTake) {
+      const int s = (int)((j + 0.5f) * inv);  // (j < 8192: the half is far above the product's error)
+      const int p = from[s];
+      share_entry<__HIP_MEMORY_SCOPE_WORKGROUP>(a, s, j - s * a.ld_tables, p, p >= 0 ? (size[p] + DTREE_PAGE - 1) / DTREE_PAGE : 0,
+                                                (size[s] + DTREE_PAGE - 1) / DTREE_PAGE, kids[s]);
+    }
+    wait_stores_done();  // (the counts' changes too)
+  }
+  __syncthreads();  // (every length is read: lengths_out may be lengths)
+  // (this launch has read no count before: none is in this CU's cache)
+  if constexpr (ONE) mask = mine < a.num_pages ? free_pages(a, mine) : 0;
   const int covered = (L + DTREE_PAGE - 1) / DTREE_PAGE, at = L / DTREE_PAGE;
   const int64_t wanted = in ? ((int64_t)L + a.rows + DTREE_PAGE - 1) / DTREE_PAGE : 0;
   const int last = (int)min(wanted, (int64_t)a.ld_tables);
   int* row = a.tables_out + (size_t)i * a.ld_tables;
-  if (i == 0) shared_any = 0;
-  __syncthreads();  // (every length is read: lengths_out may be lengths)
   if (in) a.lengths_out[i] = L;
+  if (wanted > last) atomicAdd(&past, (int)min(wanted - last, (int64_t)1 << 20));
   int page = -1, holders = 0;
   if (in && a.rows > 0 && L % DTREE_PAGE) {
     page = row[at];
     if (is_page(a, page)) holders = a.refs[page];
-    else page = -1;
   }
   writes[i] = holders > 1 ? page : -1;
-  if (holders > 1) shared_any = 1;
   __syncthreads();
   // Writers of one page, in ascending order: the k-th copies where others are left.
   bool copy = false;
-  if (shared_any) {
-    if (holders > 1) {
-      int k = 0;
-      for (int j = 0; j < i; ++j) k += writes[j] == page;
-      copy = holders - k > 1;
-    }
-  }
-  if (copy) atomicAdd(a.refs + page, -1);
-  int total, copies;
-  const int grow = in ? max(last - covered, 0) : 0;
-  const int before = block_scan((copy ? 1 : 0) + grow, waves, total);
-  start[i] = before;
-  first[i] = copy ? ~covered : covered;
-  if (i == 0) start[n] = total;
-  // (no page: the entries past the length, and a copy's own, stay without one)
-  if (copy) row[at] = a.absent;
-  __syncthreads();
-  // The free pages in ascending order: wave w looks at 64 kScan counts of a round, 256 a load.
-  const int lane = i & 63, wave = i >> 6;
-  int taken = 0;
-  for (int64_t base = 0; base < a.num_pages && taken < total; base += kRound) {
-    const int64_t w0 = base + (int64_t)wave * 64 * kScan;
-    int found = 0;
-    uint64_t mask = 0;  // bit 4 k + e: count 256 k + 4 lane + e of the wave's is 0
-#pragma unroll
-    for (int k = 0; k < kScan / 4; ++k) {
-      const int64_t p0 = w0 + 256 * k + 4 * lane;
-      int c[4] = {1, 1, 1, 1};
-      if (p0 + 3 < a.num_pages) {
-        __builtin_memcpy(c, a.refs + p0, 16);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (p0 + e < a.num_pages) c[e] = a.refs[p0 + e];
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (c[e] == 0 && (int)(p0 + e) != a.absent) mask |= 1ull << (4 * k + e);
-    }
-    found = __popcll(mask);
-    int sum = found;
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o);
-    __syncthreads();
-    if (lane == 0) waves[wave] = sum;
-    __syncthreads();
-    int rank = taken, all = 0;
-#pragma unroll
-    for (int w = 0; w < kTakeWaves; ++w) {
-      rank += w < wave ? waves[w] : 0;
-      all += waves[w];
-    }
-#pragma unroll 1
-    for (int k = 0; k < kScan / 4; ++k) {
-      if (rank >= total) break;  // (a wave's rank is the same in its lanes)
-      const int bits = (int)(mask >> (4 * k)) & 15, c = __popc(bits);
-      int inc = c;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const int u = __shfl_up(inc, o);
-        if (lane >= o) inc += u;
-      }
-      int r = rank + inc - c;
+  if (__any(holders > 1)) {
+    int k = 0, writers = 0;
+    const int4* w4 = reinterpret_cast<const int4*>(writes);
+#pragma unroll 4
+    for (int j = 0; j < (n + 3) / 4; ++j) {
+      const int4 w = w4[j];
+      const int c[4] = {w.x == page, w.y == page, w.z == page, w.w == page};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        if (!(bits >> e & 1)) continue;
-        if (r < total) {
-          const int pg = (int)(w0 + 256 * k + 4 * lane + e);
-          int lo = 0, hi = n;  // the last sequence whose range starts at r or before, of those with one
-          while (hi - lo > 1) {
-            const int mid = (lo + hi) / 2;
-            if (start[mid] <= r) lo = mid;
-            else hi = mid;
-          }
-          const int f = first[lo], j = r - start[lo];
-          int* out = a.tables_out + (size_t)lo * a.ld_tables;
-          // a copy takes the sequence's first page, for the entry before its new ones
-          out[f < 0 ? ~f + j - 1 : f + j] = pg;
-          a.refs[pg] = 1;
-        }
-        ++r;
+        writers += c[e];
+        k += 4 * j + e < i ? c[e] : 0;
       }
-      rank += __shfl(inc, 63);
     }
-    taken += all;
+    copy = holders > 1 && holders - k > 1;
+    if (copy && k == 0) a.refs[page] = holders - min(writers, holders - 1);
   }
-  __syncthreads();
-  const int to = copy ? row[at] : a.absent;
-  const bool made = copy && is_page(a, to);
-  const int spot = block_scan(made ? 1 : 0, waves, copies);
+  if (copy) row[at] = a.absent;  // (until it has a page of its own)
+  int total, copies;
+  const int grow = in ? max(last - covered, 0) : 0;
+  const int before = block_scan((copy ? 1 : 0) + grow, waves[0], total);
+  int spot = block_scan(copy ? 1 : 0, waves[1], copies);
+  start[i] = before;
+  first[i] = copy ? ~covered : covered;
+  // The free pages in ascending order, kList at a time.
+  int seen = 0;  // free pages of the rounds before
+  for (int64_t base = 0; base < a.num_pages && seen < total; base += kRound) {
+    if (base) mask = base + mine < a.num_pages ? free_pages(a, base + mine) : 0;
+    int all;
+    __syncthreads();
+    int rank = seen + block_scan(__popc(mask), waves[0], all);
+    const int end = min(total, seen + all);
+    for (int r0 = seen; r0 < end; r0 += kList) {
+      const int upto = min(end, r0 + kList);
+      while (mask && rank < upto) {
+        list[rank - r0] = (int)(base + mine) + __ffs((int)mask) - 1;
+        mask &= mask - 1;
+        ++rank;
+      }
+      __syncthreads();
+      for (int r = r0 + i; r < upto; r += kTake) {
+        int lo = 0, hi = n;  // the last sequence whose range starts at r or before: the one that holds r
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) / 2;
+          if (start[mid] <= r) lo = mid;
+          else hi = mid;
+        }
+        const int f = first[lo], j = r - start[lo], pg = list[r - r0];
+        // a copy takes the sequence's first page, for the entry before its new ones
+        a.tables_out[(size_t)lo * a.ld_tables + (f < 0 ? ~f + j - 1 : f + j)] = pg;
+        if (f < 0 && j == 0) writes[lo] = pg;
+        a.refs[pg] = 1;
+      }
+      __syncthreads();
+    }
+    seen += all;
+  }
+  // the copies, by sequence; without pages for all of them, those before some sequence
+  const bool made = copy && before < seen;
+  if (seen < total) {
+    if (copy && !made) atomicAdd(&fewer, 1);
+    __syncthreads();
+    copies -= fewer;
+  }
   if (a.copies) {
     if (made) {
       a.copies[3 * spot] = page;
-      a.copies[3 * spot + 1] = to;
+      a.copies[3 * spot + 1] = writes[i];
       a.copies[3 * spot + 2] = L % DTREE_PAGE;
     }
     if (in && i >= copies) {
@@ -222,14 +249,9 @@ __global__ __launch_bounds__(kTake) void pages_take_kernel(DtreePagesFork a) {
       a.copies[3 * i + 2] = -1;
     }
   }
-  if (a.status) {
-    const int beyond = in ? (int)min(wanted - last, (int64_t)1 << 20) : 0;
-    int past;
-    block_scan(beyond, waves, past);
-    if (i == 0) {
-      a.status[0] += max(total - taken, 0) + past;
-      a.status[1] = copies;
-    }
+  if (a.status && i == 0) {
+    a.status[0] += max(total - seen, 0) + past;
+    a.status[1] = copies;
   }
 }
 
@@ -286,10 +308,14 @@ extern "C" int dtree_pages_fork(const DtreePagesFork* a, hipStream_t stream) {
                 "pages_fork: tables and tables_out overlap");
   DTREE_REQUIRE(a->lengths == a->lengths_out || a->lengths + rows <= a->lengths_out || a->lengths_out + rows <= a->lengths,
                 "pages_fork: lengths and lengths_out partly overlap");
-  const dim3 grid(a->num_seqs, (a->ld_tables + kShare - 1) / kShare);
-  pages_share_kernel<<<grid, 256, 0, stream>>>(*a);
-  DTREE_LAUNCH_CHECK("pages_fork share launch");
-  pages_take_kernel<<<1, kTake, 0, stream>>>(*a);
+  if (size <= kOneLaunch) {
+    pages_take_kernel<true><<<1, kTake, 0, stream>>>(*a);
+  } else {
+    const dim3 grid(a->num_seqs, (a->ld_tables + kShare - 1) / kShare);
+    pages_share_kernel<<<grid, 256, 0, stream>>>(*a);
+    DTREE_LAUNCH_CHECK("pages_fork share launch");
+    pages_take_kernel<false><<<1, kTake, 0, stream>>>(*a);
+  }
   DTREE_LAUNCH_CHECK("pages_fork take launch");
   return DTREE_OK;
 }

@@ -60,7 +60,7 @@ class Select:
     def check(self, out=None, exact=False, inputs=None):
         out = {k: v.cpu().numpy() for k, v in (out or self.out).items()}
         scores, lengths, finished = inputs or self.want()
-        x = self.logits[:, :self.V].float().cpu().numpy()
+        x = self.logits[:, :self.V].float().nan_to_num(nan=float("-inf"), posinf=float("inf"), neginf=float("-inf")).cpu().numpy()
         ref = ob.select(x, scores, lengths, finished, self.G, self.K, self.M, self.eos, self.pad, self.penalty)
         if exact:
             for k in ("tokens", "parents", "lengths", "finished", "sources"):
@@ -190,12 +190,30 @@ def test_masked_rows_infinities_and_nan(gpu_device):
     x[12:16, 5:] = -torch.finfo(torch.float32).max
     x[13] = float("nan")
     x[16, 10] = 3e38; x[17, 11] = -3e38
+    x[18].view(torch.int32)[5::7] = 0x7F800001  # signalling NaNs, of both signs
+    x[18].view(torch.int32)[6::7] = -8388607
     s = Select(gpu_device, G, K, M, V, x, scores_of(G * K, 12))
     s.run()
     s.check()
     assert (s.out["tokens"][0] == -1).all()
-    top = s.out["tokens"][2].cpu().tolist()
-    assert {100, 4200} <= set(top)
+    b = Select(gpu_device, G, K, M, V, x.bfloat16(), scores_of(G * K, 12))
+    b.logits[18].view(torch.int16)[5::7] = 0x7F81
+    b.logits[18].view(torch.int16)[6::7] = -127
+    b.run()
+    b.check()
+
+
+def test_huge_logits(gpu_device):
+    """Rows around 1e30 and at fp32's ends, where differences alone say anything."""
+    G, K, M, V = 1, 5, 20, 9001
+    x = rows(gpu_device, G * K, V, seed=31)
+    x[1] = x[1] * 1e37
+    x[2] = x[2] * 1e-38
+    x[3] = torch.finfo(torch.float32).max
+    x[4] = -3e38
+    s = Select(gpu_device, G, K, M, V, x, [0.0, -3.0, -1.0, -2.0, -2.5])
+    s.run()
+    s.check()
 
 
 def test_beams_without_a_score(gpu_device):
