@@ -30,6 +30,7 @@ constexpr int kOneLaunch = 8192;      // table entries that the take workgroup s
 constexpr int kRun = 32;              // neighbouring counts of a thread in one round
 constexpr int kRound = kTake * kRun;
 constexpr int kList = 4096;           // free pages listed at a time
+constexpr int kHash = 2 * kMaxSeqs;
 constexpr int kHalfPage = DTREE_PAGE / 2;
 
 __device__ __forceinline__ int fork_parent(const DtreePagesFork& a, int i) {
@@ -101,28 +102,36 @@ __device__ __forceinline__ int block_scan(int v, int* waves, int& all) {
   return inc - v + (wave ? __builtin_amdgcn_readlane(w, wave - 1) : 0);
 }
 
-// The free pages among the kRun counts from `first` on, a bit each.
-__device__ __forceinline__ uint32_t free_pages(const DtreePagesFork& a, int64_t first) {
+// The kRun counts from `first` on (past the last page, the last one's), and the free
+// pages among them, a bit each.
+struct Counts {
   int c[kRun];
+};
+__device__ __forceinline__ Counts load_counts(const DtreePagesFork& a, int64_t first) {
+  Counts r;
   if (first + kRun <= a.num_pages) {
-    __builtin_memcpy(c, a.refs + first, sizeof(c));
-  } else {
+    __builtin_memcpy(r.c, a.refs + first, sizeof(r.c));
+  } else if (first < a.num_pages) {
 #pragma unroll
-    for (int e = 0; e < kRun; ++e) c[e] = a.refs[min(first + e, (int64_t)a.num_pages - 1)];
-#pragma unroll
-    for (int e = 0; e < kRun; ++e) c[e] |= first + e >= a.num_pages;
+    for (int e = 0; e < kRun; ++e) r.c[e] = a.refs[min(first + e, (int64_t)a.num_pages - 1)];
   }
+  return r;
+}
+__device__ __forceinline__ uint32_t free_pages(const DtreePagesFork& a, int64_t first, const Counts& r) {
+  const int64_t left = a.num_pages - first, keep = a.absent - first;
+  if (left <= 0) return 0;
   uint32_t mask = 0;
 #pragma unroll
-  for (int e = 0; e < kRun; ++e) mask |= c[e] == 0 ? 1u << e : 0u;
-  const int64_t keep = a.absent - first;
+  for (int e = 0; e < kRun; ++e) mask |= r.c[e] == 0 ? 1u << e : 0u;
+  if (left < kRun) mask &= (1u << left) - 1;
   return keep >= 0 && keep < kRun ? mask & ~(1u << keep) : mask;
 }
 
 template <bool ONE>
 __global__ __launch_bounds__(kTake) void pages_take_kernel(DtreePagesFork a) {
   __shared__ int waves[2][kTakeWaves];
-  __shared__ __attribute__((aligned(16))) int writes[kMaxSeqs];  // the shared page that a sequence is about to write, -1
+  __shared__ int got[kMaxSeqs];          // the page that a copying sequence took
+  __shared__ int pages[kHash], writers[kHash], latest[kHash];  // shared pages about to be written
   __shared__ int start[kMaxSeqs];        // pages wanted before a sequence's
   __shared__ int first[kMaxSeqs];        // its table entry of the first page past its length; copies: complemented
   __shared__ int list[kList];            // free pages, ascending
@@ -133,11 +142,17 @@ __global__ __launch_bounds__(kTake) void pages_take_kernel(DtreePagesFork a) {
   const int64_t mine = (int64_t)i * kRun;
   // (no count becomes or stops being 0 before the pages are taken: a copied page has
   // another holder)
-  uint32_t mask = 0;
-  if constexpr (!ONE) mask = mine < a.num_pages ? free_pages(a, mine) : 0;
+  Counts counts;
+  if constexpr (!ONE) counts = load_counts(a, mine);
   const int par = in ? fork_parent(a, i) : -1;
   const int L = par >= 0 ? fork_length(a, par) : 0;
   if (i == 0) past = fewer = 0;
+#pragma unroll
+  for (int h = i; h < kHash; h += kTake) {
+    pages[h] = -1;
+    writers[h] = 0;
+    latest[h] = -1;
+  }
   if constexpr (ONE) {
     const int own = in ? fork_length(a, i) : 0;
     kids[i] = a.parents ? 0 : 1;
@@ -158,7 +173,7 @@ __global__ __launch_bounds__(kTake) void pages_take_kernel(DtreePagesFork a) {
   }
   __syncthreads();  // (every length is read: lengths_out may be lengths)
   // (this launch has read no count before: none is in this CU's cache)
-  if constexpr (ONE) mask = mine < a.num_pages ? free_pages(a, mine) : 0;
+  if constexpr (ONE) counts = load_counts(a, mine);
   const int covered = (L + DTREE_PAGE - 1) / DTREE_PAGE, at = L / DTREE_PAGE;
   const int64_t wanted = in ? ((int64_t)L + a.rows + DTREE_PAGE - 1) / DTREE_PAGE : 0;
   const int last = (int)min(wanted, (int64_t)a.ld_tables);
@@ -170,25 +185,24 @@ __global__ __launch_bounds__(kTake) void pages_take_kernel(DtreePagesFork a) {
     page = row[at];
     if (is_page(a, page)) holders = a.refs[page];
   }
-  writes[i] = holders > 1 ? page : -1;
-  __syncthreads();
-  // Writers of one page, in ascending order: the k-th copies where others are left.
-  bool copy = false;
-  if (__any(holders > 1)) {
-    int k = 0, writers = 0;
-    const int4* w4 = reinterpret_cast<const int4*>(writes);
-#pragma unroll 4
-    for (int j = 0; j < (n + 3) / 4; ++j) {
-      const int4 w = w4[j];
-      const int c[4] = {w.x == page, w.y == page, w.z == page, w.w == page};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        writers += c[e];
-        k += 4 * j + e < i ? c[e] : 0;
-      }
+  // Writers of one page: all copy if others hold it too, else all but the latest.
+  uint32_t h = (uint32_t)page * 2654435761u >> 21;
+  static_assert(kHash == 1 << 11, "the hash keeps 11 bits");
+  if (holders > 1) {
+    for (;; h = (h + 1) % kHash) {
+      const int old = atomicCAS(&pages[h], -1, page);
+      if (old == -1 || old == page) break;
     }
-    copy = holders > 1 && holders - k > 1;
-    if (copy && k == 0) a.refs[page] = holders - min(writers, holders - 1);
+    atomicAdd(&writers[h], 1);
+    atomicMax(&latest[h], i);
+  }
+  uint32_t mask = free_pages(a, mine, counts);
+  __syncthreads();
+  bool copy = false;
+  if (holders > 1) {
+    const int leave = min(writers[h], holders - 1);
+    copy = leave == writers[h] || latest[h] != i;
+    if (latest[h] == i) a.refs[page] = holders - leave;
   }
   if (copy) row[at] = a.absent;  // (until it has a page of its own)
   int total, copies;
@@ -200,7 +214,7 @@ __global__ __launch_bounds__(kTake) void pages_take_kernel(DtreePagesFork a) {
   // The free pages in ascending order, kList at a time.
   int seen = 0;  // free pages of the rounds before
   for (int64_t base = 0; base < a.num_pages && seen < total; base += kRound) {
-    if (base) mask = base + mine < a.num_pages ? free_pages(a, base + mine) : 0;
+    if (base) mask = free_pages(a, base + mine, load_counts(a, base + mine));
     int all;
     __syncthreads();
     int rank = seen + block_scan(__popc(mask), waves[0], all);
@@ -223,7 +237,7 @@ __global__ __launch_bounds__(kTake) void pages_take_kernel(DtreePagesFork a) {
         const int f = first[lo], j = r - start[lo], pg = list[r - r0];
         // a copy takes the sequence's first page, for the entry before its new ones
         a.tables_out[(size_t)lo * a.ld_tables + (f < 0 ? ~f + j - 1 : f + j)] = pg;
-        if (f < 0 && j == 0) writes[lo] = pg;
+        if (f < 0 && j == 0) got[lo] = pg;
         a.refs[pg] = 1;
       }
       __syncthreads();
@@ -240,7 +254,7 @@ __global__ __launch_bounds__(kTake) void pages_take_kernel(DtreePagesFork a) {
   if (a.copies) {
     if (made) {
       a.copies[3 * spot] = page;
-      a.copies[3 * spot + 1] = writes[i];
+      a.copies[3 * spot + 1] = got[i];
       a.copies[3 * spot + 2] = L % DTREE_PAGE;
     }
     if (in && i >= copies) {
