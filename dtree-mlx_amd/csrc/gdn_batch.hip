@@ -4,7 +4,7 @@
 //
 // S' = g S + beta (v - g S k) k^T,  y = S' q = g S q + beta (v - g S k) (k . q):
 // both products need the old state alone, so it is read once, into registers, and
-// written once. A workgroup owns a (sequence, value head): 64 KB of state in 256
+// written once. A workgroup owns a (sequence, value head): 64 KB of state in 512
 // threads, 16 rows of 4 columns each, so a row's products are sums over 32 lanes. The
 // state's loads go out first; the convolution, the norms of q and k and the gates are
 // computed behind them (a key head's q and k by each of its value heads). The gated
@@ -19,7 +19,7 @@ namespace dtree {
 namespace {
 
 constexpr int D = 128;
-constexpr int kThreads = 256;
+constexpr int kThreads = 512;
 constexpr int kRows = D / (kThreads / 32);  // state rows of a thread
 
 struct BatchParams {
@@ -49,34 +49,53 @@ __global__ __launch_bounds__(kThreads) void gdn_batch_kernel(BatchParams p) {
   }
   int src = p.sources ? p.sources[b] : b;
   src = src >= 0 && src < p.seqs ? src : -1;  // -1: a sequence that begins
-  const size_t head = (size_t)h * D * D;
-  f32x4_t s[kRows];
-  {
-    const float* st = a.state + (size_t)max(src, 0) * Hv * D * D + head + r0 * D + c4;
-#pragma unroll
-    for (int i = 0; i < kRows; ++i) s[i] = src >= 0 ? ld4(st + i * (kThreads / 32) * D) : f32x4_t{0.f, 0.f, 0.f, 0.f};
-  }
+  // Everything that does not wait for another load, the gates and the gated norm's
+  // operands first, then the state.
   const float* proj = a.proj + (size_t)b * a.ld_proj;
-  if (tid < 96) {
-    const int part = tid >> 5;  // q, k, v
-    const int c = (part == 2 ? 2 * p.key_dim + h * D : part * p.key_dim + hk * D) + c4;
-    const float* win = a.window + (size_t)max(src, 0) * KEEP * p.C + c;
-    float* wout = a.window_out + (size_t)b * KEEP * p.C + c;
-    const bool writes = part == 2 || h % per == 0;
-    f32x4_t x[KEEP + 1], w[KEEP + 1];
-#pragma unroll
-    for (int r = 0; r < KEEP; ++r) x[r] = src >= 0 ? ld4(win + (size_t)r * p.C) : f32x4_t{0.f, 0.f, 0.f, 0.f};
+  const float* gates = proj + p.C + (size_t)Hv * D;
+  const float gate_a = gates[Hv + h] + a.dt_bias[h], gate_b = gates[h], a_log = a.A_log[h];
+  f32x4_t z = {0.f, 0.f, 0.f, 0.f};
+  u32x2_t nw = {0, 0};
+  if (tid < 32) {
+    z = ld4(proj + p.C + h * D + c4);
+    __builtin_memcpy(&nw, a.norm_w + c4, 8);
+  }
+  constexpr int kStep = kThreads / 32;  // rows between a thread's
+  const size_t head = (size_t)h * D * D;
+  const int part = tid >> 5;  // q, k, v of the first 96 threads
+  const int c = (part == 2 ? 2 * p.key_dim + h * D : part * p.key_dim + hk * D) + c4;
+  f32x4_t s[kRows], x[KEEP + 1], w[KEEP + 1];
+  if (part < 3) {
     x[KEEP] = ld4(proj + c);
 #pragma unroll
     for (int r = 0; r <= KEEP; ++r) w[r] = ld4(a.conv_w + (size_t)r * p.C + c);
+  }
+  if (src >= 0) {
+    if (part < 3) {
+      const float* win = a.window + (size_t)src * KEEP * p.C + c;
+#pragma unroll
+      for (int r = 0; r < KEEP; ++r) x[r] = ld4(win + (size_t)r * p.C);
+    }
+    const float* st = a.state + (size_t)src * Hv * D * D + head + r0 * D + c4;
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) s[i] = ld4(st + i * kStep * D);
+  } else {
+#pragma unroll
+    for (int r = 0; r < KEEP; ++r) x[r] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) s[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
+  if (part < 3) {
     f32x4_t y = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int r = 0; r <= KEEP; ++r)
 #pragma unroll
       for (int e = 0; e < 4; ++e) y[e] = fmaf(x[r][e], w[r][e], y[e]);
-    if (writes)
+    if (part == 2 || h % per == 0) {
+      float* wout = a.window_out + (size_t)b * KEEP * p.C + c;
 #pragma unroll
       for (int r = 0; r < KEEP; ++r) *reinterpret_cast<f32x4_t*>(wout + (size_t)r * p.C) = x[r + 1];
+    }
 #pragma unroll
     for (int e = 0; e < 4; ++e) y[e] = silu_f(y[e]);
     const float ss = row_sum32(dot4(y, y));
@@ -85,31 +104,46 @@ __global__ __launch_bounds__(kThreads) void gdn_batch_kernel(BatchParams p) {
     for (int e = 0; e < 4; ++e) y[e] *= f;
     *reinterpret_cast<f32x4_t*>(&qkv[part][c4]) = y;
   }
-  const float* gates = proj + p.C + (size_t)Hv * D;
-  const float t = gates[Hv + h] + a.dt_bias[h];
-  const float g = expf(-expf(a.A_log[h]) * (t > 20.f ? t : log1pf(expf(t))));
-  const float beta = 1.f / (1.f + expf(-gates[h]));
-  __syncthreads();
+  const float g = expf(-expf(a_log) * (gate_a > 20.f ? gate_a : log1pf(expf(gate_a))));
+  const float beta = 1.f / (1.f + expf(-gate_b));
+  lds_barrier();  // (the state's loads stay in flight)
   const f32x4_t q = ld4(&qkv[0][c4]), k = ld4(&qkv[1][c4]);
   const float kq = row_sum32(dot4(k, q));
   float* st = a.state_out + (size_t)b * Hv * D * D + head + r0 * D + c4;
+  // Four rows at a time: their sums over 32 lanes are independent chains.
+  constexpr int kTogether = 4;
+  static_assert(kRows % kTogether == 0, "whole groups of rows");
 #pragma unroll
-  for (int i = 0; i < kRows; ++i) {
-    const int r = r0 + i * (kThreads / 32);
-    const float sk = row_sum32(dot4(s[i], k)), sq = row_sum32(dot4(s[i], q));
-    const float delta = (qkv[2][r] - g * sk) * beta;
+  for (int i0 = 0; i0 < kRows; i0 += kTogether) {
+    float sk[kTogether], sq[kTogether];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) s[i][e] = fmaf(delta, k[e], g * s[i][e]);
-    *reinterpret_cast<f32x4_t*>(st + i * (kThreads / 32) * D) = s[i];
-    if ((tid & 31) == 0) ys[r] = fmaf(delta, kq, g * sq);
+    for (int j = 0; j < kTogether; ++j) {
+      sk[j] = dot4(s[i0 + j], k);
+      sq[j] = dot4(s[i0 + j], q);
+    }
+#pragma unroll
+    for (int j = 0; j < kTogether; ++j) {
+      sk[j] = row_sum32(sk[j]);
+      sq[j] = row_sum32(sq[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < kTogether; ++j) {
+      const int r = r0 + (i0 + j) * kStep;
+      const float delta = (qkv[2][r] - g * sk[j]) * beta;
+      f32x4_t& v = s[i0 + j];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = fmaf(delta, k[e], g * v[e]);
+      __builtin_nontemporal_store(v, reinterpret_cast<f32x4_t*>(st + (i0 + j) * kStep * D));
+      if ((tid & 31) == 0) ys[r] = fmaf(delta, kq, g * sq[j]);
+    }
   }
-  __syncthreads();
+  lds_barrier();  // (the new state's stores retire behind it)
   if (tid < 32) {
-    const f32x4_t y = ld4(&ys[c4]), z = ld4(proj + p.C + h * D + c4);
+    const f32x4_t y = ld4(&ys[c4]);
     const float rs = rsqrtf(row_sum32(dot4(y, y)) * (1.f / D) + a.eps);
     float o[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = y[e] * rs * bf2f(a.norm_w[c4 + e]) * silu_f(z[e]);
+    for (int e = 0; e < 4; ++e) o[e] = y[e] * rs * __uint_as_float((e & 1) ? nw[e >> 1] & 0xffff0000u : nw[e >> 1] << 16) * silu_f(z[e]);
     store_act4(a.out, a.out_lo, oi, o, h16);
   }
 }
