@@ -18,6 +18,7 @@ from typing import Any
 import torch
 
 from .adapters import LoadedTargetModel, load_target_model
+from .beam import beam_generate
 from .dtree_runtime import dtree_generate
 from .runtime import dflash_generate
 
@@ -46,7 +47,8 @@ def _resolve_draft(spec, target: LoadedTargetModel, seed: int, quant_bits: int |
 
 class DFlashGenerator:
     """api.py:29-170: owns a target and a drafter, dispatches generate calls to
-    dflash_generate (linear verify) or dtree_generate (tree verify)."""
+    dflash_generate (linear verify), dtree_generate (tree verify) or
+    beam_generate (decode_mode "beam": on the 8-bit cache, target_kv_bits=8)."""
 
     def __init__(self, target_model=DEFAULT_TARGET_MODEL, draft_model=DEFAULT_DRAFT_MODEL,
                  draft_attention_mask: str = "auto", target_quant_bits: int | None = None,
@@ -101,7 +103,8 @@ class DFlashGenerator:
                              speculative_tokens: int | None = None, decode_mode: str = "dflash",
                              tree_budget: int | None = None, verify_mode: str = "parallel-replay",
                              verify_chunk_size: int = 4, reset_peak_memory: bool = True,
-                             skip_special_tokens: bool = False, profile: bool = False) -> DFlashResult:
+                             skip_special_tokens: bool = False, profile: bool = False, num_beams: int = 4,
+                             length_penalty: float = 1.0) -> DFlashResult:
         if reset_peak_memory and torch.cuda.is_available():
             torch.cuda.reset_peak_memory_stats()
         if decode_mode == "dflash":
@@ -116,8 +119,15 @@ class DFlashGenerator:
                 temperature=temperature, stop_token_ids=self.target.stop_token_ids(), layer_ids=self._layer_ids(),
                 speculative_tokens=speculative_tokens, tree_budget=tree_budget, verify_mode=verify_mode,
                 profile=profile)
+        elif decode_mode == "beam":
+            # beam search of the target alone (no drafter): the best of num_beams hypotheses
+            prompt = [int(t) for t in torch.as_tensor(prompt_tokens).reshape(-1).tolist()]
+            (best,), metrics = beam_generate(self.target, [prompt], num_beams=num_beams, max_new_tokens=max_new_tokens,
+                                             length_penalty=length_penalty)
+            output_tokens = prompt + best[0].tokens
+            metrics["hypotheses"] = best
         else:
-            raise ValueError(f"Unknown decode_mode={decode_mode!r}. Expected 'dflash' or 'dtree'.")
+            raise ValueError(f"Unknown decode_mode={decode_mode!r}. Expected 'dflash', 'dtree' or 'beam'.")
         generated_tokens = output_tokens[metrics["num_input_tokens"]:]
         tok = self.target.tokenizer
         text = tok.decode(generated_tokens, skip_special_tokens=skip_special_tokens) if tok is not None else ""
@@ -127,12 +137,14 @@ class DFlashGenerator:
     def generate(self, prompt_text: str, max_new_tokens: int = 256, temperature: float = 0.0,
                  speculative_tokens: int | None = None, decode_mode: str = "dflash", tree_budget: int | None = None,
                  verify_mode: str = "parallel-replay", verify_chunk_size: int = 4, reset_peak_memory: bool = True,
-                 skip_special_tokens: bool = False, profile: bool = False) -> DFlashResult:
+                 skip_special_tokens: bool = False, profile: bool = False, num_beams: int = 4,
+                 length_penalty: float = 1.0) -> DFlashResult:
         return self.generate_from_tokens(
             prompt_tokens=self.encode_prompt(prompt_text), max_new_tokens=max_new_tokens, temperature=temperature,
             speculative_tokens=speculative_tokens, decode_mode=decode_mode, tree_budget=tree_budget,
             verify_mode=verify_mode, verify_chunk_size=verify_chunk_size, reset_peak_memory=reset_peak_memory,
-            skip_special_tokens=skip_special_tokens, profile=profile)
+            skip_special_tokens=skip_special_tokens, profile=profile, num_beams=num_beams,
+            length_penalty=length_penalty)
 
 
 # Method-agnostic alias (api.py:170).

@@ -25,6 +25,7 @@ import torch
 from . import _native as N
 from .cache import PagedKVCache, PagedKVCacheQ8
 from .config import Qwen3Config
+from .pool import HypothesisCache, PagedKVPool
 from .weights import W_TILED, W_TILED_F16, Q4Linear, Qwen3Weights, tile_weight, tile_weight_f16
 
 
@@ -492,6 +493,34 @@ class TreeEngineBase:
         a.ancestors = d + N.StepDesc.ancestors.offset
         self._attention_q8(lw, kv, rec, a, self.qkv, self.q8_ws, st)
 
+    # ---- hypotheses side by side (beam.py) -----------------------------------------
+    # Row b of a step is hypothesis b's next token, at the position that is its length:
+    # each reads its own pages, and they share most of them.
+    def _hypotheses_attention(self, lw, cache: HypothesisCache, layer: int, st: int) -> None:
+        kv = cache.batches[cache.turn]
+        rec = kv.record(layer, cache.positions, cache.ones, cache.max_past, 1, cache.num_seqs)
+        a = self._q8_args(lw, self.qkv, self.rope_cos, self.rope_sin, self.attn, 0)
+        self._attention_q8(lw, kv, rec, a, self.qkv, cache.workspace, st)
+
+    def reserve_hypotheses(self, cache: HypothesisCache, longest: int) -> None:
+        """The attention's workspace for hypotheses of up to ``longest`` positions."""
+        a = N.AttnQ8Args()
+        a.num_heads = self.cfg.num_attention_heads
+        need = 16
+        for past in {self.attn_grid_past(min(b, longest)) for b in (*self.ATTN_GRID_PAST, longest)}:
+            rec = cache.batches[0].record(0, None, None, past, 1, cache.num_seqs)
+            need = max(need, self.lib.dtree_attention_q8_workspace_bytes(C.byref(rec), C.byref(a)))
+        cache.workspace = torch.empty(need, dtype=torch.uint8, device=self.dev)
+
+    def launch_hypotheses(self, cache: HypothesisCache, advance: int, st: int) -> None:
+        """One step: the caches of the hypotheses that are continued (forked from
+        ``cache.sources``, their lengths ``advance`` longer, with room for a row), the
+        layers over the rows of ``cache.desc``, and the LM head's logits."""
+        pos = cache.positions.data_ptr()
+        cache.pool.launch_fork(cache.turn, pos, pos, cache.sources.data_ptr(), 1, advance, st)
+        self.launch_forward(cache, st)
+        self.launch_lm_head(st, want_logits=True)
+
     def _prefill_workspace_q8(self, kv: PagedKVCacheQ8, past: int, tokens: int, seg: int) -> None:
         """Room for the key ranges of all of a prompt's segments, before its first
         row is written (a longer prefix may want more of it). Where the device has
@@ -795,9 +824,18 @@ class Qwen3TreeEngine(TreeEngineBase):
     def new_cache(self, page_order=None) -> PagedKVCache | PagedKVCacheQ8:
         return self._new_kv_cache(self.cfg.num_hidden_layers, self.max_past + self.max_nodes, page_order)
 
+    def new_pool(self, num_seqs: int, num_pages: int | None = None) -> PagedKVPool:
+        """A pool of ``num_seqs`` forkable sequences whose ``sequence(i)`` this engine
+        takes as its cache (each with its own prefix, most of it shared)."""
+        c = self.cfg
+        return PagedKVPool(c.num_hidden_layers, c.num_key_value_heads, c.head_dim, self.max_past + self.max_nodes,
+                           num_seqs, num_pages=num_pages, kv_bits=self.kv_bits, device=self.dev)
+
     def _attention(self, li, cache: PagedKVCache, st, write_cache=True):
         c = self.cfg
         lw = self.w.layers[li]
+        if isinstance(cache, HypothesisCache):
+            return self._hypotheses_attention(lw, cache, li, st)
         if self.kv_bits == 8:
             return self._tree_attention_q8(lw, cache, li, st, write_cache)
         a = N.AttnArgs()
@@ -818,12 +856,13 @@ class Qwen3TreeEngine(TreeEngineBase):
         """embed + all layers; tree K/V rows land in the cache at [P, P+L)."""
         c = self.cfg
         H = c.hidden_size
-        self._check_kv(cache)
-        if cache.capacity < self.max_past + self.max_nodes:
-            raise ValueError("cache capacity is smaller than max_past + max_nodes")
+        if not isinstance(cache, HypothesisCache):
+            self._check_kv(cache)
+            if cache.capacity < self.max_past + self.max_nodes:
+                raise ValueError("cache capacity is smaller than max_past + max_nodes")
         emb, emb_layout, emb_sb = self._embedding()
         N.check(self.lib.dtree_embed(
-            self.desc.data_ptr(), emb, emb_layout, emb_sb, c.vocab_size, H,
+            (cache.desc if isinstance(cache, HypothesisCache) else self.desc).data_ptr(), emb, emb_layout, emb_sb, c.vocab_size, H,
             self.w.layers[0].input_norm.data_ptr(),
             self.MP,
             self.x.data_ptr(), self.xg[0].data_ptr(), self.lo_ptr(self.xg), self.w.layout, self.ss.data_ptr(),

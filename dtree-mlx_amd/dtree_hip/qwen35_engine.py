@@ -32,6 +32,7 @@ import torch
 from . import _native as N
 from .cache import Qwen35Cache
 from .engine import TreeEngineBase
+from .pool import HypothesisCache
 from .weights import W_TILED, W_TILED_F16, GdnLayerWeights
 
 
@@ -83,7 +84,8 @@ class Qwen35TreeEngine(TreeEngineBase):
                            kv_bits=self.kv_bits)
 
     # ---- launches ----------------------------------------------------------------
-    def gdn_args(self, li: int, cache: Qwen35Cache) -> N.GdnArgs:
+    def gdn_args(self, li: int, cache: Qwen35Cache, window: torch.Tensor | None = None,
+                 state: torch.Tensor | None = None) -> N.GdnArgs:
         c = self.cfg
         gi = cache.slot[li]
         lw: GdnLayerWeights = self.w.layers[li]
@@ -93,9 +95,9 @@ class Qwen35TreeEngine(TreeEngineBase):
         a.head_k_dim = c.linear_key_head_dim; a.head_v_dim = c.linear_value_head_dim
         a.conv_keep = c.linear_conv_kernel_dim - 1
         a.proj = self.proj[gi].data_ptr(); a.ld_proj = c.in_proj_dim
-        a.window = cache.windows[gi].data_ptr(); a.conv_w = lw.conv_w.data_ptr()
+        a.window = (cache.windows[gi] if window is None else window).data_ptr(); a.conv_w = lw.conv_w.data_ptr()
         a.A_log = lw.A_log.data_ptr(); a.dt_bias = lw.dt_bias.data_ptr()
-        a.state = cache.states[gi].data_ptr()
+        a.state = (cache.states[gi] if state is None else state).data_ptr()
         a.q = self.gq[gi].data_ptr(); a.k = self.gk[gi].data_ptr(); a.v = self.gv[gi].data_ptr()
         a.g = self.gg[gi].data_ptr(); a.beta = self.gbeta[gi].data_ptr()
         a.y = self.gy.data_ptr()
@@ -108,6 +110,8 @@ class Qwen35TreeEngine(TreeEngineBase):
         c = self.cfg
         ai = cache.slot[li]
         lw = self.w.layers[li]
+        if isinstance(cache, HypothesisCache):
+            return self._hypotheses_attention(lw, cache, ai, st)
         kv = cache.kv
         if self.kv_bits == 8:
             return self._tree_attention_q8(lw, kv, ai, st, write_cache)
@@ -126,17 +130,31 @@ class Qwen35TreeEngine(TreeEngineBase):
         a.rope_dims = c.rope_dims; a.gated = 1
         N.check(self.lib.dtree_tree_attention(C.byref(a), st), "tree attention")
 
+    def _launch_gdn(self, li: int, cache: Qwen35Cache | HypothesisCache, st: int) -> None:
+        """A GatedDeltaNet layer's core over the rows in proj, into gout."""
+        if isinstance(cache, HypothesisCache):  # each row from its source's window and state
+            gi, t = cache.slot[li], cache.turn
+            ga = self.gdn_args(li, cache, cache.windows[t, gi], cache.states[t, gi])
+            ga.window_out = cache.windows[1 - t, gi].data_ptr(); ga.state_out = cache.states[1 - t, gi].data_ptr()
+            N.check(self.lib.dtree_gdn_layer_batch(C.byref(ga), cache.sources.data_ptr(), cache.num_seqs, st), "gdn batch")
+            return
+        ga = self.gdn_args(li, cache)
+        # one launch for trees of up to 32 nodes, else prep + recurrence
+        N.check(self.lib.dtree_gdn_layer_prep_recurrence(C.byref(ga), st), "gdn prep + recurrence")
+        N.check(self.lib.dtree_gdn_layer_gated_norm(C.byref(ga), st), "gdn gated norm")
+
     def launch_forward(self, cache: Qwen35Cache, st: int, norm_hidden: bool = False) -> None:
         """embed + all layers; attention-layer tree K/V land in the cache at
         [P, P + L); GatedDeltaNet per-node inputs stay in the layer buffers."""
         c = self.cfg
         H = c.hidden_size
-        self._check_kv(cache.kv)
-        if cache.capacity < self.max_past + self.max_nodes:
-            raise ValueError("cache capacity is smaller than max_past + max_nodes")
+        if not isinstance(cache, HypothesisCache):
+            self._check_kv(cache.kv)
+            if cache.capacity < self.max_past + self.max_nodes:
+                raise ValueError("cache capacity is smaller than max_past + max_nodes")
         emb, emb_layout, emb_sb = self._embedding()
         N.check(self.lib.dtree_embed(
-            self.desc.data_ptr(), emb, emb_layout, emb_sb, c.vocab_size, H,
+            (cache.desc if isinstance(cache, HypothesisCache) else self.desc).data_ptr(), emb, emb_layout, emb_sb, c.vocab_size, H,
             self.w.layers[0].input_norm.data_ptr(), self.MP,
             self.x.data_ptr(), self.xg[0].data_ptr(), self.lo_ptr(self.xg), self.w.layout, self.ss.data_ptr(),
             c.rope_dims, c.rope_theta, self.rope_cos.data_ptr(), self.rope_sin.data_ptr(), st), "embed")
@@ -148,10 +166,7 @@ class Qwen35TreeEngine(TreeEngineBase):
             if c.is_linear(li):
                 gi = cache.slot[li]
                 self._gemm("in", self.xg, H, lw.w_in, N.EPI_STORE_F32, st, ss_in=self.ss, out_f32=self.proj[gi])
-                ga = self.gdn_args(li, cache)
-                # one launch for trees of up to 32 nodes, else prep + recurrence
-                N.check(self.lib.dtree_gdn_layer_prep_recurrence(C.byref(ga), st), "gdn prep + recurrence")
-                N.check(self.lib.dtree_gdn_layer_gated_norm(C.byref(ga), st), "gdn gated norm")
+                self._launch_gdn(li, cache, st)
                 self._gemm("out", self.gout, c.value_dim, lw.w_out, N.EPI_RESIDUAL, st, out_f32=self.x,
                            out_bf16=self.xg, next_norm=lw.post_norm, ss_out=self.ss)
             else:
