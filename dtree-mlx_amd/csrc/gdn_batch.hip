@@ -164,6 +164,8 @@ extern "C" int dtree_gdn_layer_batch(const DtreeGdnArgs* a, const int32_t* sourc
                 "gdn_layer_batch: num_seqs in [1, rows_padded]");
   DTREE_REQUIRE(a->num_k_heads > 0 && a->num_v_heads > 0 && a->num_v_heads <= 256 && a->num_v_heads % a->num_k_heads == 0,
                 "gdn_layer_batch: num_v_heads % num_k_heads, at most 256");
+  DTREE_REQUIRE((int64_t)a->rows_padded * a->num_v_heads < (1 << 23),
+                "gdn_layer_batch: rows_padded * num_v_heads below 2^23 (2^32 work items)");
   DTREE_REQUIRE(a->head_k_dim == D && a->head_v_dim == D, "gdn_layer_batch: head dims 128 are compiled");
   DTREE_REQUIRE(a->conv_keep >= 1 && a->conv_keep <= 7, "gdn_layer_batch: conv_keep in [1, 7]");
   DTREE_REQUIRE(a->proj && a->window && a->conv_w && a->A_log && a->dt_bias && a->state && a->norm_w && a->out &&

@@ -116,6 +116,8 @@ class BeamDecoder:
 
     def start(self) -> None:
         """The prompts, one after another, and the first tokens."""
+        if self.made:
+            raise RuntimeError("the prompts have run: a decoder is used once")
         eng, cache = self.eng, self.cache
         cache.pool.start([len(p) for p in self.prompts])
         first = torch.empty(self.groups, eng.cfg.vocab_size, dtype=torch.float32, device=eng.dev)
@@ -153,10 +155,12 @@ class BeamDecoder:
         self._record()
 
     def _graph(self, advance: int) -> int:
-        key = (self.cache.turn, self.cache.max_past, advance)
+        # (a graph holds the engine's buffers: those of its hidden layers may change)
+        eng = self.eng
+        key = (self.cache.turn, self.cache.max_past, advance, tuple(eng.layer_ids), eng.hidden.data_ptr())
         if key not in self._graphs:
-            lib = self.eng.lib
-            side = torch.cuda.Stream(device=self.eng.dev)
+            lib = eng.lib
+            side = torch.cuda.Stream(device=eng.dev)
             side.wait_stream(torch.cuda.current_stream())
             N.check(lib.dtree_graph_begin(side.cuda_stream), "graph begin")
             ex = C.c_void_p()

@@ -798,7 +798,7 @@ int dtree_pages_copy(const DtreePagesCopy* args, hipStream_t stream);
  * [num_seqs][Hv][Dv][Dk], the new ones in buffers of their own. Rows num_seqs ..
  * rows_padded - 1 of out become zero; desc, q, k, v, g, beta and y are not used.
  * proj, conv_w, windows and states 16-byte aligned, ld_proj a multiple of 4.
- * Compiled for Dk = Dv = 128.
+ * Compiled for Dk = Dv = 128, up to 256 value heads; rows_padded * Hv below 2^23.
  */
 int dtree_gdn_layer_batch(const DtreeGdnArgs* args, const int32_t* sources, int32_t num_seqs, hipStream_t stream);
 

@@ -103,7 +103,7 @@ GDN = dict(rows_padded=32, num_k_heads=2, num_v_heads=4, head_k_dim=128, head_v_
 
 
 @pytest.mark.parametrize("kw,seqs,word", [
-    ({}, 0, "num_seqs"), ({}, 33, "num_seqs"), (dict(rows_padded=1 << 17), 4, "num_seqs"), (dict(num_k_heads=0), 4, "heads"),
+    (dict(rows_padded=1 << 16, num_v_heads=128), 4, "2^23"), ({}, 0, "num_seqs"), ({}, 33, "num_seqs"), (dict(rows_padded=1 << 17), 4, "num_seqs"), (dict(num_k_heads=0), 4, "heads"),
     (dict(num_v_heads=5), 4, "heads"), (dict(num_v_heads=512), 4, "heads"), (dict(head_k_dim=64), 4, "dims"),
     (dict(head_v_dim=256), 4, "dims"), (dict(conv_keep=0), 4, "conv_keep"), (dict(conv_keep=8), 4, "conv_keep"),
     (dict(ld_proj=1540), 4, "ld_proj"), (dict(ld_proj=2049), 4, "ld_proj"), (dict(proj=4100), 4, "aligned"),

@@ -102,6 +102,43 @@ def test_graphs_and_eager_steps_agree(gpu_device, family):
         assert [h[1] for h in hyps] == sorted((h[1] for h in hyps), reverse=True)
 
 
+def test_two_decoders_and_the_engines_own_steps_in_turns(gpu_device):
+    """Decoders interleaved with each other, with verify steps and with a change of the
+    engine's hidden layers (whose buffers a captured step holds)."""
+    target = _target("qwen3")
+    eng = target.model.engine
+    prompts = _prompts(target, (40, 90))
+    want = [beam_generate(target, [p], num_beams=4, max_new_tokens=9)[0][0] for p in prompts]
+    ds = [BeamDecoder(target, [p], 4, 9) for p in prompts]
+    for d in ds:
+        d.start()
+    cache = eng.new_cache()
+    eng.prefill(cache, prompts[0])
+    for k in range(8):
+        if k == 4:
+            eng.set_layer_ids([1])
+            junk = [torch.full((eng.MP, eng.cfg.hidden_size), 3.0, dtype=torch.bfloat16, device=gpu_device) for _ in range(8)]
+        for d in ds:
+            d.step()
+            _step(eng, cache, k)
+    assert all(bool((j == 3.0).all()) for j in junk)
+    for d, w in zip(ds, want):
+        assert [(h.tokens, h.score) for h in d.hypotheses()[0]] == [(h.tokens, h.score) for h in w]
+        with pytest.raises(RuntimeError, match="once"):
+            d.start()
+
+
+def test_another_stream(gpu_device):
+    target = _target("qwen3_5")
+    prompts = _prompts(target, (50,))
+    want, _ = beam_generate(target, prompts, num_beams=3, max_new_tokens=6)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got, _ = beam_generate(target, prompts, num_beams=3, max_new_tokens=6)
+    assert [h.tokens for h in got[0]] == [h.tokens for h in want[0]]
+
+
 def test_requests_beyond_the_engines_rows_run_in_turns(gpu_device):
     target = _target("qwen3")
     prompts = _prompts(target, (10, 20, 30, 40, 50))

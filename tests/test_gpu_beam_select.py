@@ -229,6 +229,27 @@ def test_beams_without_a_score(gpu_device):
     assert (s.out["parents"][2] == -1).all() and (s.out["parents"][0] == 0).all()
 
 
+@pytest.mark.parametrize("K,V", [(64, 266241), (5, 1 << 20), (3, (1 << 20) - 1)])
+def test_more_chunks_than_the_quick_way_takes_and_the_largest_vocabulary(gpu_device, K, V):
+    s = Select(gpu_device, 1, K, 64, V, rows(gpu_device, K, V, torch.bfloat16, seed=21), scores_of(K, 22))
+    s.run()
+    s.check()
+
+
+@pytest.mark.parametrize("score", [3.0e38, 1e30, 0.0, -1e30, -3.0e38])
+@pytest.mark.parametrize("penalty", [0.0, 2.0, -3.0])
+def test_scores_at_fp32s_ends(gpu_device, score, penalty):
+    """Ranks beyond fp32, and sums in which the logits are lost (all of a beam tie)."""
+    s = Select(gpu_device, 1, 3, 12, 5000, rows(gpu_device, 3, 5000, seed=23), [score, score * 0.5, score * 0.25],
+               lengths=[3, 9, 70], penalty=penalty)
+    out = {k: v.cpu() for k, v in s.run().items()}
+    scores, lengths, finished = s.want()
+    ref = ob.select(s.logits.cpu().numpy(), scores, lengths, finished, 1, 3, 12, -1, 0, penalty)
+    if abs(score) >= 1e30:  # (every sum of a beam rounds to its score: positions decide)
+        assert np.array_equal(out["tokens"].numpy(), ref["tokens"]) and np.array_equal(out["parents"].numpy(), ref["parents"])
+    assert np.allclose(out["scores"].double().numpy(), ref["scores"], rtol=2.0 ** -23, atol=2 * LSE)
+
+
 def test_rows_past_32_bit_offsets(gpu_device):
     G, K, V, ld = 33, 64, 90, 1 << 20  # 2112 rows, 2.2e9 elements apart
     x = torch.empty(G * K, ld, dtype=torch.bfloat16, device=gpu_device)
