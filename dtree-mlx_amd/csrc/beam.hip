@@ -93,10 +93,10 @@ __device__ __forceinline__ float logit(const DtreeBeamArgs& a, int row, int t) {
 }
 
 // v_med3_f32 itself: the compiler's median of a constant infinity is a minimum, which
-// gives the number for a NaN.
+// gives the number for a NaN. Volatile: it stays behind the mode's change below.
 __device__ __forceinline__ float median(float x, float low, float high) {
   float y;
-  asm("v_med3_f32 %0, %1, %2, %3" : "=v"(y) : "v"(x), "s"(low), "v"(high));
+  asm volatile("v_med3_f32 %0, %1, %2, %3" : "=v"(y) : "v"(x), "s"(low), "v"(high));
   return y;
 }
 

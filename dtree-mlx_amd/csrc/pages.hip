@@ -116,9 +116,19 @@ __device__ __forceinline__ int block_scan(int v, int* waves, int& all) {
 struct Counts {
   int c[kRun];
 };
+// ONE: this launch changed counts by atomics, which the loads have to see: past this
+// CU's cache, where a line may lie that other arrays share with the counts.
+template <bool ONE>
 __device__ __forceinline__ Counts load_counts(const DtreePagesFork& a, int64_t first) {
   Counts r;
-  if (first + kRun <= a.num_pages) {
+  if constexpr (ONE) {
+    if (first < a.num_pages) {
+      const int most = (int)min((int64_t)kRun, a.num_pages - first) - 1;
+#pragma unroll
+      for (int e = 0; e < kRun; ++e)
+        r.c[e] = __hip_atomic_load(a.refs + first + min(e, most), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    }
+  } else if (first + kRun <= a.num_pages) {
     __builtin_memcpy(r.c, a.refs + first, sizeof(r.c));
   } else if (first < a.num_pages) {
 #pragma unroll
@@ -152,7 +162,7 @@ __global__ __launch_bounds__(kTake) void pages_take_kernel(DtreePagesFork a) {
   // (no count becomes or stops being 0 before the pages are taken: a copied page has
   // another holder)
   Counts counts;
-  if constexpr (!ONE) counts = load_counts(a, mine);
+  if constexpr (!ONE) counts = load_counts<ONE>(a, mine);
   const int par = in ? fork_parent(a, i) : -1;
   const int L = par >= 0 ? fork_length(a, par) : 0;
   if (i == 0) past = fewer = 0;
@@ -181,8 +191,7 @@ __global__ __launch_bounds__(kTake) void pages_take_kernel(DtreePagesFork a) {
     wait_stores_done();  // (the counts' changes too)
   }
   __syncthreads();  // (every length is read: lengths_out may be lengths)
-  // (this launch has read no count before: none is in this CU's cache)
-  if constexpr (ONE) counts = load_counts(a, mine);
+  if constexpr (ONE) counts = load_counts<ONE>(a, mine);
   const int covered = (L + DTREE_PAGE - 1) / DTREE_PAGE, at = L / DTREE_PAGE;
   const int64_t wanted = in ? ((int64_t)L + a.rows + DTREE_PAGE - 1) / DTREE_PAGE : 0;
   const int last = (int)min(wanted, (int64_t)a.ld_tables);
@@ -192,7 +201,7 @@ __global__ __launch_bounds__(kTake) void pages_take_kernel(DtreePagesFork a) {
   int page = -1, holders = 0;
   if (in && a.rows > 0 && L % DTREE_PAGE) {
     page = row[at];
-    if (is_page(a, page)) holders = a.refs[page];
+    if (is_page(a, page)) holders = ONE ? __hip_atomic_load(a.refs + page, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP) : a.refs[page];
   }
   // Writers of one page: all copy if others hold it too, else all but the latest.
   uint32_t h = (uint32_t)page * 2654435761u >> 21;
@@ -223,7 +232,7 @@ __global__ __launch_bounds__(kTake) void pages_take_kernel(DtreePagesFork a) {
   // The free pages in ascending order, kList at a time.
   int seen = 0;  // free pages of the rounds before
   for (int64_t base = 0; base < a.num_pages && seen < total; base += kRound) {
-    if (base) mask = free_pages(a, base + mine, load_counts(a, base + mine));
+    if (base) mask = free_pages(a, base + mine, load_counts<ONE>(a, base + mine));
     int all;
     __syncthreads();
     int rank = seen + block_scan(__popc(mask), waves[0], all);

@@ -108,7 +108,8 @@ class PagedKVPool:
 
     def fork(self, parents=None, rows: int = 0) -> None:
         """Sequence i continues sequence parents[i] (-1: empty; None: itself), with room
-        for ``rows`` more positions. Raises if the pool has no pages left for that."""
+        for ``rows`` more positions. Raises if the pool has no pages left for that; the
+        sequences that found none have lost rows then, and the pool is to be started anew."""
         old = self.lengths
         if parents is None:
             src, new = None, old

@@ -133,3 +133,14 @@ def test_oracle_fork_by_hand():
                                                      [100, 0, 0], [0, 0, -1], 0, 1)
     assert tables.tolist() == [[0, 2, -1], [0, 1, -1], [3, -1, -1]] and copies == [(1, 2, 36)]
     assert refs.tolist() == [2, 1, 1, 1, 0, 0] and lengths.tolist() == [100, 100, 0] and missing == 0
+
+
+def test_kernels_use_no_scratch():
+    from test_kernel_scratch import _code_objects, _kernels
+
+    if not N.LIB_PATH.exists():
+        pytest.skip("library not built")
+    names = ("beam_scan", "beam_pick", "pages_share", "pages_take", "pages_copy", "gdn_batch")
+    mine = [k for o in _code_objects(N.LIB_PATH.read_bytes()) for k in _kernels(o) if any(n in k[".name"] for n in names)]
+    assert len(mine) == 4 + 1 + 2 + 1 + 7
+    assert [k[".name"] for k in mine if k[".private_segment_fixed_size"]] == []

@@ -159,6 +159,41 @@ def test_parents_and_tables_that_are_not_there(gpu_device):
     p.fork([0, 1, 1, 0], rows=0)
 
 
+@pytest.mark.parametrize("ld,pages", [(7, 40), (7, 3000), (900, 9000)])
+def test_arrays_side_by_side_in_memory(gpu_device, ld, pages):
+    """One allocation holds all arrays, so that neighbours share cache lines with the counts
+    that the launch changes and then reads (forks of one launch and of two)."""
+    n = 12
+    p = Pool(gpu_device, n, ld, pages, seed=ld).fill([200, 64, 130, 400, 1, 0, 63])
+    sizes = dict(parents=n, lengths=n, refs=pages, out=n, tables=n * ld, tables_out=n * ld, copies=3 * n, status=2)
+    flat = torch.zeros(sum(sizes.values()), dtype=torch.int32, device=gpu_device)
+    at, view = 0, {}
+    for k, m in sizes.items():
+        view[k] = flat[at:at + m]
+        at += m
+    g = np.random.default_rng(ld)
+    for k in range(6):
+        parents = g.integers(-1, 7 if k == 0 else n, n)
+        for name, x in (("parents", parents), ("lengths", p.lengths), ("refs", p.refs), ("tables", p.tables.reshape(-1))):
+            view[name].copy_(torch.as_tensor(np.asarray(x, np.int32)))
+        view["status"].zero_()
+        a = N.PagesFork()
+        a.refs = view["refs"].data_ptr(); a.num_pages = pages; a.num_seqs = n; a.ld_tables = ld
+        a.tables = view["tables"].data_ptr(); a.tables_out = view["tables_out"].data_ptr()
+        a.lengths = view["lengths"].data_ptr(); a.lengths_out = view["out"].data_ptr()
+        a.parents = view["parents"].data_ptr(); a.advance = 1; a.rows = 5; a.absent = -1
+        a.copies = view["copies"].data_ptr(); a.status = view["status"].data_ptr()
+        N.check(N.lib().dtree_pages_fork(C.byref(a), stream()), "fork")
+        torch.cuda.synchronize()
+        ref = ob.fork(p.refs, p.tables, p.lengths, parents, 1, 5)
+        assert np.array_equal(view["refs"].cpu().numpy(), ref[0])
+        assert np.array_equal(view["tables_out"].cpu().numpy().reshape(n, ld), ref[1])
+        assert np.array_equal(view["out"].cpu().numpy(), ref[2])
+        assert [tuple(c) for c in view["copies"].view(n, 3)[:len(ref[3])].tolist()] == ref[3]
+        assert view["status"].tolist() == [ref[4], len(ref[3])]
+        p.refs, p.tables, p.lengths = ref[:3]
+
+
 def kv(dev, layers, pages, heads, dim, bits, seed):
     g = torch.Generator(device=dev).manual_seed(seed)
     if bits == 16:
