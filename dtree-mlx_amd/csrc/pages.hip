@@ -105,7 +105,7 @@ __device__ __forceinline__ int wave_scan(int v) {
 __device__ __forceinline__ int block_scan(int v, int* waves, int& all) {
   const int wave = threadIdx.x >> 6, inc = wave_scan(v);
   if ((threadIdx.x & 63) == 63) waves[wave] = inc;
-  __syncthreads();
+  lds_barrier();
   const int w = wave_scan((threadIdx.x & 63) < kTakeWaves ? waves[threadIdx.x & 63] : 0);
   all = __builtin_amdgcn_readlane(w, kTakeWaves - 1);
   return inc - v + (wave ? __builtin_amdgcn_readlane(w, wave - 1) : 0);
@@ -222,7 +222,6 @@ __global__ __launch_bounds__(kTake) void pages_take_kernel(DtreePagesFork a) {
     copy = leave == writers[h] || latest[h] != i;
     if (latest[h] == i) a.refs[page] = holders - leave;
   }
-  if (copy) row[at] = a.absent;  // (until it has a page of its own)
   int total, copies;
   const int grow = in ? max(last - covered, 0) : 0;
   const int before = block_scan((copy ? 1 : 0) + grow, waves[0], total);
@@ -234,7 +233,7 @@ __global__ __launch_bounds__(kTake) void pages_take_kernel(DtreePagesFork a) {
   for (int64_t base = 0; base < a.num_pages && seen < total; base += kRound) {
     if (base) mask = free_pages(a, base + mine, load_counts<ONE>(a, base + mine));
     int all;
-    __syncthreads();
+    lds_barrier();
     int rank = seen + block_scan(__popc(mask), waves[0], all);
     const int end = min(total, seen + all);
     for (int r0 = seen; r0 < end; r0 += kList) {
@@ -244,7 +243,7 @@ __global__ __launch_bounds__(kTake) void pages_take_kernel(DtreePagesFork a) {
         mask &= mask - 1;
         ++rank;
       }
-      __syncthreads();
+      lds_barrier();
       for (int r = r0 + i; r < upto; r += kTake) {
         int lo = 0, hi = n;  // the last sequence whose range starts at r or before: the one that holds r
         while (hi - lo > 1) {
@@ -258,14 +257,17 @@ __global__ __launch_bounds__(kTake) void pages_take_kernel(DtreePagesFork a) {
         if (f < 0 && j == 0) got[lo] = pg;
         a.refs[pg] = 1;
       }
-      __syncthreads();
+      lds_barrier();
     }
     seen += all;
   }
   // the copies, by sequence; without pages for all of them, those before some sequence
   const bool made = copy && before < seen;
   if (seen < total) {
-    if (copy && !made) atomicAdd(&fewer, 1);
+    if (copy && !made) {
+      atomicAdd(&fewer, 1);
+      row[at] = a.absent;
+    }
     __syncthreads();
     copies -= fewer;
   }
@@ -287,9 +289,14 @@ __global__ __launch_bounds__(kTake) void pages_take_kernel(DtreePagesFork a) {
   }
 }
 
+// 16-byte pieces of a unit's blocks in all pools, one after the other; a thread's loads
+// of kFlight pieces go out before their first store.
 __global__ __launch_bounds__(256) void pages_copy_kernel(DtreePagesCopy a) {
+  constexpr int kFlight = 4;
   __shared__ int ends;  // the list's first negative source
   const int tid = threadIdx.x, per = a.layers * a.num_heads;
+  int u = blockIdx.x;
+  int src = a.copies[3 * (u / per)], dst = a.copies[3 * (u / per) + 1], used = a.copies[3 * (u / per) + 2];
   if (tid == 0) ends = a.max_copies;
   __syncthreads();
   for (int c = tid; c < a.max_copies; c += 256)
@@ -299,20 +306,41 @@ __global__ __launch_bounds__(256) void pages_copy_kernel(DtreePagesCopy a) {
     }
   __syncthreads();
   const int units = ends * per;
-  for (int u = blockIdx.x; u < units; u += gridDim.x) {
-    const int c = u / per, lh = u % per, layer = lh / a.num_heads, head = lh % a.num_heads;
-    const int src = a.copies[3 * c], dst = a.copies[3 * c + 1], used = a.copies[3 * c + 2];
-    if (src >= a.num_pages || dst < 0 || dst >= a.num_pages || used <= 0) continue;
+  while (u < units) {
+    const int lh = u % per, layer = lh / a.num_heads, head = lh % a.num_heads;
+    if (src < a.num_pages && dst >= 0 && dst < a.num_pages && used > 0) {
+      int upto[4], all = 0;  // pieces up to the end of pool i's
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (!a.pools[i]) continue;
-      const int bytes = a.block_bytes[i], n = (used > kHalfPage ? bytes : bytes / 2) / 16;
-      char* pool = static_cast<char*>(a.pools[i]);
+      for (int i = 0; i < 4; ++i) {
+        all += a.pools[i] ? (used > kHalfPage ? a.block_bytes[i] : a.block_bytes[i] / 2) / 16 : 0;
+        upto[i] = all;
+      }
       const size_t layer0 = (size_t)layer * a.num_pages;
-      const u32x4_t* from = reinterpret_cast<const u32x4_t*>(pool + ((layer0 + src) * a.num_heads + head) * bytes);
-      u32x4_t* to = reinterpret_cast<u32x4_t*>(pool + ((layer0 + dst) * a.num_heads + head) * bytes);
-      for (int v = tid; v < n; v += 256) to[v] = from[v];
+      const size_t from = (layer0 + src) * a.num_heads + head, to = (layer0 + dst) * a.num_heads + head;
+      for (int v0 = tid; v0 < all; v0 += 256 * kFlight) {
+        u32x4_t piece[kFlight];
+        u32x4_t* at[kFlight];
+#pragma unroll
+        for (int k = 0; k < kFlight; ++k) {
+          const int v = min(v0 + 256 * k, all - 1);
+          const int i = (v >= upto[0]) + (v >= upto[1]) + (v >= upto[2]);
+          const int w = v - (i == 0 ? 0 : i == 1 ? upto[0] : i == 2 ? upto[1] : upto[2]);
+          char* pool = static_cast<char*>(i == 0 ? a.pools[0] : i == 1 ? a.pools[1] : i == 2 ? a.pools[2] : a.pools[3]);
+          const size_t bytes = (size_t)(i == 0 ? a.block_bytes[0] : i == 1 ? a.block_bytes[1] : i == 2 ? a.block_bytes[2] : a.block_bytes[3]);
+          piece[k] = reinterpret_cast<const u32x4_t*>(pool + from * bytes)[w];
+          at[k] = reinterpret_cast<u32x4_t*>(pool + to * bytes) + w;
+        }
+#pragma unroll
+        for (int k = 0; k < kFlight; ++k)
+          if (v0 + 256 * k < all) *at[k] = piece[k];
+      }
     }
+    u += gridDim.x;
+    if (u >= units) break;
+    const int c = 3 * (u / per);
+    src = a.copies[c];
+    dst = a.copies[c + 1];
+    used = a.copies[c + 2];
   }
 }
 
@@ -331,6 +359,7 @@ extern "C" int dtree_pages_fork(const DtreePagesFork* a, hipStream_t stream) {
   DTREE_REQUIRE(a->num_pages >= 1, "pages_fork: num_pages");
   DTREE_REQUIRE(a->ld_tables >= 1 && a->ld_tables <= (1 << 22), "pages_fork: ld_tables in [1, 2^22]");
   DTREE_REQUIRE(a->rows >= 0 && a->advance >= 0, "pages_fork: rows and advance not negative");
+  DTREE_REQUIRE(a->copies || a->rows == 0, "pages_fork: copies are needed where rows > 0");
   DTREE_REQUIRE(a->absent >= -1 && a->absent < a->num_pages, "pages_fork: absent is -1 or a page");
   DTREE_REQUIRE(a->tables != a->tables_out || !a->parents, "pages_fork: in place without parents alone");
   const int64_t rows = a->num_seqs;

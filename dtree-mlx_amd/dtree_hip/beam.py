@@ -147,17 +147,17 @@ class BeamDecoder:
         cache.max_past = eng.attn_grid_past(min(self.longest - self.max_new + self.made - 1, eng.max_past))
         advance = 0 if self.made == 1 else 1
         st = eng.stream_handle()
-        if self.use_graph:
-            N.check(eng.lib.dtree_graph_launch(C.c_void_p(self._graph(advance)), st), "graph launch")
+        if self.use_graph and advance:  # (the step behind the prompts is one of its kind)
+            N.check(eng.lib.dtree_graph_launch(C.c_void_p(self._graph()), st), "graph launch")
         else:
             self._launch_step(advance, st)
         cache.flip()
         self._record()
 
-    def _graph(self, advance: int) -> int:
+    def _graph(self) -> int:
         # (a graph holds the engine's buffers: those of its hidden layers may change)
         eng = self.eng
-        key = (self.cache.turn, self.cache.max_past, advance, tuple(eng.layer_ids), eng.hidden.data_ptr())
+        key = (self.cache.turn, self.cache.max_past, tuple(eng.layer_ids), eng.hidden.data_ptr())
         if key not in self._graphs:
             lib = eng.lib
             side = torch.cuda.Stream(device=eng.dev)
@@ -165,7 +165,7 @@ class BeamDecoder:
             N.check(lib.dtree_graph_begin(side.cuda_stream), "graph begin")
             ex = C.c_void_p()
             try:
-                self._launch_step(advance, side.cuda_stream)
+                self._launch_step(1, side.cuda_stream)
             except Exception:
                 lib.dtree_graph_end(side.cuda_stream, C.byref(ex))
                 raise

@@ -747,8 +747,8 @@ int dtree_beam_select(const DtreeBeamArgs* args, hipStream_t stream);
  * taken in ascending order, by ascending sequence, the copy's before the new ones.
  * Entries of tables outside [0, num_pages) count as absent.
  *
- * copies (optional) [num_seqs][3]: the page copies to make (dtree_pages_copy), by
- * ascending sequence: source, destination, positions in use (L % 64); the rest -1.
+ * copies [num_seqs][3] (optional with rows = 0, which copies nothing): the page copies
+ * to make (dtree_pages_copy), by ascending sequence: source, destination, positions in use (L % 64); the rest -1.
  * status (optional) [2]: the number of pages that were not to be had (none free, or
  * the table full) is added to the first word, and their entries are absent; the
  * second becomes the number of copies. refs change in place. tables_out may be

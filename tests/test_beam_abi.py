@@ -70,7 +70,7 @@ FORK = dict(refs=4096, num_pages=16, num_seqs=4, ld_tables=8, tables=1 << 16, ta
     (dict(lengths_out=None), "null"), (dict(num_seqs=0), "num_seqs"), (dict(num_seqs=1025), "num_seqs"),
     (dict(num_pages=0), "num_pages"), (dict(ld_tables=0), "ld_tables"), (dict(ld_tables=(1 << 22) + 1), "ld_tables"),
     (dict(num_seqs=1024, ld_tables=1 << 22), "entries"), (dict(rows=-1), "rows"), (dict(advance=-1), "rows"),
-    (dict(absent=-2), "absent"), (dict(absent=16), "absent"), (dict(tables_out=1 << 16), "in place"),
+    (dict(rows=1), "copies"), (dict(absent=-2), "absent"), (dict(absent=16), "absent"), (dict(tables_out=1 << 16), "in place"),
     (dict(tables_out=(1 << 16) + 64), "overlap"), (dict(lengths_out=4100), "overlap"),
 ])
 def test_fork_refusals(kw, word):
