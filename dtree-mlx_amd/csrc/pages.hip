@@ -9,7 +9,8 @@
 //
 // share  The entry of a sequence's parent into its new table, and its old table's pages'
 //        counts by (children - 1), or down by one past its length. Sequences with one
-//        child touch no count. A workgroup per (sequence, 1024 entries).
+//        child touch no count, and neighbours that hold a page change it together. A
+//        workgroup per 256 entries of a few sequences.
 // take   One workgroup, a thread per sequence: which page must be copied (held by others
 //        and about to be written), how many are needed, a prefix sum over the
 //        sequences. The free pages come from one pass over the counts in page order,
@@ -22,18 +23,19 @@
 // The copies are bound by their bytes, the tables by latency (four loads in a row: the
 // parent, its length, its page, the page's count). Measured: 8 sequences of 1020
 // positions, 36 layers of 8 heads of 128 in 8 bits: take 6.0 us, copy 6.5 (29 MB moved,
-// 4.5 TB/s), 13.1 together; 128 sequences of 4100, 8 layers of 4 heads of 256: share 3.8,
-// take 5.9, copy 13.4 (78 MB, 5.8 TB/s); 512 sequences of 32808: share 9.4 (264 000
-// entries, half of them change counts), take 9.1, copy 6.8. The share step within the
-// take workgroup (one launch fewer) pays up to about 8000 entries: 8448 entries took 34.7
-// us there in all and 28.6 in two launches.
+// 4.5 TB/s), 12.8 together; 128 sequences of 4100, 8 layers of 4 heads of 256: share 4,
+// take 6.0, copy 12.9 (78 MB, 6 TB/s); 512 sequences of 32808 (264 000 entries): share 6,
+// take 9.0, copy 6.3. The share step within the take workgroup (one launch fewer) pays up
+// to about 8000 entries: 8448 entries took 34.7 us there in all and 28.6 in two launches.
 #include "common.h"
 
 namespace dtree {
 namespace {
 
 constexpr int kMaxSeqs = 1024;
-constexpr int kShare = 1024;          // table entries of a share workgroup
+// Neighbouring sequences of a share workgroup: 512 sequences of 32808 positions take 21.1
+// us (24.4 with one, each by its own atomics), 20.6 with 8, 128 of 4100 25.5 and 26.5.
+constexpr int kSide = 4;
 constexpr int kTake = 1024, kTakeWaves = kTake / 64;
 constexpr int kOneLaunch = 8192;      // table entries that the take workgroup shares by itself (figures above)
 constexpr int kRun = 32;              // neighbouring counts of a thread in one round
@@ -54,9 +56,8 @@ __device__ __forceinline__ bool is_page(const DtreePagesFork& a, int page) {
   return page >= 0 && page < a.num_pages && page != a.absent;
 }
 
-// Entry e of sequence s: the new table's, and the old one's page's count. (SCOPE: an
-// agent's atomics are done behind the XCDs' caches, a lone workgroup's in its own.)
-template <int SCOPE>
+// Entry e of sequence s: the new table's, and the old one's page's count, by a lone
+// workgroup, whose atomics are done in its own cache (an agent's behind the XCDs').
 __device__ __forceinline__ void share_entry(const DtreePagesFork& a, int s, int e, int par, int take, int have, int children) {
   const int mine = a.tables[(size_t)s * a.ld_tables + e];
   int out = a.absent;
@@ -66,28 +67,51 @@ __device__ __forceinline__ void share_entry(const DtreePagesFork& a, int s, int 
   }
   a.tables_out[(size_t)s * a.ld_tables + e] = out;
   const int by = e < have ? children - 1 : -1;
-  if (by && is_page(a, mine)) __hip_atomic_fetch_add(a.refs + mine, by, __ATOMIC_RELAXED, SCOPE);
+  if (by && is_page(a, mine)) __hip_atomic_fetch_add(a.refs + mine, by, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
 }
 
+// A workgroup: 256 entries of kSide neighbouring sequences, a thread an entry of all of
+// them. Neighbours that hold one page there, as a prompt's hypotheses do, change its
+// count once, by the sum, which is often 0.
 __global__ __launch_bounds__(256) void pages_share_kernel(DtreePagesFork a) {
-  __shared__ int kids;
-  const int s = blockIdx.x, tid = threadIdx.x;
-  int children = 1;
-  if (a.parents) {
-    if (tid == 0) kids = 0;
-    __syncthreads();
-    int c = 0;
-    for (int i = tid; i < a.num_seqs; i += 256) c += a.parents[i] == s;
-    if (c) atomicAdd(&kids, c);
-    __syncthreads();
-    children = kids;
+  __shared__ int kids[kSide], from[kSide], have[kSide], take[kSide];
+  const int s0 = blockIdx.x * kSide, tid = threadIdx.x, e = blockIdx.y * 256 + tid;
+  if (tid < kSide) {
+    const int s = min(s0 + tid, a.num_seqs - 1), p = fork_parent(a, s);
+    kids[tid] = a.parents ? 0 : 1;
+    from[tid] = p;
+    have[tid] = (fork_length(a, s) + DTREE_PAGE - 1) / DTREE_PAGE;
+    take[tid] = p >= 0 ? (fork_length(a, p) + DTREE_PAGE - 1) / DTREE_PAGE : 0;
   }
-  const int par = fork_parent(a, s);
-  const int have = (fork_length(a, s) + DTREE_PAGE - 1) / DTREE_PAGE;
-  const int take = par >= 0 ? (fork_length(a, par) + DTREE_PAGE - 1) / DTREE_PAGE : 0;
-  const int end = min(a.ld_tables, (int)(blockIdx.y + 1) * kShare);
-  for (int e = blockIdx.y * kShare + tid; e < end; e += 256)
-    share_entry<__HIP_MEMORY_SCOPE_AGENT>(a, s, e, par, take, have, children);
+  __syncthreads();
+  if (a.parents) {
+    for (int i = tid; i < a.num_seqs; i += 256) {
+      const uint32_t k = (uint32_t)a.parents[i] - (uint32_t)s0;  // (no sequence: 2^31 or more)
+      if (k < kSide) atomicAdd(&kids[k], 1);
+    }
+    __syncthreads();
+  }
+  if (e >= a.ld_tables) return;
+  int mine[kSide], out[kSide];
+#pragma unroll
+  for (int j = 0; j < kSide; ++j) {  // (loads without branches go out together)
+    mine[j] = a.tables[(size_t)min(s0 + j, a.num_seqs - 1) * a.ld_tables + e];
+    out[j] = a.tables[(size_t)max(from[j], 0) * a.ld_tables + e];
+  }
+  int page = -1, by = 0;
+#pragma unroll
+  for (int j = 0; j < kSide; ++j) {
+    if (s0 + j >= a.num_seqs) break;
+    a.tables_out[(size_t)(s0 + j) * a.ld_tables + e] = e < take[j] && is_page(a, out[j]) ? out[j] : a.absent;
+    if (!is_page(a, mine[j])) continue;
+    if (mine[j] != page) {
+      if (by) atomicAdd(a.refs + page, by);
+      page = mine[j];
+      by = 0;
+    }
+    by += e < have[j] ? kids[j] - 1 : -1;
+  }
+  if (by) atomicAdd(a.refs + page, by);
 }
 
 // Inclusive prefix sum over a wave: within rows of 16, then from row to row.
@@ -185,7 +209,7 @@ __global__ __launch_bounds__(kTake) void pages_take_kernel(DtreePagesFork a) {
     for (int j = i; j < all; j += kTake) {
       const int s = (int)((j + 0.5f) * inv);  // (j < 8192: the half is far above the product's error)
       const int p = from[s];
-      share_entry<__HIP_MEMORY_SCOPE_WORKGROUP>(a, s, j - s * a.ld_tables, p, p >= 0 ? (size[p] + DTREE_PAGE - 1) / DTREE_PAGE : 0,
+      share_entry(a, s, j - s * a.ld_tables, p, p >= 0 ? (size[p] + DTREE_PAGE - 1) / DTREE_PAGE : 0,
                                                 (size[s] + DTREE_PAGE - 1) / DTREE_PAGE, kids[s]);
     }
     wait_stores_done();  // (the counts' changes too)
@@ -372,7 +396,7 @@ extern "C" int dtree_pages_fork(const DtreePagesFork* a, hipStream_t stream) {
   if (size <= kOneLaunch) {
     pages_take_kernel<true><<<1, kTake, 0, stream>>>(*a);
   } else {
-    const dim3 grid(a->num_seqs, (a->ld_tables + kShare - 1) / kShare);
+    const dim3 grid((a->num_seqs + kSide - 1) / kSide, (a->ld_tables + 255) / 256);
     pages_share_kernel<<<grid, 256, 0, stream>>>(*a);
     DTREE_LAUNCH_CHECK("pages_fork share launch");
     pages_take_kernel<false><<<1, kTake, 0, stream>>>(*a);
