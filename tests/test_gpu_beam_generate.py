@@ -102,6 +102,29 @@ def test_graphs_and_eager_steps_agree(gpu_device, family):
         assert [h[1] for h in hyps] == sorted((h[1] for h in hyps), reverse=True)
 
 
+@pytest.mark.parametrize("family,quant,max_nodes,groups,beams", [
+    ("qwen3", "q4", 32, 2, 6), ("qwen3_5", "q4", 32, 1, 4), ("qwen3", "bf16", 128, 3, 40), ("qwen3_5", "bf16", 64, 7, 9)])
+def test_quantised_targets_and_more_rows_than_a_block(gpu_device, family, quant, max_nodes, groups, beams):
+    target = load_target_model(tiny_qwen3() if family == "qwen3" else tiny_qwen35(), seed=0, max_past=300, norm_jitter=0.1,
+                               quant=quant, kv_bits=8)
+    m = target.model
+    target.model = type(m)(m.args, m.weights, max_past=300, max_nodes=max_nodes, kv_bits=8)
+    prompts = _prompts(target, [20 + 9 * g for g in range(groups)])
+    d = BeamDecoder(target, prompts, beams, 4)
+    d.start()
+    texts = [prompts[i // beams] + [t] for i, t in enumerate(d.tokens.tolist())]
+    for _ in range(3):
+        d.step()
+        torch.cuda.synchronize()
+        logits = target.model.engine.logits[:d.rows].double().cpu().numpy()
+        for i in range(0, d.rows, 5):
+            want = _alone(target, texts[i])
+            assert np.abs(logits[i] - want).max() <= TOL * np.abs(want).max(), (d.made, i)
+        texts = [texts[p] + [t] for p, t in zip(d.parents.tolist(), d.tokens.tolist())]
+    assert [prompts[g] + h.tokens for g, hyps in enumerate(d.hypotheses()) for h in hyps] == texts
+    d.release()
+
+
 def test_two_decoders_and_the_engines_own_steps_in_turns(gpu_device):
     """Decoders interleaved with each other, with verify steps and with a change of the
     engine's hidden layers (whose buffers a captured step holds)."""
