@@ -118,6 +118,10 @@ class BeamDecoder:
         """The prompts, one after another, and the first tokens."""
         if self.made:
             raise RuntimeError("the prompts have run: a decoder is used once")
+        with torch.cuda.device(self.scores.device):
+            self._start()
+
+    def _start(self) -> None:
         eng, cache = self.eng, self.cache
         cache.pool.start([len(p) for p in self.prompts])
         first = torch.empty(self.groups, eng.cfg.vocab_size, dtype=torch.float32, device=eng.dev)
@@ -140,9 +144,13 @@ class BeamDecoder:
 
     def step(self) -> None:
         """One token of every hypothesis that goes on."""
-        eng, cache = self.eng, self.cache
         if not 1 <= self.made < self.max_new:
             raise RuntimeError("start() comes first, and max_new_tokens bounds the steps")
+        with torch.cuda.device(self.scores.device):
+            self._step()
+
+    def _step(self) -> None:
+        eng, cache = self.eng, self.cache
         # a hypothesis is as long as its prompt and the tokens that it has fed
         cache.max_past = eng.attn_grid_past(min(self.longest - self.max_new + self.made - 1, eng.max_past))
         advance = 0 if self.made == 1 else 1

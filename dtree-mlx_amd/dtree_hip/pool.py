@@ -122,8 +122,9 @@ class PagedKVPool:
         if rows < 0 or max(new) + rows > self.capacity:
             raise ValueError(f"{max(new)} positions and {rows} rows exceed the capacity of {self.capacity}")
         lengths = torch.tensor(old, dtype=torch.int32, device=self.device)
-        self.launch_fork(self.turn, lengths.data_ptr(), lengths.data_ptr(), None if src is None else src.data_ptr(), rows,
-                         0, torch.cuda.current_stream(self.device).cuda_stream)
+        with torch.cuda.device(self.refs.device):
+            self.launch_fork(self.turn, lengths.data_ptr(), lengths.data_ptr(), None if src is None else src.data_ptr(), rows,
+                             0, torch.cuda.current_stream().cuda_stream)
         if src is not None:
             self.turn = 1 - self.turn
         self._lengths = new
