@@ -52,6 +52,9 @@ constexpr int kMaxVocab = 1 << 20;
 constexpr int kPickThreads = 512, kPickWaves = kPickThreads / 64;
 constexpr int kKeep = 2 * kMaxSelect;  // survivors of a level
 constexpr float kBig = 3.40282347e38f;
+// Maxima below which c = max log2 e, rounded, is within 1/16 of it, and 2^(its error) is a
+// harmless factor of a sum. (An error grows with the maximum: 440 at 1e10.)
+constexpr float kNear = 1048576.f;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct BeamParams {
@@ -184,7 +187,7 @@ __global__ __launch_bounds__(256) void beam_scan_kernel(BeamParams p) {
     mx = fmaxf(fmaxf(wm[turn][0], wm[turn][1]), fmaxf(wm[turn][2], wm[turn][3]));
     const float base = fmaxf(mx, -kBig);
     float sum = 0.f;
-    if (fabsf(base) < 1e30f) {
+    if (fabsf(base) < kNear) {
       // one operation an exponent: x log2 e - c, c = base log2 e rounded, whose rounding
       // is a factor of the whole sum
       const float c = base * kLog2e;
@@ -193,7 +196,7 @@ __global__ __launch_bounds__(256) void beam_scan_kernel(BeamParams p) {
 #pragma unroll
         for (int e = 0; e < E; ++e) sum += fast_exp2(fmaf(x[i][e], kLog2e, -c));
       sum *= fast_exp2(-fmaf(base, kLog2e, -c));
-    } else {
+    } else {  // (the difference first, which no magnitude spoils)
 #pragma unroll
       for (int i = 0; i < NL; ++i)
 #pragma unroll
