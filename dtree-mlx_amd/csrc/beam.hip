@@ -722,7 +722,8 @@ extern "C" size_t dtree_beam_args_bytes(void) { return sizeof(DtreeBeamArgs); }
 
 extern "C" size_t dtree_beam_select_workspace_bytes(const DtreeBeamArgs* a) {
   if (beam_check(a)) return 0;
-  return (size_t)a->groups * a->beams * beam_chunks(a) * (sizeof(float2) + kSegs * sizeof(float));
+  const size_t bytes = (size_t)a->groups * a->beams * beam_chunks(a) * (kSegs * sizeof(float) + sizeof(float2));
+  return (bytes + 15) & ~(size_t)15;
 }
 
 extern "C" int dtree_beam_select(const DtreeBeamArgs* a, hipStream_t stream) {
@@ -746,8 +747,8 @@ extern "C" int dtree_beam_select(const DtreeBeamArgs* a, hipStream_t stream) {
   const size_t blocks = (size_t)a->groups * a->beams * p.chunks;
   p.run = blocks >= kPairs ? 2 : 1;
   const unsigned scans = (unsigned)((size_t)a->groups * a->beams * ((p.chunks + p.run - 1) / p.run));
-  p.part = static_cast<float2*>(a->workspace);
-  p.seg = reinterpret_cast<float*>(p.part + blocks);
+  p.seg = static_cast<float*>(a->workspace);  // (first: it is read 16 bytes at a time)
+  p.part = reinterpret_cast<float2*>(p.seg + blocks * kSegs);
   if (a->type == DTREE_T_BF16) {
     beam_scan_kernel<true><<<scans, 256, 0, stream>>>(p);
     DTREE_LAUNCH_CHECK("beam_select scan launch");
