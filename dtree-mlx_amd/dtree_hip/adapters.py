@@ -15,7 +15,7 @@ from typing import Any
 import numpy as np
 import torch
 
-from .cache import PagedKVCache, Qwen35Cache
+from .cache import PagedKVCache, Qwen35Cache, check_room
 from .config import QWEN3_4B, QWEN35_4B, Qwen35Config, Qwen3Config
 from .engine import Qwen3TreeEngine, ancestor_bitsets
 from .qwen35_engine import Qwen35TreeEngine
@@ -250,6 +250,7 @@ class Qwen3TargetAdapter(MLXTargetAdapter):
             return
         if any(i < 0 or i >= current for i in keep):
             raise IndexError(f"keep indices must lie in [0, {current})")
+        check_room(cache, past_length, current)
         eng = model.engine
         eng.set_step([0] * current, [0] * current, [-1] + [0] * (current - 1), past_length, aux=True, accepted=keep)
         eng.launch_compact(cache, eng.stream_handle(), select_hidden=False, aux=True)

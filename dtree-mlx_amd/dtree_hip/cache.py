@@ -53,6 +53,18 @@ def v_block_index(head_dim: int) -> torch.Tensor:
     return _block_index(head_dim, "v")
 
 
+def check_room(cache, start: int, rows: int) -> None:
+    """Raises if positions start .. start + rows - 1 are not all the cache's own to write:
+    ``room`` (first, end) bounds them in a pool's sequence (PagedKVPool), whose other
+    positions are shared or have no page. Any other cache is its own throughout."""
+    room = getattr(cache, "room", None)
+    if room is not None and not room[0] <= start <= start + rows <= room[1]:
+        raise ValueError(f"positions {start} .. {start + rows - 1} of a pool's sequence, which has room at "
+                         f"{room[0]} .. {room[1] - 1} alone (fork the pool with rows)" if room[0] < room[1] else
+                         f"positions {start} .. {start + rows - 1} of a pool's sequence, which has no room (fork the "
+                         f"pool with rows)")
+
+
 class LayerCacheView:
     """Per-layer handle with the fields the reference runtime reads (offset)."""
 
@@ -74,6 +86,8 @@ class LayerCacheView:
 
 
 class PagedKVCache:
+    room: tuple[int, int] | None = None  # check_room
+
     def __init__(self, layers: int, kv_heads: int, head_dim: int, capacity: int, device="cuda",
                  page_order: torch.Tensor | None = None):
         self.layers = layers
@@ -137,6 +151,7 @@ class PagedKVCache:
         T = keys.shape[0]
         if start + T > self.capacity:
             raise ValueError("cache capacity exceeded")
+        check_room(self, start, T)
         dev = self.k_pages.device
         keys = keys.to(dev, torch.bfloat16)
         values = values.to(dev, torch.bfloat16)
@@ -189,6 +204,7 @@ class PagedKVCacheQ8:
 
     ``offset`` is the committed length of a single sequence, as PagedKVCache's.
     """
+    room: tuple[int, int] | None = None  # check_room
 
     def __init__(self, layers: int, kv_heads: int, head_dim: int, capacity: int, num_seqs: int = 1, device="cuda",
                  page_order: torch.Tensor | None = None):
@@ -282,6 +298,7 @@ class PagedKVCacheQ8:
         T = keys.shape[0]
         if start + T > self.capacity:
             raise ValueError("cache capacity exceeded")
+        check_room(self, start, T)
         dev = self.k_pages.device
         pos = torch.arange(start, start + T, device=dev)
         page = self.page_table[seq].long()[pos // PAGE]

@@ -23,7 +23,7 @@ import numpy as np
 import torch
 
 from . import _native as N
-from .cache import PagedKVCache, PagedKVCacheQ8
+from .cache import PagedKVCache, PagedKVCacheQ8, check_room
 from .config import Qwen3Config
 from .pool import HypothesisCache, PagedKVPool
 from .weights import W_TILED, W_TILED_F16, Q4Linear, Qwen3Weights, tile_weight, tile_weight_f16
@@ -193,6 +193,7 @@ class TreeEngineBase:
         self.result_host = torch.zeros(4 + 2 * N.MAX_NODES, dtype=torch.int32).pin_memory()
         self._result_np = self.result_host.numpy()
         self._step_past = 0  # P of the step the descriptor holds (host copy)
+        self._step_rows = 1  # and its nodes, or as many as it may have
         self._graphs: dict = {}
         self._dead_graphs: list = []
         self._tree_ws = None
@@ -240,7 +241,7 @@ class TreeEngineBase:
                                 else (self.desc_pinned, self.desc, self._desc_event, self._desc_rec))
         ev.synchronize()  # the previous upload from this pinned buffer has finished
         if not aux:
-            self._step_past = int(past_length)
+            self._step_past, self._step_rows = int(past_length), L
         rec["past_length"] = int(past_length)
         rec["num_nodes"] = L
         rec["n_accepted"] = 0 if accepted is None else len(accepted)
@@ -468,6 +469,10 @@ class TreeEngineBase:
         if self.kv_bits == 8 and kv.num_seqs != 1:
             raise ValueError("the engines verify one sequence: the cache must have num_seqs 1")
 
+    def _check_room(self, cache) -> None:
+        """The step's rows are the cache's to write."""
+        check_room(getattr(cache, "kv", cache), self._step_past, self._step_rows)
+
     def _attention_q8(self, lw, kv: PagedKVCacheQ8, rec: N.KvQ8, a: N.AttnQ8Args, qkv: torch.Tensor,
                       ws: torch.Tensor | None, st: int) -> None:
         """Append the rows' K / V, then attend (qkv rows are [q heads | k heads | v heads])."""
@@ -620,7 +625,7 @@ class TreeEngineBase:
                 self._tree_ws = torch.zeros(need, dtype=torch.uint8, device=self.dev)
             ws_ptr, ws_bytes = self._tree_ws.data_ptr(), self._tree_ws.numel()
         self._desc_event.synchronize()  # no host upload into the descriptor is still in flight
-        self._step_past = int(past_length)
+        self._step_past, self._step_rows = int(past_length), 1 + (budget if D > 0 else 0)
         N.check(self.lib.dtree_tree_build(x.data_ptr(), V, D, V, k, budget, int(root_token), int(past_length),
                                           ws_ptr, ws_bytes, self.desc.data_ptr(), self.tree_out.data_ptr(), None,
                                           None, st), "tree build")
@@ -758,6 +763,7 @@ class TreeEngineBase:
             self.lib.dtree_graph_destroy(C.c_void_p(self._dead_graphs.pop()))
 
     def graph_launch(self, cache: PagedKVCache, st: int) -> None:
+        self._check_room(cache)
         g = self._graph_for(cache)
         N.check(self.lib.dtree_graph_launch(C.c_void_p(g), st), "graph launch")
 
@@ -860,6 +866,7 @@ class Qwen3TreeEngine(TreeEngineBase):
             self._check_kv(cache)
             if cache.capacity < self.max_past + self.max_nodes:
                 raise ValueError("cache capacity is smaller than max_past + max_nodes")
+            self._check_room(cache)
         emb, emb_layout, emb_sb = self._embedding()
         N.check(self.lib.dtree_embed(
             (cache.desc if isinstance(cache, HypothesisCache) else self.desc).data_ptr(), emb, emb_layout, emb_sb, c.vocab_size, H,
@@ -946,6 +953,7 @@ class Qwen3TreeEngine(TreeEngineBase):
         if cache.offset + len(toks) > self.max_past:
             raise ValueError(f"prefill of {len(toks)} tokens beyond max_past {self.max_past}")
         self._check_kv(cache)
+        check_room(cache, cache.offset, len(toks))
         st = self.stream_handle()
         emb, emb_layout, emb_sb = self._embedding()
         slot = {li: i for i, li in enumerate(self.layer_ids)}

@@ -39,6 +39,10 @@ class PagedKVPool:
     copies   [num_seqs, 3] int32, status [2] int32: dtree_pages_fork's
     lengths  the sequences' positions on the host, as the last fork left them or
              ``sequence(i).offset`` has moved them since
+
+    A sequence may be written where its pages are its own (``sequence(i).room``, (first,
+    end) positions): behind ``start`` on its first lengths[i], behind a fork on the rows
+    asked for, from the page of the fork's length on. The engines refuse steps elsewhere.
     """
 
     def __init__(self, layers: int, kv_heads: int, head_dim: int, capacity: int, num_seqs: int,
@@ -73,6 +77,7 @@ class PagedKVPool:
         self.status = torch.zeros(2, **i32)
         self.turn = 0
         self._lengths = [0] * num_seqs
+        self._rooms = [(0, 0)] * num_seqs
         self._sequences: dict[int, PagedKVCache | PagedKVCacheQ8] = {}
 
     @property
@@ -121,7 +126,10 @@ class PagedKVPool:
             new = [old[p] if p >= 0 else 0 for p in par]
         if rows < 0 or max(new) + rows > self.capacity:
             raise ValueError(f"{max(new)} positions and {rows} rows exceed the capacity of {self.capacity}")
+        if any(n > end for n, (_, end) in zip(old, self._rooms)):
+            raise ValueError("a sequence's offset lies behind the positions that it has pages for")
         lengths = torch.tensor(old, dtype=torch.int32, device=self.device)
+        self._set_rooms([(0, 0)] * self.num_seqs)
         with torch.cuda.device(self.refs.device):
             self.launch_fork(self.turn, lengths.data_ptr(), lengths.data_ptr(), None if src is None else src.data_ptr(), rows,
                              0, torch.cuda.current_stream().cuda_stream)
@@ -132,6 +140,12 @@ class PagedKVPool:
             c.offset = new[i]
             c.page_table.view(-1).copy_(self.table[i])
         self.check()
+        self._set_rooms([(n // PAGE * PAGE, _pages(n + rows) * PAGE) if rows else (n, n) for n in new])
+
+    def _set_rooms(self, rooms: list[tuple[int, int]]) -> None:
+        self._rooms = rooms
+        for i, c in self._sequences.items():
+            c.room = rooms[i]
 
     def check(self) -> None:
         """Raises if a fork since the last check found no page (waits for the stream)."""
@@ -158,6 +172,7 @@ class PagedKVPool:
         self.refs.copy_(refs)
         self.status.zero_()
         self._lengths = [0] * self.num_seqs
+        self._set_rooms([(0, _pages(n) * PAGE) for n in need])
         for i, c in self._sequences.items():
             c.offset = 0
             c.page_table.view(-1).copy_(self.table[i])
@@ -178,13 +193,14 @@ class PagedKVPool:
     def sequence(self, i: int):
         """Sequence i as the engines take a cache. It follows the pool's forks: its page
         table and offset are those of sequence i after each. Its rows need room
-        (``fork(..., rows=n)``) before an engine writes them."""
+        (``fork(..., rows=n)``) before an engine writes them: a step whose rows would lie
+        in pages that other sequences hold, or in none, is refused."""
         if not 0 <= i < self.num_seqs:
             raise IndexError(i)
         if i not in self._sequences:
             row = self.table[i].clone()
             c = self._cache(row[None] if self.kv_bits == 8 else row, 1)
-            c.offset = self._lengths[i]
+            c.offset, c.room = self._lengths[i], self._rooms[i]
             self._sequences[i] = c
         return self._sequences[i]
 

@@ -30,7 +30,7 @@ import ctypes as C
 import torch
 
 from . import _native as N
-from .cache import Qwen35Cache
+from .cache import Qwen35Cache, check_room
 from .engine import TreeEngineBase
 from .pool import HypothesisCache
 from .weights import W_TILED, W_TILED_F16, GdnLayerWeights
@@ -152,6 +152,7 @@ class Qwen35TreeEngine(TreeEngineBase):
             self._check_kv(cache.kv)
             if cache.capacity < self.max_past + self.max_nodes:
                 raise ValueError("cache capacity is smaller than max_past + max_nodes")
+            self._check_room(cache)
         emb, emb_layout, emb_sb = self._embedding()
         N.check(self.lib.dtree_embed(
             (cache.desc if isinstance(cache, HypothesisCache) else self.desc).data_ptr(), emb, emb_layout, emb_sb, c.vocab_size, H,
@@ -326,6 +327,7 @@ class Qwen35TreeEngine(TreeEngineBase):
         if cache.offset + len(toks) > self.max_past:
             raise ValueError(f"prefill of {len(toks)} tokens beyond max_past {self.max_past}")
         self._check_kv(cache.kv)
+        check_room(cache.kv, cache.offset, len(toks))
         st = self.stream_handle()
         emb, emb_layout, emb_sb = self._embedding()
         slot = {li: i for i, li in enumerate(self.layer_ids)}
