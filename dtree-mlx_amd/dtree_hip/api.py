@@ -104,26 +104,31 @@ class DFlashGenerator:
                              tree_budget: int | None = None, verify_mode: str = "parallel-replay",
                              verify_chunk_size: int = 4, reset_peak_memory: bool = True,
                              skip_special_tokens: bool = False, profile: bool = False, num_beams: int = 4,
-                             length_penalty: float = 1.0) -> DFlashResult:
+                             length_penalty: float = 1.0, stop_token_ids=None) -> DFlashResult:
+        """``stop_token_ids``: the tokens that end the answer, the tokenizer's by
+        default; decode_mode "beam" takes one at most."""
+        stops = self.target.stop_token_ids() if stop_token_ids is None else {int(t) for t in stop_token_ids}
         if reset_peak_memory and torch.cuda.is_available():
             torch.cuda.reset_peak_memory_stats()
         if decode_mode == "dflash":
             output_tokens, metrics = dflash_generate(
                 target=self.target, draft=self.draft, prompt_tokens=prompt_tokens, max_new_tokens=max_new_tokens,
-                temperature=temperature, stop_token_ids=self.target.stop_token_ids(), layer_ids=self._layer_ids(),
+                temperature=temperature, stop_token_ids=stops, layer_ids=self._layer_ids(),
                 speculative_tokens=speculative_tokens, verify_mode=verify_mode,
                 verify_chunk_size=verify_chunk_size, profile=profile)
         elif decode_mode == "dtree":
             output_tokens, metrics = dtree_generate(
                 target=self.target, draft=self.draft, prompt_tokens=prompt_tokens, max_new_tokens=max_new_tokens,
-                temperature=temperature, stop_token_ids=self.target.stop_token_ids(), layer_ids=self._layer_ids(),
+                temperature=temperature, stop_token_ids=stops, layer_ids=self._layer_ids(),
                 speculative_tokens=speculative_tokens, tree_budget=tree_budget, verify_mode=verify_mode,
                 profile=profile)
         elif decode_mode == "beam":
             # beam search of the target alone (no drafter): the best of num_beams hypotheses
+            if len(stops) > 1:
+                raise ValueError(f"the stop tokens are {sorted(stops)}: beam search takes one (stop_token_ids={{id}})")
             prompt = [int(t) for t in torch.as_tensor(prompt_tokens).reshape(-1).tolist()]
             (best,), metrics = beam_generate(self.target, [prompt], num_beams=num_beams, max_new_tokens=max_new_tokens,
-                                             length_penalty=length_penalty)
+                                             stop_token_ids=stops, length_penalty=length_penalty)
             output_tokens = prompt + best[0].tokens
             metrics["hypotheses"] = best
         else:
@@ -138,13 +143,13 @@ class DFlashGenerator:
                  speculative_tokens: int | None = None, decode_mode: str = "dflash", tree_budget: int | None = None,
                  verify_mode: str = "parallel-replay", verify_chunk_size: int = 4, reset_peak_memory: bool = True,
                  skip_special_tokens: bool = False, profile: bool = False, num_beams: int = 4,
-                 length_penalty: float = 1.0) -> DFlashResult:
+                 length_penalty: float = 1.0, stop_token_ids=None) -> DFlashResult:
         return self.generate_from_tokens(
             prompt_tokens=self.encode_prompt(prompt_text), max_new_tokens=max_new_tokens, temperature=temperature,
             speculative_tokens=speculative_tokens, decode_mode=decode_mode, tree_budget=tree_budget,
             verify_mode=verify_mode, verify_chunk_size=verify_chunk_size, reset_peak_memory=reset_peak_memory,
             skip_special_tokens=skip_special_tokens, profile=profile, num_beams=num_beams,
-            length_penalty=length_penalty)
+            length_penalty=length_penalty, stop_token_ids=stop_token_ids)
 
 
 # Method-agnostic alias (api.py:170).
