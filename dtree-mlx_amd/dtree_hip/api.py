@@ -106,7 +106,7 @@ class DFlashGenerator:
                              skip_special_tokens: bool = False, profile: bool = False, num_beams: int = 4,
                              length_penalty: float = 1.0, stop_token_ids=None) -> DFlashResult:
         """``stop_token_ids``: the tokens that end the answer, the tokenizer's by
-        default; decode_mode "beam" takes one at most."""
+        default; decode_mode "beam" takes one at most, and is without sampling."""
         stops = self.target.stop_token_ids() if stop_token_ids is None else {int(t) for t in stop_token_ids}
         if reset_peak_memory and torch.cuda.is_available():
             torch.cuda.reset_peak_memory_stats()
@@ -124,6 +124,8 @@ class DFlashGenerator:
                 profile=profile)
         elif decode_mode == "beam":
             # beam search of the target alone (no drafter): the best of num_beams hypotheses
+            if temperature:
+                raise ValueError(f"temperature {temperature}: beam search takes the best tokens and samples none")
             if len(stops) > 1:
                 raise ValueError(f"the stop tokens are {sorted(stops)}: beam search takes one (stop_token_ids={{id}})")
             prompt = [int(t) for t in torch.as_tensor(prompt_tokens).reshape(-1).tolist()]

@@ -60,3 +60,9 @@ def test_the_other_modes_take_any_number(generator, monkeypatch, mode):
     generator.generate_from_tokens([1], decode_mode=mode)
     generator.generate_from_tokens([1], decode_mode=mode, stop_token_ids=[4, 5, 6])
     assert got == [{7, 9}, {4, 5, 6}]
+
+
+def test_a_temperature_is_refused(generator):
+    with pytest.raises(ValueError, match="temperature"):
+        generator.generate("a", decode_mode="beam", temperature=0.7, stop_token_ids=[7])
+    assert not generator.calls
