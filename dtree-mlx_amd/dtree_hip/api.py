@@ -131,6 +131,8 @@ class DFlashGenerator:
             prompt = [int(t) for t in torch.as_tensor(prompt_tokens).reshape(-1).tolist()]
             (best,), metrics = beam_generate(self.target, [prompt], num_beams=num_beams, max_new_tokens=max_new_tokens,
                                              stop_token_ids=stops, length_penalty=length_penalty)
+            if not best:
+                raise RuntimeError("no token continues the prompt: the target's logits hold no number above -inf")
             output_tokens = prompt + best[0].tokens
             metrics["hypotheses"] = best
         else:

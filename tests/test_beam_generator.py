@@ -66,3 +66,9 @@ def test_a_temperature_is_refused(generator):
     with pytest.raises(ValueError, match="temperature"):
         generator.generate("a", decode_mode="beam", temperature=0.7, stop_token_ids=[7])
     assert not generator.calls
+
+
+def test_no_continuation(generator):
+    generator.found = []
+    with pytest.raises(RuntimeError, match="no token continues"):
+        generator.generate("a", decode_mode="beam", stop_token_ids=[7])

@@ -1,4 +1,4 @@
-"""The generator's beam mode with a tokenizer of two end tokens."""
+"""The generator's beam mode with a tokenizer of two end tokens, and logits without a number."""
 import pytest
 
 from dtree_hip.adapters import load_target_model
@@ -33,3 +33,11 @@ def test_a_tokenizer_with_two_end_tokens(gpu_device, family):
     res = gen.generate("a prompt of some characters", max_new_tokens=12, decode_mode="beam", num_beams=1, stop_token_ids={end})
     assert res.generated_tokens == free[:free.index(end) + 1]
     assert res.metrics["hypotheses"][0].finished and res.text == ",".join(map(str, res.generated_tokens))
+
+
+def test_logits_of_nan(gpu_device):
+    target = load_target_model(tiny_qwen3(), seed=0, max_past=200, kv_bits=8)
+    target.model.weights.final_norm.fill_(float("nan"))
+    gen = DFlashGenerator(target_model=target, draft_model=object())
+    with pytest.raises(RuntimeError, match="no token continues"):
+        gen.generate_from_tokens([5, 6, 7], max_new_tokens=4, decode_mode="beam", num_beams=3)
