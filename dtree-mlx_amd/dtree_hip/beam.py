@@ -165,6 +165,7 @@ class BeamDecoder:
     def _graph(self) -> int:
         # (a graph holds the engine's buffers: those of its hidden layers may change)
         eng = self.eng
+        eng._destroy_pending()
         key = (self.cache.turn, self.cache.max_past, tuple(eng.layer_ids), eng.hidden.data_ptr())
         if key not in self._graphs:
             lib = eng.lib
@@ -216,10 +217,10 @@ class BeamDecoder:
             self._graphs.clear()
 
     def __del__(self):
-        try:
-            self.release()
-        except Exception:
-            pass
+        # (may run at any point, during a capture too: the engine destroys them at a launch)
+        graphs = self.__dict__.get("_graphs")
+        if graphs:
+            self.eng._dead_graphs.extend(graphs.values())
 
 
 def beam_generate(target, prompts, num_beams: int = 4, max_new_tokens: int = 256, stop_token_ids=None, pad_token: int = 0,
