@@ -26,7 +26,9 @@
 // 4.5 TB/s), 12.8 together; 128 sequences of 4100, 8 layers of 4 heads of 256: share 4,
 // take 6.0, copy 12.9 (78 MB, 6 TB/s); 512 sequences of 32808 (264 000 entries): share 6,
 // take 9.0, copy 6.3. The share step within the take workgroup (one launch fewer) pays up
-// to about 8000 entries: 8448 entries took 34.7 us there in all and 28.6 in two launches.
+// to 4096 entries, us of a fork in one launch and in two: 8 sequences of 64 entries 5.6
+// and 7.9, of 129 5.7 and 7.7; 32 of 64 6.8 and 8.3; 24 of 129 7.1 to 7.5 and 8.4; 32 of
+// 129 8.3 to 8.7 and 8.4; 64 of 96 9.2 and 8.6; 128 of 64 11.7 and 8.7; 512 of 16 15.1 and 9.5.
 #include "common.h"
 
 namespace dtree {
@@ -37,7 +39,7 @@ constexpr int kMaxSeqs = 1024;
 // us (24.4 with one, each by its own atomics), 20.6 with 8, 128 of 4100 25.5 and 26.5.
 constexpr int kSide = 4;
 constexpr int kTake = 1024, kTakeWaves = kTake / 64;
-constexpr int kOneLaunch = 8192;      // table entries that the take workgroup shares by itself (figures above)
+constexpr int kOneLaunch = 4096;      // table entries that the take workgroup shares by itself (figures above)
 constexpr int kRun = 32;              // neighbouring counts of a thread in one round
 constexpr int kRound = kTake * kRun;
 constexpr int kList = 4096;           // free pages listed at a time
@@ -207,7 +209,7 @@ __global__ __launch_bounds__(kTake) void pages_take_kernel(DtreePagesFork a) {
     const int all = n * a.ld_tables;
     const float inv = 1.f / a.ld_tables;
     for (int j = i; j < all; j += kTake) {
-      const int s = (int)((j + 0.5f) * inv);  // (j < 8192: the half is far above the product's error)
+      const int s = (int)((j + 0.5f) * inv);  // (j < 4096: the half is far above the product's error)
       const int p = from[s];
       share_entry(a, s, j - s * a.ld_tables, p, p >= 0 ? (size[p] + DTREE_PAGE - 1) / DTREE_PAGE : 0,
                                                 (size[s] + DTREE_PAGE - 1) / DTREE_PAGE, kids[s]);
