@@ -8,12 +8,13 @@
 //
 // Two launches.
 //
-// scan   One pass over the logits, a workgroup per (row, 4096 logits) in registers:
-//        the chunk's maximum and sum of exp(x - max), and the maximum of each run of
-//        32 logits ("segment"). Bound by the logits' bytes: 244 MB of bf16 in 47 us (5.2
-//        TB/s; a copy on this card reaches 4.7, reads and writes together), 59 MB of fp32
-//        in 11 us, 1.2 MB in 3.5 us (latency). Loads past the caches: the pick kernel's
-//        code, partials and segments stay in them (20.0 against 21.2 us for the 59 MB).
+// scan   One pass over the logits, a workgroup per (row, 4096 logits; many of bf16 two
+//        in turn) in registers: the chunk's maximum and sum of exp(x - max), and the
+//        maximum of each run of 32 logits ("segment"). Bound by the logits' bytes: 244 MB
+//        of bf16 in 47 us (5.2 TB/s; a copy on this card reaches 4.7, reads and writes
+//        together), 59 MB of fp32 in 11 us, 1.2 MB in 3.5 us (latency). Loads past the
+//        caches: the pick kernel's code, partials and segments stay in them (20.0 against
+//        21.2 us for the 59 MB).
 // pick   A workgroup per group. rank grows with x inside a beam, so a selected token
 //        lies in one of the num_select best segments by their maxima, and such a
 //        segment in one of the num_select best units (chunks, or parts of them). The
@@ -41,11 +42,15 @@ namespace {
 constexpr int kChunk = 4096;           // logits of a scan workgroup
 constexpr int kSeg = 32;               // logits of a segment
 constexpr int kSegs = kChunk / kSeg;   // segments of a chunk
-// Chunks from which a scan workgroup takes two of a row, the second's loads in flight
-// during the first: eight times what the card holds at once (2048 workgroups). 32224
-// live chunks of bf16: 61 us for the selection by twos, 66 one by one, 64 by fours; 3876
-// chunks (fp32): 21.7 by twos, 20.0 one by one.
-constexpr int kPairs = 16384;
+// Chunks of bf16 (of all rows) from which a scan workgroup takes two of a row, the
+// second's loads in flight during the first: four times what the card holds at once (2048
+// workgroups). us of a selection, one by one and by twos: 4864 chunks 19.3 and 19.4 (21.3 and
+// 21.6 for 32 selected of 16 beams), 9728 26.7 and 26.3 (29.0 and 28.5), 16416 41.1 and 39.5,
+// 19456 42.3 and 39.9, 38912 73.9 and 67.3 (76.2 and 71.0). A chunk of fp32 has twice the
+// loads in flight by itself: 4864 chunks 23.4 and 24.5, 16384 53.0 and 55.5, 38912 114 and
+// 117, so it is taken alone (in the same loop: with one chunk a workgroup by construction
+// the compiler's order of the loads costs 1 us at 4864).
+constexpr int kPairs = 8192;
 constexpr int kMaxBeams = 64;
 constexpr int kMaxSelect = 64;
 constexpr int kMaxVocab = 1 << 20;
@@ -745,7 +750,7 @@ extern "C" int dtree_beam_select(const DtreeBeamArgs* a, hipStream_t stream) {
   p.a = *a;
   p.chunks = beam_chunks(a);
   const size_t blocks = (size_t)a->groups * a->beams * p.chunks;
-  p.run = blocks >= kPairs ? 2 : 1;
+  p.run = a->type == DTREE_T_BF16 && blocks >= kPairs ? 2 : 1;
   const unsigned scans = (unsigned)((size_t)a->groups * a->beams * ((p.chunks + p.run - 1) / p.run));
   p.seg = static_cast<float*>(a->workspace);  // (first: it is read 16 bytes at a time)
   p.part = reinterpret_cast<float2*>(p.seg + blocks * kSegs);

@@ -1,5 +1,5 @@
 """The forms that selections, forks and copies take at larger sizes: scans of two blocks of
-4096 logits a workgroup (16384 blocks and more in all rows), forks of more table entries
+4096 logits a workgroup (8192 blocks of bf16 and more in all rows), forks of more table entries
 than one workgroup shares by itself, copies of more units than there are workgroups."""
 import ctypes as C
 
@@ -27,12 +27,13 @@ def _logits(dev, n, V, dtype, seed):
 @pytest.mark.parametrize("G,K,M,V,dtype", [(86, 64, 5, 2 * CHUNK + 37, torch.float32),
                                            (28, 16, 32, 36 * CHUNK + 5, torch.bfloat16),
                                            (64, 64, 3, 4 * CHUNK, torch.bfloat16),
+                                           (43, 64, 5, 2 * CHUNK + 37, torch.bfloat16),
                                            (1025, 8, 8, 2 * CHUNK - 1, torch.float32)])
 def test_scans_of_two_blocks(gpu_device, G, K, M, V, dtype):
     """Against the selection in 64 bits, and bit for bit what the same groups give a few at
     a time, whose scans take the blocks one by one."""
     chunks = -(-V // CHUNK)
-    assert G * K * chunks >= 16384
+    assert G * K * chunks >= 8192
     n = G * K
     x = _logits(gpu_device, n, V, dtype, seed=V)
     x[5, CHUNK:] = float("-inf")   # rows whose later blocks hold nothing, or all of it
@@ -45,7 +46,7 @@ def test_scans_of_two_blocks(gpu_device, G, K, M, V, dtype):
     lengths = torch.randint(0, 9, (n,), generator=g)
     s = Select(gpu_device, G, K, M, V, x, scores, lengths, finished, eos=17, pad=3, penalty=0.7)
     out = s.run()
-    few = max(1, min(G // 3, 16383 // (K * chunks)))
+    few = max(1, min(G // 3, 8191 // (K * chunks)))
     for at in range(0, G, few):
         m = min(few, G - at)
         r = slice(at * K, (at + m) * K)
@@ -70,8 +71,8 @@ def test_scans_of_two_blocks(gpu_device, G, K, M, V, dtype):
         assert ((out["scores"][at:at + m].double() - exact).abs() <= LSE + 2.0 ** -24 * exact.abs()).all()
 
 
-# numbers of sequences that are and are no multiple of 4, tables on both sides of 8192
-# entries and of each power of two below it
+# numbers of sequences that are and are no multiple of 4, tables on both sides of 4096
+# entries and of its neighbours among the powers of two
 @pytest.mark.parametrize("seqs,ld", [(67, 130), (301, 33), (1023, 9), (5, 1700), (3, 2731), (2, 4096), (128, 65), (6, 86),
                                      (33, 32), (41, 50), (64, 64), (91, 45), (127, 64), (64, 128)])
 @pytest.mark.parametrize("absent", [-1, 0, 500])
