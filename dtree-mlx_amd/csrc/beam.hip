@@ -2,8 +2,10 @@
 // continuations by summed log-probability (the batched, several-hypotheses
 // counterpart of the greedy argmax of adapters.py:114-118).
 //
-// s(b, t) = score_b + (x_bt - lse_b), rank(b, t) = s / length^penalty, all in fp64:
-// two candidates of different beams that fp32 would round together are told apart.
+// s(b, t) = score_b + (x_bt - lse_b), rank(b, t) = s / length^penalty, in fp64, but for
+// the exponentials and their sums over 4096 logits (lse is within 64 2^-24 = 4e-6: |x - m|
+// 2^-23 of a term, log(V) 2^-23 on average, and the additions): two candidates that fp32
+// would round together are told apart.
 // Ties go to the lower beam, then the lower token.
 //
 // Two launches.
@@ -260,7 +262,7 @@ __device__ __forceinline__ float from_order(uint32_t o) {
   return __uint_as_float((o >> 31) ? o & 0x7fffffffu : ~o);
 }
 
-// ln s for s >= 1/2, within 1e-9 (the sums are good to 1e-7): s = 2^e m, m in [0.7,
+// ln s for s >= 1/2, within 1e-9 (the sums are good to 4e-6): s = 2^e m, m in [0.7,
 // 1.4], ln m = 2 atanh((m - 1) / (m + 1)). Little code: the kernel's own instructions
 // are part of its latency.
 __device__ __forceinline__ double ln_of(double s) {

@@ -695,8 +695,8 @@ int dtree_attention_q8(const DtreeKvQ8* kv, const DtreeAttnQ8Args* args, hipStre
  * a finished beam has one continuation, pad_token with its own score and length
  * (its logits are not read); a beam with the score -inf (or NaN) has none. The best
  * are those of the largest sum / max(length, 1)^length_penalty, ties to the lower
- * beam, then the lower token; sums and comparisons are fp64, lse is within about
- * 1e-7.
+ * beam, then the lower token; sums and comparisons are fp64, lse is within 4e-6
+ * (its terms are fp32; 2e-8 to 3e-7 measured on normal logits).
  *
  * Outputs, [groups][num_select], best first: the sum (fp32), the token, the parent
  * (its row r), and optionally its length, whether it is finished (its beam was, or
