@@ -26,6 +26,7 @@ def test_a_decoder_dies_during_a_capture(gpu_device):
         d.step()
     n = len(d._graphs)
     assert n >= 2 and not eng._dead_graphs
+    gc.collect()  # (whatever else is garbage, other tests' engines among it, goes before the capture)
     torch.cuda.synchronize()
     lib, side = N.lib(), torch.cuda.Stream()
     N.check(lib.dtree_graph_begin(side.cuda_stream), "begin")
