@@ -133,6 +133,7 @@ class BeamDecoder:
                 cache.windows[cache.turn, :, g].copy_(seq.windows)
                 cache.states[cache.turn, :, g].copy_(seq.states)
         cache.pool._sequences.clear()  # (the tables are the device's from here on)
+        cache.pool._set_rooms([(0, 0)] * self.rows)
         cache.positions.zero_()
         cache.positions[:self.groups].copy_(torch.tensor([len(p) for p in self.prompts], dtype=torch.int32))
         self._launch_select(first, 1, eng.stream_handle())

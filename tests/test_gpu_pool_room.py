@@ -4,6 +4,7 @@ import numpy as np
 import pytest
 import torch
 
+from dtree_hip import BeamDecoder
 from dtree_hip.adapters import load_target_model
 from dtree_hip.config import tiny_qwen3
 from dtree_hip.synthetic import make_tree, random_prefix
@@ -128,3 +129,14 @@ def test_pages_used_up_leave_no_room(gpu_device, kv_bits):
         pool.fork([0, 0], rows=1)
     pool.start([4])
     eng.prefill(a, [1, 2, 3, 4])
+
+
+def test_a_decoders_pages_are_its_own(gpu_device):
+    """Behind the prompts the device forks a decoder's pool: the host has no room in it."""
+    target = _target(8)
+    d = BeamDecoder(target, [[3, 4, 5]], 3, 6)
+    d.start()
+    for i in range(3):
+        with pytest.raises(ValueError, match="no room"):
+            target.model.engine.prefill(d.cache.pool.sequence(i), [1, 2])
+    d.step()
